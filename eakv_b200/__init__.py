@@ -86,6 +86,14 @@ SIGNATURES = {
     "eakv_cache_validate": (_I, [_P, _P]),
     "eakv_cache_dequantize_device": (_I, [_P, _I, _I, _I, _I, _P, _P]),
     "eakv_cache_dequantize": (_I, [_P, _I, _I, _I, _I, _P]),
+    "eakv_append_rotary": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
+    "eakv_extend_attention": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _I, _P, _P, _P, _c.c_size_t, _P]),
+    "eakv_extend_workspace": (_I, [_P, _I, _P, _I, _I, _I, _I, _c.POINTER(_c.c_size_t)]),
+    "eakv_cache_copy": (_I, [_P, _I, _I, _P, _I, _I, _P]),
+    "eakv_cache_fork": (_I, [_P, _I, _I, _c.POINTER(_P)]),
+    "eakv_cache_gather": (_I, [_P, _I, _P, _P, _c.c_int64, _c.c_int64, _I, _P]),
+    "eakv_cache_compact": (_I, [_P, _I, _P, _c.c_int64, _c.c_int64, _I, _P]),
+    "eakv_cache_read": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _c.c_int64, _P]),
     # eakv_nccl.h
     "eakv_nccl_version": (_I, []),
     "eakv_nccl_unique_id": (_I, [_P]),
@@ -236,6 +244,22 @@ class Cache:
                                                          pos_end, _ptr(d_out), stream),
                       "eakv_cache_dequantize_device")
 
+    # --- copies -----------------------------------------------------------------
+    def fork(self, n, max_seq_len=None):
+        """eakv_cache_fork: a new cache holding the first n positions."""
+        out = ctypes.c_void_p()
+        _check(lib().eakv_cache_fork(self.h, n, max_seq_len or self.max_seq_len, ctypes.byref(out)),
+               "eakv_cache_fork")
+        return Cache(_handle=out.value)
+
+    def compact(self, begin, index, stream=None):
+        """eakv_cache_compact: position begin + j becomes position index[..., j].
+        index: int32 device tensor [n], [heads, n] or [layers, heads, n] (a
+        size of 1 is shared)."""
+        index, ls, hs = _index(index, self)
+        return _check(lib().eakv_cache_compact(self.h, begin, _ptr(index), ls, hs, index.shape[-1],
+                                               stream), "eakv_cache_compact")
+
     # --- info ----------------------------------------------------------------
     @property
     def seq_len(self):
@@ -376,6 +400,187 @@ def decode_attention_partial(caches, d_queries, n_q_heads, pos_begin, pos_end, d
                                                       n_q_heads, pos_begin, pos_end,
                                                       _ptr(d_output), _ptr(d_lse), stream),
                   "eakv_decode_attention_partial")
+
+
+# --- several tokens per call ------------------------------------------------------
+EAKV_F32, EAKV_F16, EAKV_BF16 = 0, 1, 2
+_DTYPES = {"float32": EAKV_F32, "float16": EAKV_F16, "bfloat16": EAKV_BF16}
+
+
+class _Rows(ctypes.Structure):
+    """eakv_rows_t"""
+    _fields_ = [("data", _P), ("token_stride", _c.c_int64), ("head_stride", _c.c_int64), ("dtype", _I)]
+
+
+class _Rotary(ctypes.Structure):
+    """eakv_rotary_t"""
+    _fields_ = [("cos_table", _P), ("sin_table", _P), ("n_rows", _I), ("rot_dim", _I),
+                ("interleaved", _I), ("positions", _P), ("axis_stride", _c.c_int64), ("n_axes", _I),
+                ("sections", _I * 4)]
+
+
+def _dtype(x):
+    name = str(x.dtype).replace("torch.", "")
+    if name not in _DTYPES:
+        raise TypeError(f"float32, float16 or bfloat16 expected, got {x.dtype}")
+    return _DTYPES[name]
+
+
+def _on(x, cache, what):
+    """Refuses a tensor that is not on the cache's device."""
+    dev = getattr(x, "device", None)
+    if dev is not None and (dev.type != "cuda" or dev.index != cache.device):
+        raise ValueError(f"{what} is on {dev}, the cache on cuda:{cache.device}")
+    return x
+
+
+def _rows(x, cache, heads, tokens, what):
+    """eakv_rows_t of a tensor [tokens, heads, head_dim] whose last dim is contiguous."""
+    if x is None:
+        return None
+    if tuple(x.shape) != (tokens, heads, cache.head_dim):
+        raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(tokens, heads, cache.head_dim)}")
+    if x.stride(2) != 1:
+        raise ValueError(f"{what}: the last dim must be contiguous")
+    _on(x, cache, what)
+    return _Rows(x.data_ptr(), x.stride(0), x.stride(1), _dtype(x))
+
+
+def _ref(x):
+    return None if x is None else ctypes.byref(x)
+
+
+def _ints(values, n, what):
+    values = [int(v) for v in values]
+    if len(values) != n:
+        raise ValueError(f"{what}: {len(values)} entries for {n} caches")
+    return (_I * n)(*values)
+
+
+def _contiguous(x, cache, dtype, shape, what):
+    if str(x.dtype) != "torch." + dtype or not x.is_contiguous() or tuple(x.shape) != shape:
+        raise ValueError(f"{what}: a contiguous {dtype} tensor {shape} expected")
+    return _on(x, cache, what)
+
+
+def _index(index, cache):
+    """An int32 position list [n], [heads, n] or [layers, heads, n] and its
+    layer and head strides (0 where it is shared)."""
+    if str(index.dtype) != "torch.int32" or index.dim() not in (1, 2, 3) or index.stride(-1) not in (0, 1):
+        raise ValueError("index: an int32 tensor [n], [heads, n] or [layers, heads, n] expected")
+    if index.shape[-1] > 1 and index.stride(-1) != 1:
+        raise ValueError("index: the last dim must be contiguous")
+    x = index.reshape((1,) * (3 - index.dim()) + tuple(index.shape)) if index.dim() < 3 else index
+    if x.shape[0] not in (1, cache.n_layers) or x.shape[1] not in (1, cache.n_kv_heads):
+        raise ValueError(f"index: {tuple(index.shape)} for {cache.n_layers} layers, {cache.n_kv_heads} heads")
+    _on(index, cache, "index")
+    return x, (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+
+
+def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin=None,
+                  positions=None, sections=None, interleaved=False, stream=None):
+    """eakv_append_rotary. k, v: [total, n_kv_heads, head_dim] (any token and
+    head stride), q and q_out: [total, n_q_heads, head_dim] (q_out defaults to
+    q); counts[i] tokens of each cache, packed. cos, sin: f32 tables [rows,
+    rot_dim/2]; positions: int32 [axes, total] (or [total]); sections: pairs
+    that follow each axis. Without tables K goes in as it is."""
+    c, counts = caches[0], list(counts)
+    total = sum(counts)
+    if q is not None and q_out is None:
+        q_out = q
+    nq = q.shape[1] if q is not None else c.n_kv_heads
+    rk, rv = (_rows(x, c, c.n_kv_heads, total, n) for x, n in ((k, "k"), (v, "v")))
+    rq, ro = (_rows(x, c, nq, total, n) for x, n in ((q, "q"), (q_out, "q_out")))
+    rot = None
+    if cos is not None:
+        if positions.dim() == 1:
+            positions = positions[None]
+        if cos.dim() != 2 or cos.dtype != sin.dtype:
+            raise ValueError("cos, sin: f32 tables [rows, rot_dim/2] expected")
+        shape = tuple(cos.shape)
+        _contiguous(cos, c, "float32", shape, "cos")
+        _contiguous(sin, c, "float32", shape, "sin")
+        axes = positions.shape[0]
+        if (str(positions.dtype) != "torch.int32" or positions.dim() != 2 or axes > 4 or
+                positions.shape[1] != total or (total > 1 and positions.stride(1) != 1)):
+            raise ValueError(f"positions: int32 [1..4, {total}] expected")
+        _on(positions, c, "positions")
+        sections = list(sections) if sections is not None else [shape[1]]
+        if len(sections) != axes:
+            raise ValueError(f"{len(sections)} sections for {axes} axes")
+        rot = _Rotary(_ptr(cos), _ptr(sin), shape[0], 2 * shape[1], int(interleaved), _ptr(positions),
+                      positions.stride(0) if axes > 1 else 0, axes, (_I * 4)(*sections))
+    return _check(lib().eakv_append_rotary(_handles(caches), len(caches), layer,
+                                           _ints(counts, len(caches), "counts"), _ref(rk), _ref(rv),
+                                           _ref(rq), _ref(ro), nq, _ref(rot), stream),
+                  "eakv_append_rotary")
+
+
+def extend_workspace(caches, counts, dtype, n_q_heads, window=0, tree=False):
+    """Bytes of workspace eakv_extend_attention takes for this call; dtype is
+    EAKV_F32, EAKV_F16 or EAKV_BF16."""
+    out = ctypes.c_size_t()
+    _check(lib().eakv_extend_workspace(_handles(caches), len(caches),
+                                       _ints(counts, len(caches), "counts"), dtype, n_q_heads, window,
+                                       int(bool(tree)), ctypes.byref(out)), "eakv_extend_workspace")
+    return out.value
+
+
+def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=None, scale=0.0,
+                     workspace=None, stream=None):
+    """eakv_extend_attention. q, out: [total, n_q_heads, head_dim] (any token
+    and head stride); tree: int64 or uint64 [total] bit masks over the cache's
+    new tokens; lse: f32 [total, n_q_heads]; workspace: a uint8 tensor, zeroed
+    once, or None for the first cache's scratch."""
+    c, counts = caches[0], list(counts)
+    total, nq = sum(counts), q.shape[1]
+    rq, ro = _rows(q, c, nq, total, "q"), _rows(out, c, nq, total, "out")
+    if tree is not None:
+        kind = "uint64" if str(tree.dtype) == "torch.uint64" else "int64"
+        _contiguous(tree, c, kind, (total,), "tree")
+    if lse is not None:
+        _contiguous(lse, c, "float32", (total, nq), "lse")
+    size = 0
+    if workspace is not None:
+        size = workspace.numel()
+        _contiguous(workspace, c, "uint8", (size,), "workspace")
+    return _check(lib().eakv_extend_attention(_handles(caches), len(caches), layer,
+                                              _ints(counts, len(caches), "counts"), _ref(rq), _ref(ro),
+                                              nq, scale, window, _ptr(tree), _ptr(lse),
+                                              _ptr(workspace), size, stream),
+                  "eakv_extend_attention")
+
+
+def copy_positions(dsts, dst_pos, src, src_pos, n, stream=None):
+    """eakv_cache_copy: positions [src_pos, src_pos + n) of src to dst_pos.. of
+    every cache of dsts, whose seq_len becomes dst_pos + n."""
+    return _check(lib().eakv_cache_copy(_handles(dsts), len(dsts), dst_pos, src.h, src_pos, n, stream),
+                  "eakv_cache_copy")
+
+
+def gather_positions(dst, dst_pos, src, index, stream=None):
+    """eakv_cache_gather: position dst_pos + j of dst becomes position
+    index[..., j] of src. index: int32 [n], [heads, n] or [layers, heads, n]."""
+    index, ls, hs = _index(index, src)
+    return _check(lib().eakv_cache_gather(dst.h, dst_pos, src.h, _ptr(index), ls, hs, index.shape[-1],
+                                          stream), "eakv_cache_gather")
+
+
+def read_positions(caches, begins, counts, out, layer=0, stream=None):
+    """eakv_cache_read: the values of positions [begins[i], begins[i] +
+    counts[i]) of each cache, into out [layers, 2, total, n_kv_heads, head_dim]
+    (layers from `layer` on; K then V)."""
+    c, counts = caches[0], list(counts)
+    total = sum(counts)
+    if out.dim() != 5 or out.shape[1] != 2:
+        raise ValueError("out: [layers, 2, total, n_kv_heads, head_dim] expected")
+    if out.shape[0] == 0:
+        raise ValueError("out: no layers")
+    rk, rv = (_rows(out[0, i], c, c.n_kv_heads, total, "out") for i in (0, 1))
+    return _check(lib().eakv_cache_read(_handles(caches), len(caches), layer, out.shape[0],
+                                        _ints(begins, len(caches), "begins"),
+                                        _ints(counts, len(caches), "counts"), _ref(rk), _ref(rv),
+                                        out.stride(0), stream), "eakv_cache_read")
 
 
 def lse_combine(n_parts, n_rows, head_dim, d_parts, d_lse, d_output, d_lse_out=None,

@@ -18,6 +18,7 @@
 #define EAKV_CUDA_H
 
 #include <stddef.h>
+#include <stdint.h>
 #include "eakv.h"
 
 #ifdef __cplusplus
@@ -174,6 +175,132 @@ int eakv_cache_dequantize_device(const eakv_cache_t *cache, int layer, int kv_id
                                  int pos_end, float *d_out, void *stream);
 int eakv_cache_dequantize(const eakv_cache_t *cache, int layer, int kv_idx, int pos_begin,
                           int pos_end, float *out);
+
+/* ---- several tokens per call --------------------------------------------
+ *
+ * A model's layer loop over a batch of caches, with any number of new tokens
+ * per cache: append the layer's K and V (rotated and quantized in one
+ * launch), attend, and after the last layer advance (or keep only the
+ * accepted tokens with eakv_cache_compact). The tokens of a call are packed:
+ * cache 0's n_new[0] tokens first, then cache 1's, and so on; a count may be
+ * 0. The caches of a call share a shape and a device, n_caches <= 256,
+ * head_dim is 64 or 128. n_new and the other count arrays are host memory,
+ * read before the call returns. All calls are asynchronous on `stream`
+ * (NULL: the first cache's own stream) and can be captured into a graph,
+ * which keeps the counts and sequence lengths of the captured call. */
+
+/* Element types of device buffers. */
+#define EAKV_F32  0
+#define EAKV_F16  1
+#define EAKV_BF16 2
+
+/* Rows [token][head][head_dim] of a device buffer: element d of (token t,
+ * head h) is at data + t*token_stride + h*head_stride + d (strides in
+ * elements), so a slice of a fused q/k/v projection needs no copy. Rows that
+ * do not start on a 4-element boundary are read and written one element at a
+ * time. */
+typedef struct {
+    void     *data;
+    int64_t   token_stride;
+    int64_t   head_stride;
+    int       dtype;        /* EAKV_F32, EAKV_F16 or EAKV_BF16 */
+} eakv_rows_t;
+
+/* Rotary positions. The first rot_dim dims of a head (a multiple of 8) are
+ * rot_dim/2 pairs: (i, i + rot_dim/2), or (2i, 2i+1) when interleaved. Pair
+ * i of a token turns by the angle whose cosine and sine are at
+ * [position][i] of the f32 tables [n_rows][rot_dim/2], with the token's
+ * position on the axis that pair i follows: the first sections[0] pairs
+ * follow axis 0, the next sections[1] axis 1, and so on (one axis for text;
+ * time, height and width for images and video). positions is device
+ * int32[n_axes][total tokens], axis a at positions + a*axis_stride. */
+#define EAKV_MAX_AXES 4
+typedef struct {
+    const float   *cos_table;
+    const float   *sin_table;
+    int            n_rows;
+    int            rot_dim;
+    int            interleaved;
+    const int32_t *positions;
+    int64_t        axis_stride;
+    int            n_axes;
+    int            sections[EAKV_MAX_AXES];
+} eakv_rotary_t;
+
+/* Quantizes the new tokens' K and V rows of one layer into the pages of
+ * their caches, at positions seq_len .. seq_len + n_new - 1 (seq_len is not
+ * changed, as with eakv_cache_append), K turned by `rotary` first (NULL: not
+ * turned); and writes the turned q rows (n_q_heads heads; q NULL: none) to
+ * q_out, which may be q itself. k, v, q and q_out have one element type. The
+ * turned K is rounded once, to f32, and then quantized like
+ * eakv_cache_append's f32 input: the same groups, bit for bit. A token with a
+ * position outside the table sets status bit 2 (eakv_device_status) and its
+ * rows are not written. */
+int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, const int *n_new,
+                       const eakv_rows_t *k, const eakv_rows_t *v, const eakv_rows_t *q,
+                       const eakv_rows_t *q_out, int n_q_heads, const eakv_rotary_t *rotary,
+                       void *stream);
+
+/* Attention of the new tokens of one layer over the caches. Token t of cache
+ * i stands at position seq_len + t and attends positions 0 .. seq_len + t,
+ * its own and the earlier new tokens' among them (they are appended, and not
+ * yet advanced over); with window > 0 only the last `window` of those; with
+ * tree (device uint64[total tokens], n_new <= 64) of the new tokens exactly
+ * those j whose bit j is set in its word, within the window. Query head h reads KV
+ * head h / (n_q_heads / n_kv_heads). out gets softmax(scale q.k) v, scale
+ * 1/sqrt(head_dim) when given as 0; lse (device f32[total tokens][n_q_heads],
+ * or NULL) the natural-log log-sum-exp of the scaled scores. A token that
+ * attends nothing gets zeros and -inf. What is not attended has no influence,
+ * NaN among it. q and out have one element type; f32 runs on split operands
+ * that keep 22 bits, 16-bit types on 16-bit tensor-core operands with 32-bit
+ * sums. workspace (device, 16-byte aligned) holds the records of long rows'
+ * sequence splits: at least eakv_extend_workspace bytes, zeroed once before
+ * its first use, and not shared by calls that may overlap; NULL takes the
+ * first cache's scratch, which then must not be in use on another stream. A
+ * captured call takes a workspace of its own, since the scratch moves when a
+ * later call needs more of it. */
+int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int layer,
+                          const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
+                          int n_q_heads, float scale, int window, const uint64_t *tree, float *lse,
+                          void *workspace, size_t workspace_bytes, void *stream);
+/* Bytes of workspace that call needs (0: none). */
+int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const int *n_new,
+                          int dtype, int n_q_heads, int window, int tree, size_t *bytes);
+
+/* Copies positions [src_pos, src_pos + n) of every layer and head to
+ * [dst_pos, dst_pos + n) of n_dst other caches in one launch, as they are
+ * (nibbles, scales and biases), and sets their seq_len to dst_pos + n:
+ * dst_pos <= their seq_len, src_pos + n <= src's. The caches agree in layers,
+ * heads and head_dim; their max_seq_len may differ. n_dst <= 256. */
+int eakv_cache_copy(eakv_cache_t *const *dsts, int n_dst, int dst_pos, const eakv_cache_t *src,
+                    int src_pos, int n, void *stream);
+/* A new cache of max_seq_len positions on src's device with src's first n. Not
+ * for stream capture (it allocates). */
+int eakv_cache_fork(const eakv_cache_t *src, int n, int max_seq_len, eakv_cache_t **out);
+/* Position dst_pos + j of (layer l, KV head h) of dst becomes position
+ * index[l*layer_stride + h*head_stride + j] of src, j < n, for K and V; sets
+ * dst's seq_len to dst_pos + n. index is device int32; a stride of 0 shares
+ * one list between layers or heads. An index outside [0, src's seq_len) sets
+ * status bit 2 and leaves its position as it was. */
+int eakv_cache_gather(eakv_cache_t *dst, int dst_pos, const eakv_cache_t *src, const int32_t *index,
+                      int64_t layer_stride, int64_t head_stride, int n, void *stream);
+/* The same within one cache: position begin + j becomes index[..+ j], and
+ * seq_len begin + n; keeps a drafted branch, or evicts. index may reach up to
+ * max_seq_len (appended tokens not yet advanced over), and no entry is below
+ * its own place (index >= begin + j, as in every ascending list); one that is,
+ * sets status bit 2 and leaves its position as it was. */
+int eakv_cache_compact(eakv_cache_t *cache, int begin, const int32_t *index, int64_t layer_stride,
+                       int64_t head_stride, int n, void *stream);
+
+/* The values (nibble * scale + bias, rounded once to f32 and from there to the
+ * rows' type) of positions [begin[i], begin[i] + n[i]) of cache i, i <
+ * n_caches, for layers layer0 .. layer0 + n_layers - 1: rows packed like the
+ * tokens of eakv_append_rotary, K of layer l at k->data + l*layer_stride
+ * elements, V at v->data + the same (either may be NULL). Positions up to
+ * max_seq_len may be read. */
+int eakv_cache_read(const eakv_cache_t *const *caches, int n_caches, int layer0, int n_layers,
+                    const int *begin, const int *n, const eakv_rows_t *k, const eakv_rows_t *v,
+                    int64_t layer_stride, void *stream);
 
 /* ---- testing aid ------------------------------------------------------ */
 
