@@ -32,8 +32,12 @@ struct ExtendArgs {
   float *part_o, *part_m, *part_l;   // [item][split][row of the tile]..., see part_row
 };
 
+// The caches of one launch, all with new tokens.
 struct ExtendBatch {
-  TokenBatch t;
+  const uint8_t *base[kMaxBatch];
+  int old[kMaxBatch];        // position of the first new token
+  int first[kMaxBatch];      // its index in the packed rows
+  int n_new[kMaxBatch];
   int tile0[kMaxBatch + 1];  // first row tile of each cache, over one KV head
 };
 
@@ -65,9 +69,9 @@ __device__ __forceinline__ ExtItem extend_item(const ExtendArgs &a, const Extend
     else hi = mid - 1;
   }
   it.b = lo;
-  it.old = batch.t.pos[lo];
-  it.tok0 = batch.t.first[lo];
-  it.n_new = batch.t.first[lo + 1] - it.tok0;
+  it.old = batch.old[lo];
+  it.tok0 = batch.first[lo];
+  it.n_new = batch.n_new[lo];
   it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
   it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
   const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
@@ -77,7 +81,7 @@ __device__ __forceinline__ ExtItem extend_item(const ExtendArgs &a, const Extend
   it.all_hi = a.tree ? it.old : it.old + t_first + 1;
   const int P0 = it.lo / kPagePositions;
   const int P1 = (it.hi + kPagePositions - 1) / kPagePositions;
-  it.pg0 = P0 + it.split * a.split_pages;
+  it.pg0 = min(P0 + it.split * a.split_pages, P1);
   const int pg1 = min(P1, it.pg0 + a.split_pages);
   it.npages = pg1 > it.pg0 ? pg1 - it.pg0 : 0;
   return it;
@@ -192,5 +196,9 @@ constexpr int kExtendMmaRows = 16;
 int extend_mma_resident(int head_dim, int dtype);
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec,
                       cudaStream_t s);
+// extend_umma.cu: 16-bit types
+constexpr int kExtendUmmaRows = 256;
+int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec,
+                       cudaStream_t s);
 
 }  // namespace eakv

@@ -125,7 +125,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
     return;
   }
   const uint8_t *kpages =
-      batch.t.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
+      batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
   const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
 
   if (threadIdx.x == 0) {

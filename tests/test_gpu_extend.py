@@ -12,12 +12,23 @@ DT = {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}
 HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 
 
+# both kernels on every case: the library's choice (few rows: warp-level
+# kernel, many: tcgen05), or one of them for 16-bit types
+PATH = "auto"
+CODE = {"auto": 0, "mma": 2, "umma": 3}
+
+
 @pytest.fixture(autouse=True)
-def _reset():
+def _reset(request):
+    global PATH
+    PATH = request.node.callspec.params.get("path", "auto") if hasattr(request.node, "callspec") else "auto"
     E.force_splits(0)
+    E.force_path(CODE[PATH])
     yield
     E.force_splits(0)
+    E.force_path(0)
     E.test_stall(-1)
+    PATH = "auto"
 
 
 class Batch:
@@ -104,7 +115,7 @@ def limits(dtype, out, size, rows_per_head, longest):
     positions, at most `longest` / 64 steps per warp and 256 for the merge.
     Then half a step of the output's type."""
     vmean, reach = size
-    wide = dtype != "f32" and rows_per_head > 32
+    wide = dtype != "f32" and (PATH == "umma" or (PATH == "auto" and rows_per_head > 32))
     d = reach * (2.0 ** -16 + (3 * 2.0 ** -11 if wide else 0.0))
     w = (2.0 ** -22 if dtype == "f32" else 2.0 ** -11) + (3 * 2.0 ** -11 if wide else 0.0)
     w += (longest / 64 + 256) * 2.0 ** -23
@@ -165,9 +176,12 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+KINDS = [("f32", "auto"), ("f16", "auto"), ("bf16", "auto"), ("bf16", "mma"), ("bf16", "umma")]
+
+
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("hd,nq,nkv,old,new", CASES)
-def test_causal(gpu, hd, nq, nkv, old, new, dtype):
+def test_causal(gpu, hd, nq, nkv, old, new, dtype, path):
     rng = np.random.default_rng(hd + nq + sum(old))
     b = Batch(rng, 2, nkv, hd, old, new, size=max(x + y for x, y in zip(old, new)) + 5)
     q = rng.standard_normal((sum(new), nq, hd)).astype(np.float32)
@@ -176,11 +190,11 @@ def test_causal(gpu, hd, nq, nkv, old, new, dtype):
     b.free()
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 128, 300])
 @pytest.mark.parametrize("hd,nq,nkv,old,new", [(128, 8, 2, [500, 10], [3, 1]), (64, 8, 4, [200], [70]),
                                                (128, 4, 1, [131, 0], [100, 90])])
-def test_window(gpu, hd, nq, nkv, old, new, window, dtype):
+def test_window(gpu, hd, nq, nkv, old, new, window, dtype, path):
     rng = np.random.default_rng(window)
     b = Batch(rng, 1, nkv, hd, old, new)
     q = rng.standard_normal((sum(new), nq, hd)).astype(np.float32)
@@ -188,11 +202,11 @@ def test_window(gpu, hd, nq, nkv, old, new, window, dtype):
     b.free()
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("hd,nq,nkv,old,new", [(128, 8, 2, [0], [1]), (64, 8, 1, [100, 0], [13, 64]),
                                                (128, 8, 8, [61], [9]), (128, 32, 8, [63, 128], [64, 40])])
-def test_tree(gpu, hd, nq, nkv, old, new, window, dtype):
+def test_tree(gpu, hd, nq, nkv, old, new, window, dtype, path):
     """Random masks: tokens that attend none, one or all of the new tokens,
     later ones too; with no cached position a token may attend nothing."""
     rng = np.random.default_rng(hd + sum(new) + window)
@@ -210,9 +224,9 @@ def test_tree(gpu, hd, nq, nkv, old, new, window, dtype):
     b.free()
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("splits", [2, 3, 7, 50])
-def test_forced_splits_and_own_workspace(gpu, splits, dtype):
+def test_forced_splits_and_own_workspace(gpu, splits, dtype, path):
     """Splits of any length, with the cache's scratch and with a workspace of
     the caller's, three calls on it: the same bits each time."""
     import torch
@@ -233,9 +247,9 @@ def test_forced_splits_and_own_workspace(gpu, splits, dtype):
     b.free()
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("new", [[4], [150]])
-def test_what_is_not_attended_has_no_influence(gpu, new, dtype):
+def test_what_is_not_attended_has_no_influence(gpu, new, dtype, path):
     """NaN and infinities in later tokens, in a tree's siblings, before the
     window and behind the appended tokens leave the bits as they were; where
     they are attended, the outputs are NaN."""
@@ -294,11 +308,11 @@ def test_what_is_not_attended_has_no_influence(gpu, new, dtype):
     assert E.device_status(0) == 0
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,path", [k for k in KINDS if k[0] != "f16"])   # f16 holds no 1e20
 @pytest.mark.parametrize("n", [3, 160])
 @pytest.mark.parametrize("kscale,vscale,qscale", [(1, 1e-30, 1), (1, 1e30, 1), (1e-20, 1, 1e20), (1e20, 1, 1e-20),
                                                   (1, 1e4, 1e-6), (1, 1, 30.0)])
-def test_magnitudes(gpu, n, kscale, vscale, qscale, dtype):
+def test_magnitudes(gpu, n, kscale, vscale, qscale, dtype, path):
     """Values over 60 orders of magnitude, and V growing 2^14 along the sequence."""
     rng = np.random.default_rng(17)
     H, hd, nq, old = 2, 128, 8, 300
