@@ -182,6 +182,9 @@ class Cache:
             self.h = L.eakv_cache_create(n_layers, n_kv_heads, head_dim, max_seq_len)
             if not self.h:
                 raise EakvError(None, "eakv_cache_create")
+        # fixed for the cache's life: (layers, KV heads, head_dim, device)
+        self.shape = (L.eakv_cache_n_layers(self.h), L.eakv_cache_n_heads(self.h),
+                      L.eakv_cache_head_dim(self.h), L.eakv_cache_device(self.h))
 
     # --- lifecycle ---------------------------------------------------------
     def free(self):
@@ -419,18 +422,27 @@ class _Rotary(ctypes.Structure):
                 ("sections", _I * 4)]
 
 
+_names = {}   # torch dtype -> its name, filled as types are met
+
+
+def _name(x):
+    name = _names.get(x.dtype)
+    if name is None:
+        name = _names[x.dtype] = str(x.dtype).replace("torch.", "")
+    return name
+
+
 def _dtype(x):
-    name = str(x.dtype).replace("torch.", "")
-    if name not in _DTYPES:
+    code = _DTYPES.get(_name(x))
+    if code is None:
         raise TypeError(f"float32, float16 or bfloat16 expected, got {x.dtype}")
-    return _DTYPES[name]
+    return code
 
 
 def _on(x, cache, what):
     """Refuses a tensor that is not on the cache's device."""
-    dev = getattr(x, "device", None)
-    if dev is not None and (dev.type != "cuda" or dev.index != cache.device):
-        raise ValueError(f"{what} is on {dev}, the cache on cuda:{cache.device}")
+    if x.get_device() != cache.shape[3]:
+        raise ValueError(f"{what} is on {x.device}, the cache on cuda:{cache.shape[3]}")
     return x
 
 
@@ -438,12 +450,13 @@ def _rows(x, cache, heads, tokens, what):
     """eakv_rows_t of a tensor [tokens, heads, head_dim] whose last dim is contiguous."""
     if x is None:
         return None
-    if tuple(x.shape) != (tokens, heads, cache.head_dim):
-        raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(tokens, heads, cache.head_dim)}")
-    if x.stride(2) != 1:
+    if x.shape != (tokens, heads, cache.shape[2]):
+        raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(tokens, heads, cache.shape[2])}")
+    t, h, d = x.stride()
+    if d != 1:
         raise ValueError(f"{what}: the last dim must be contiguous")
     _on(x, cache, what)
-    return _Rows(x.data_ptr(), x.stride(0), x.stride(1), _dtype(x))
+    return _Rows(x.data_ptr(), t, h, _dtype(x))
 
 
 def _ref(x):
@@ -451,14 +464,13 @@ def _ref(x):
 
 
 def _ints(values, n, what):
-    values = [int(v) for v in values]
     if len(values) != n:
         raise ValueError(f"{what}: {len(values)} entries for {n} caches")
     return (_I * n)(*values)
 
 
 def _contiguous(x, cache, dtype, shape, what):
-    if str(x.dtype) != "torch." + dtype or not x.is_contiguous() or tuple(x.shape) != shape:
+    if _name(x) != dtype or not x.is_contiguous() or x.shape != shape:
         raise ValueError(f"{what}: a contiguous {dtype} tensor {shape} expected")
     return _on(x, cache, what)
 
@@ -466,15 +478,15 @@ def _contiguous(x, cache, dtype, shape, what):
 def _index(index, cache):
     """An int32 position list [n], [heads, n] or [layers, heads, n] and its
     layer and head strides (0 where it is shared)."""
-    if str(index.dtype) != "torch.int32" or index.dim() not in (1, 2, 3) or index.stride(-1) not in (0, 1):
+    if _name(index) != "int32" or index.dim() not in (1, 2, 3):
         raise ValueError("index: an int32 tensor [n], [heads, n] or [layers, heads, n] expected")
     if index.shape[-1] > 1 and index.stride(-1) != 1:
         raise ValueError("index: the last dim must be contiguous")
-    x = index.reshape((1,) * (3 - index.dim()) + tuple(index.shape)) if index.dim() < 3 else index
-    if x.shape[0] not in (1, cache.n_layers) or x.shape[1] not in (1, cache.n_kv_heads):
-        raise ValueError(f"index: {tuple(index.shape)} for {cache.n_layers} layers, {cache.n_kv_heads} heads")
+    dims, strides = (1, 1, *index.shape)[-3:], (0, 0, *index.stride())[-3:]
+    if dims[0] not in (1, cache.shape[0]) or dims[1] not in (1, cache.shape[1]):
+        raise ValueError(f"index: {tuple(index.shape)} for {cache.shape[0]} layers, {cache.shape[1]} heads")
     _on(index, cache, "index")
-    return x, (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+    return index, strides[0] if dims[0] > 1 else 0, strides[1] if dims[1] > 1 else 0
 
 
 def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin=None,
@@ -485,23 +497,23 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
     rot_dim/2]; positions: int32 [axes, total] (or [total]); sections: pairs
     that follow each axis. Without tables K goes in as it is."""
     c, counts = caches[0], list(counts)
-    total = sum(counts)
+    total, nkv = sum(counts), c.shape[1]
     if q is not None and q_out is None:
         q_out = q
-    nq = q.shape[1] if q is not None else c.n_kv_heads
-    rk, rv = (_rows(x, c, c.n_kv_heads, total, n) for x, n in ((k, "k"), (v, "v")))
-    rq, ro = (_rows(x, c, nq, total, n) for x, n in ((q, "q"), (q_out, "q_out")))
+    nq = q.shape[1] if q is not None else nkv
+    rk, rv = _rows(k, c, nkv, total, "k"), _rows(v, c, nkv, total, "v")
+    rq, ro = _rows(q, c, nq, total, "q"), _rows(q_out, c, nq, total, "q_out")
     rot = None
     if cos is not None:
         if positions.dim() == 1:
             positions = positions[None]
         if cos.dim() != 2 or cos.dtype != sin.dtype:
             raise ValueError("cos, sin: f32 tables [rows, rot_dim/2] expected")
-        shape = tuple(cos.shape)
+        shape = cos.shape
         _contiguous(cos, c, "float32", shape, "cos")
         _contiguous(sin, c, "float32", shape, "sin")
         axes = positions.shape[0]
-        if (str(positions.dtype) != "torch.int32" or positions.dim() != 2 or axes > 4 or
+        if (_name(positions) != "int32" or positions.dim() != 2 or axes > 4 or
                 positions.shape[1] != total or (total > 1 and positions.stride(1) != 1)):
             raise ValueError(f"positions: int32 [1..4, {total}] expected")
         _on(positions, c, "positions")
@@ -536,7 +548,7 @@ def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=Non
     total, nq = sum(counts), q.shape[1]
     rq, ro = _rows(q, c, nq, total, "q"), _rows(out, c, nq, total, "out")
     if tree is not None:
-        kind = "uint64" if str(tree.dtype) == "torch.uint64" else "int64"
+        kind = "uint64" if _name(tree) == "uint64" else "int64"
         _contiguous(tree, c, kind, (total,), "tree")
     if lse is not None:
         _contiguous(lse, c, "float32", (total, nq), "lse")
@@ -576,11 +588,18 @@ def read_positions(caches, begins, counts, out, layer=0, stream=None):
         raise ValueError("out: [layers, 2, total, n_kv_heads, head_dim] expected")
     if out.shape[0] == 0:
         raise ValueError("out: no layers")
-    rk, rv = (_rows(out[0, i], c, c.n_kv_heads, total, "out") for i in (0, 1))
+    if out.shape[2:] != (total, c.shape[1], c.shape[2]):
+        raise ValueError(f"out: {tuple(out.shape)}, expected [.., 2, {total}, {c.shape[1]}, {c.shape[2]}]")
+    layers, kv, tok, head, last = out.stride()
+    if last != 1:
+        raise ValueError("out: the last dim must be contiguous")
+    _on(out, c, "out")
+    rk = _Rows(out.data_ptr(), tok, head, _dtype(out))
+    rv = _Rows(rk.data and rk.data + kv * out.element_size(), tok, head, rk.dtype)
     return _check(lib().eakv_cache_read(_handles(caches), len(caches), layer, out.shape[0],
                                         _ints(begins, len(caches), "begins"),
                                         _ints(counts, len(caches), "counts"), _ref(rk), _ref(rv),
-                                        out.stride(0), stream), "eakv_cache_read")
+                                        layers, stream), "eakv_cache_read")
 
 
 def lse_combine(n_parts, n_rows, head_dim, d_parts, d_lse, d_output, d_lse_out=None,

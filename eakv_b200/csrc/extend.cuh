@@ -149,39 +149,86 @@ __device__ __forceinline__ float part_weight(float m, float M) {
   return m == -INFINITY ? 1.0f : ex2(m - M);
 }
 
+// Output row of row r of the item's tile.
+template <typename T>
+__device__ __forceinline__ T *extend_out(const ExtendArgs &a, const ExtItem &it, int r) {
+  const int row = it.row0 + r;
+  return reinterpret_cast<T *>(a.out.data) + (long long)(it.tok0 + row / a.G) * a.out.token_stride +
+         (long long)(it.h * a.G + row % a.G) * a.out.head_stride;
+}
+
+// LSE of row r from its base-2 maximum and sum.
+__device__ __forceinline__ void extend_lse(const ExtendArgs &a, const ExtItem &it, int r, float M, float L) {
+  const int row = it.row0 + r;
+  a.lse[(long long)(it.tok0 + row / a.G) * a.n_q + it.h * a.G + row % a.G] =
+      L == 0.0f ? -INFINITY : ((M == -INFINITY ? 0.0f : M) + log2f(L)) * kLn2;
+}
+
 // Four neighbouring dims of the finished row r (unnormalized sums O, base-2
 // maximum M, sum L) to the output; the lane with d == 0 writes the LSE.
 template <typename T>
 __device__ __forceinline__ void extend_store(const ExtendArgs &a, const ExtItem &it, int r, int d,
                                              const float (&O)[4], float M, float L, bool vec) {
-  const int row = it.row0 + r, t = it.tok0 + row / a.G, qh = it.h * a.G + row % a.G;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // nothing attended: zeros
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) y[e] = O[e] * inv;
-  T *p = reinterpret_cast<T *>(a.out.data) + (long long)t * a.out.token_stride +
-         (long long)qh * a.out.head_stride + d;
+  T *p = extend_out<T>(a, it, r) + d;
   if (vec) store4<T, true>(p, y);
   else store4<T, false>(p, y);
-  if (a.lse && d == 0)
-    a.lse[(long long)t * a.n_q + qh] = L == 0.0f ? -INFINITY : ((M == -INFINITY ? 0.0f : M) + log2f(L)) * kLn2;
+  if (a.lse && d == 0) extend_lse(a, it, r, M, L);
 }
 
 // The last CTA of an item: rows merged over the splits, in split order, four
-// dims per thread at a time.
+// dims per thread at a time. `ws` is free shared memory of ws_floats: the
+// splits' weights of a row are worked out once into it, and the records' loads
+// then depend on nothing.
 template <int HD, typename T, int NT>
-__device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem &it, bool vec) {
+__device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem &it, bool vec, float *ws,
+                                             int ws_floats) {
+  const int ns = a.n_splits;
+  float *m_s = ws, *l_s = ws + it.rows, *f_s = ws + 2 * it.rows;   // [rows], [rows], [rows][ns]
+  const bool staged = (ns + 2) * it.rows <= ws_floats;
+  __syncthreads();
+  if (staged) {
+    for (int x = threadIdx.x; x < it.rows * ns; x += NT)
+      f_s[x] = __ldcg(a.part_m + part_row(a, it, x % ns, x / ns));
+    __syncthreads();
+    for (int r = threadIdx.x; r < it.rows; r += NT) {
+      float M = -INFINITY, L = 0.0f;
+      for (int s = 0; s < ns; s++) M = fmaxf(M, f_s[r * ns + s]);
+#pragma unroll 4
+      for (int s = 0; s < ns; s++) {
+        const float f = part_weight(f_s[r * ns + s], M);
+        f_s[r * ns + s] = f;
+        L = fmaf(f, __ldcg(a.part_l + part_row(a, it, s, r)), L);
+      }
+      m_s[r] = M;
+      l_s[r] = L;
+    }
+    __syncthreads();
+  }
   for (int x = threadIdx.x; x < it.rows * (HD / 4); x += NT) {
     const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-    float M = -INFINITY;
-    for (int s = 0; s < a.n_splits; s++) M = fmaxf(M, __ldcg(a.part_m + part_row(a, it, s, r)));
-    float O[4] = {0.0f, 0.0f, 0.0f, 0.0f}, L = 0.0f;
+    float M = -INFINITY, L = 0.0f;
+    if (staged) {
+      M = m_s[r];
+      L = l_s[r];
+    } else {
+      for (int s = 0; s < ns; s++) M = fmaxf(M, __ldcg(a.part_m + part_row(a, it, s, r)));
+    }
+    float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int s = 0; s < a.n_splits; s++) {
+    for (int s = 0; s < ns; s++) {
       const size_t pr = part_row(a, it, s, r);
-      const float f = part_weight(__ldcg(a.part_m + pr), M);
       const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + pr * HD + d));
-      L = fmaf(f, __ldcg(a.part_l + pr), L);
+      float f;
+      if (staged) {
+        f = f_s[r * ns + s];
+      } else {
+        f = part_weight(__ldcg(a.part_m + pr), M);
+        L = fmaf(f, __ldcg(a.part_l + pr), L);
+      }
       O[0] = fmaf(f, o.x, O[0]);
       O[1] = fmaf(f, o.y, O[1]);
       O[2] = fmaf(f, o.z, O[2]);

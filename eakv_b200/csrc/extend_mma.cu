@@ -530,7 +530,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       }
     }
   }
-  if (a.n_splits > 1 && extend_arrive_last(a, it.item)) extend_merge<HD, T, C::THREADS>(a, it, vec);
+  if (a.n_splits > 1 && extend_arrive_last(a, it.item)) extend_merge<HD, T, C::THREADS>(a, it, vec, reinterpret_cast<float *>(smem), C::MAIN / 4);
 }
 
 template <int HD, int LIMBS, typename T>

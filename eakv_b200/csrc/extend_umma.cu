@@ -29,17 +29,17 @@
 // Non-finite V groups are kept out of the products (0 NaN is NaN) and
 // listed by position; a row that attends one gets NaN in the group's dims.
 //
-// Roles (13 warps). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
-// per row; they read S twice (maximum, then weights), write P' over S, and
-// scale O when a maximum moves. Warps 8-11: dequantize, one thread per position
-// row: the raw row comes from global memory a tile ahead in registers
-// and leaves as sixteen 16-byte stores in the 128-byte swizzle. A
-// 32-bit word of nibbles becomes one 16-byte chunk [d, d+2, d+1, d+3, d+32, d+34, d+33,
-// d+35] (the pairs that one mask selects); Q' is stored in the same order and
-// the output's columns are read back in it, so the order costs nothing. Warp
-// 12: one thread issues the MMAs: for tile i, PV of row tile 0, S(i+1) of row tile 0,
-// the same for row tile 1, so one row tile's softmax runs under the other's
-// MMAs. P' of a tile lies over its S; the tensor pipe runs the MMAs in order.
+// Roles (16 warps, the last three idle). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
+// per row; the weights go over S, and O is scaled when a maximum moves. Warps 8-11: dequantize, one thread per position: its K
+// and V rows come from global memory a tile ahead in registers and leave as
+// 16-byte stores in the 128-byte swizzle. A 32-bit word of nibbles becomes one
+// 16-byte chunk [d, d+2, d+1, d+3, d+32, d+34, d+33, d+35] (the pairs that one mask
+// selects); Q' is stored in the same order and the output's columns are read back
+// in it, so the order costs nothing. Warp 12 issues the MMAs: for tile i, PV of
+// row tile 0, S(i+1) of row tile 0, the same for row tile 1, so one row tile's
+// softmax runs under the other's MMAs. P' of a tile lies over its S (tensor
+// memory: 2 x 128 columns of S, 2 x 128 of O: all 512); the tensor pipe runs the
+// MMAs in order.
 //
 // All hand-overs are mbarriers with bounded, suspending waits; one that runs
 // out sets the status word, and every role leaves at its next wait.
@@ -57,8 +57,17 @@ namespace {
 using namespace umma;
 
 constexpr int BN = 128;                       // positions per tile
+constexpr int kStages = 2;                    // K and V operands in flight
+// Tiles whose marks are kept: those of tile i+2 are written when S(i) is done,
+// and the softmax threads look at tile i's, and i-1's, until P'(i) is.
+constexpr int kInfo = 4;
 constexpr int kSoftWarps = 8, kConvWarps = 4;
-constexpr int kThreads = (kSoftWarps + kConvWarps + 1) * 32;
+constexpr int kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kThreads = (kSoftWarps + kConvWarps + 4) * 32;   // four warpgroups, the last mostly idle
+// Registers per thread: the launch gives each thread kRegs, and the warpgroups
+// trade them (512 threads x 128 = 128 x (2 kRegsSoft + kRegsConv + kRegsMma)).
+constexpr int kRegs = 128, kRegsSoft = 176, kRegsConv = 104, kRegsMma = 56;
+static_assert(2 * kRegsSoft + kRegsConv + kRegsMma == 4 * kRegs, "register split");
 constexpr int kUnset = -100000;
 constexpr int kUp = 12, kDown = 10;           // rows within 2^kUp, 2^-kDown of eref need no mark
 constexpr float kPShift = 7.0f;               // P' = 2^7 p
@@ -69,27 +78,31 @@ struct WCfg {
   static constexpr int NG = HD / 64;
   static constexpr int PB = kPagePositions * NG * 40;
   static constexpr int NIB = kPagePositions * NG * 32;
-  static constexpr int TILE = 128 * HD * 2;   // bytes of a 128 x HD f16 operand
-  static constexpr int HALF = 128 * 128;      // bytes of its 64-dim half
+  static constexpr int QTILE = 128 * HD * 2;  // bytes of a row tile of Q'
+  static constexpr int QHALF = 128 * 128;     // bytes of its 64-dim half
+  static constexpr int TILE = BN * HD * 2;    // bytes of a tile's K' or V'
+  static constexpr int HALF = BN * 128;
   static constexpr int Q = 0;                 // two row tiles
-  static constexpr int K = Q + 2 * TILE;      // two stages
-  static constexpr int V = K + 2 * TILE;      // two stages
-  static constexpr int EXPS = V + 2 * TILE;   // short2 [4][BN]: exponents of marked rows
-  static constexpr int INFO = EXPS + 4 * BN * 4;   // int4 [4 tiles][4 warps]
-  static constexpr int BARS = INFO + 4 * 4 * 16;
-  // barriers: kfull[2] vfull[2] kfree[2] vfree[2] sfull[2] pfull[2] odone[2] drain
-  static constexpr int N_BARS = 15;
-  static constexpr int REF = BARS + 8 * N_BARS + 8;    // int2: eref of K, V
-  static constexpr int SLOT = REF + 8;
+  static constexpr int K = Q + 2 * QTILE;
+  static constexpr int V = K + kStages * TILE;
+  // marked rows' exponents and the warps' marks of kInfo tiles
+  static constexpr int EXPS = V + kStages * TILE;            // short2 [kInfo][BN]: K, V
+  static constexpr int INFO = EXPS + kInfo * BN * 4;         // int [kInfo][4 warps]
+  static constexpr int NANS = INFO + kInfo * 16;             // uint2 [kInfo][4 warps]
+  static constexpr int ROWC = NANS + kInfo * 32;         // float [256]: score factor of a row
+  static constexpr int BARS = ROWC + 256 * 4;
+  static constexpr int SLOT = BARS + 8 * 18;
   static constexpr int RED = SLOT + 8;                 // int2 [4]
   static constexpr int END = RED + 32;
   static constexpr int SMEM = END + 1024;              // alignment slack
   // tensor memory columns
   static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
-  static_assert(REF % 8 == 0 && SLOT % 8 == 0 && RED % 8 == 0, "alignment");
+  static_assert(BARS % 8 == 0 && ROWC % 16 == 0 && SLOT % 8 == 0, "alignment");
 };
 
-enum { kKFull = 0, kVFull = 2, kKFree = 4, kVFree = 6, kSFull = 8, kPFull = 10, kODone = 12, kDrain = 14 };
+// Barriers: per stage K and V filled and free; per row tile scores there, each
+// half of the weights there, all outputs summed.
+enum { kKFull = 0, kVFull = 2, kKFree = 4, kVFree = 6, kSFull = 8, kPFull = 10, kODone = 14, kDrain = 16 };
 
 // D[128 x N] (+)= A B, f16 operands, f32 accumulate: A in shared memory
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
@@ -135,6 +148,41 @@ __device__ __forceinline__ uint4 ldg_row(const void *p) {
 __device__ __forceinline__ float pow2i(int e) {   // 2^e, 0 below the normal range
   return __uint_as_float((uint32_t)min(max(127 + e, 0), 254) << 23);
 }
+// Two values as T in one word.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) { return pack_f16(x, y); }
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Waits for the warp's tensor-memory loads, and ties the registers of one to
+// the wait: what reads them cannot be moved ahead of it.
+__device__ __forceinline__ void wait_ld_of(uint32_t (&v)[32]) {
+#define EAKV_T8(i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), \
+                   "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : EAKV_T8(0), EAKV_T8(8), EAKV_T8(16), EAKV_T8(24)::"memory");
+#undef EAKV_T8
+}
+
+// The first trade ends with a barrier of the whole CTA: a warpgroup that has
+// little to do would otherwise ask for its registers back before the softmax
+// warps have got theirs, and both would wait for good.
+__device__ __forceinline__ void regs_traded() { named_sync(2, kThreads); }
+template <int N> __device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // One nibble row (HD/2 bytes) with its (scale, bias) pairs.
@@ -238,18 +286,16 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
   const uint32_t budget = min(a.wait_budget, 1u << 18);
   const int base_pos = it.pg0 * kPagePositions;
   const int end_pos = (it.pg0 + it.npages) * kPagePositions;   // of this split
-  // positions and tiles of each row tile
-  const int n_mt = it.rows > 128 ? 2 : 1;
-  int nt[2];
-#pragma unroll
-  for (int m = 0; m < 2; m++) {
+  // tiles of each row tile
+  auto tiles_of = [&](int m) {
+    if (it.rows <= 128 * m) return 0;
     const int last = min(it.row0 + 128 * m + 127, it.row0 + it.rows - 1);
     const int hi = min(a.tree ? it.hi : it.old + last / a.G + 1, end_pos);
-    nt[m] = (m < n_mt && hi > base_pos) ? (hi - base_pos + BN - 1) / BN : 0;
-  }
-  const int n_tiles = max(nt[0], nt[1]);
+    return hi > base_pos ? (hi - base_pos + BN - 1) / BN : 0;
+  };
+  const int nt0 = tiles_of(0), nt1 = tiles_of(1), n_tiles = max(nt0, nt1);
 
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(smem + C::SLOT), C::COLS);
     tmem_relinquish();
   }
@@ -261,80 +307,24 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       mbar_init(bar(kVFree + i), 1);
       mbar_init(bar(kSFull + i), 1);
       mbar_init(bar(kPFull + i), 4);
+      mbar_init(bar(kPFull + 2 + i), 4);
       mbar_init(bar(kODone + i), 1);
     }
     mbar_init(bar(kDrain), 1);
     fence_mbar_init();
   }
 
-  // ---- Q' (softmax threads: one row each) --------------------------------------
-  float c_row = 0.0f;      // score factor: |scale| log2 e / 2^(q exponent)
-  RowMask mask = {};
-  const int mt = warp >> 2;                       // row tile of a softmax warp
-  const int r_loc = 128 * mt + (threadIdx.x & 127);   // row within the item
-  if (warp < kSoftWarps) {
-    mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
-    const int row = it.row0 + min(r_loc, it.rows - 1);
-    const T *qp = reinterpret_cast<const T *>(a.q.data) +
-                  (long long)(it.tok0 + row / a.G) * a.q.token_stride +
-                  (long long)(it.h * a.G + row % a.G) * a.q.head_stride;
-    float mx = 0.0f;
-    bool bad = false;
-#pragma unroll 4
-    for (int d = 0; d < HD; d += 4) {
-      float v[4];
-      if (vec) load4<T, true>(qp + d, v);
-      else load4<T, false>(qp + d, v);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        mx = fmaxf(mx, fabsf(v[e]));
-        bad = bad || v[e] != v[e];
-      }
-    }
-    const bool fine = !bad && mx <= 3.0e38f;
-    int qe = 0;
-    frexpf(mx > 0.0f && fine ? mx : 1.0f, &qe);   // mx in [2^(qe-1), 2^qe)
-    qe = max(min(5 - qe, 126), -126);
-    const float up = fine ? (a.scale_log2 < 0.0f ? -1.0f : 1.0f) * pow2i(qe) : 0.0f;
-    c_row = fine ? fabsf(a.scale_log2) * pow2i(-qe) : __uint_as_float(0x7fc00000u);
-    uint8_t *op = smem + C::Q + mt * C::TILE;
-    const int rr = threadIdx.x & 127;
-#pragma unroll 2
-    for (int j = 0; j < HD / 8; j++) {
-      const int g = j >> 3, d = 64 * g + 4 * (j & 7);
-      float lo[4], hi[4];
-      if (vec) {
-        load4<T, true>(qp + d, lo);
-        load4<T, true>(qp + d + 32, hi);
-      } else {
-        load4<T, false>(qp + d, lo);
-        load4<T, false>(qp + d + 32, hi);
-      }
-      if (!fine) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) lo[e] = hi[e] = 0.0f;
-      }
-      *reinterpret_cast<uint4 *>(op + g * C::HALF + rr * 128 + (((j & 7) ^ (rr & 7)) << 4)) =
-          make_uint4(pack_f16(lo[0] * up, lo[2] * up), pack_f16(lo[1] * up, lo[3] * up),
-                     pack_f16(hi[0] * up, hi[2] * up), pack_f16(hi[1] * up, hi[3] * up));
-    }
-    fence_proxy_async_smem();
-  }
-
   // ---- dequantizing threads: the first tile, and the references -----------------
   const int crow = threadIdx.x & 127;             // position row of a converter thread
-  const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
+  const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, it.pg0) * C::PB +
+                          (size_t)(crow / kPagePositions) * C::PB;
   const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
   RawRow<HD> kr, vr;
-  // row of tile i held by this thread: live when some row of the item may attend it
-  auto live = [&](int i) {
-    const int p = base_pos + i * BN + crow;
-    return i < n_tiles && p >= it.lo && p < it.hi && p < end_pos;
-  };
+  // This thread's row of tile i, zeros when no row of the item may attend it.
   auto fetch = [&](RawRow<HD> &r, const uint8_t *pages, int i) {
-    if (live(i)) {
-      const int p = base_pos + i * BN + crow;
-      load_row<HD>(r, pages + (size_t)(p / kPagePositions) * C::PB, p % kPagePositions);
+    const int p = base_pos + i * BN + crow;
+    if (i < n_tiles && p >= it.lo && p < it.hi && p < end_pos) {
+      load_row<HD>(r, pages + (size_t)i * (2 * C::PB), crow % kPagePositions);
     } else {
 #pragma unroll
       for (int k = 0; k < HD / 32; k++) r.w[k] = make_uint4(0, 0, 0, 0);
@@ -342,9 +332,65 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       for (int k = 0; k < 2 * C::NG; k++) r.sb[k] = 0.0f;
     }
   };
-  if (warp >= kSoftWarps && warp < kSoftWarps + kConvWarps) {
+  const bool is_conv = warp >= kSoftWarps && warp < kSoftWarps + kConvWarps;
+  if (is_conv) {
     fetch(kr, kpages, 0);
     fetch(vr, vpages, 0);
+  }
+
+  // ---- Q' ------------------------------------------------------------------------
+  // A row is HD/8 lanes of eight dims each; its power of two goes into ROWC with
+  // the scale.
+  if (warp < kSoftWarps) {
+    constexpr int LPR = HD / 8, RPW = 32 / LPR;   // lanes per row, rows per warp and step
+    const int d = 8 * (lane % LPR);
+#pragma unroll 8
+    for (int s = 0; s < 32 / RPW; s++) {
+      const int rl = 32 * warp + s * RPW + lane / LPR;
+      const int row = it.row0 + min(rl, it.rows - 1);
+      const T *qp = reinterpret_cast<const T *>(a.q.data) +
+                    (long long)(it.tok0 + row / a.G) * a.q.token_stride +
+                    (long long)(it.h * a.G + row % a.G) * a.q.head_stride + d;
+      float v0[4], v1[4];
+      if (vec) {
+        load4<T, true>(qp, v0);
+        load4<T, true>(qp + 4, v1);
+      } else {
+        load4<T, false>(qp, v0);
+        load4<T, false>(qp + 4, v1);
+      }
+      float mx = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        // NaN counts as an infinity
+        mx = fmaxf(mx, v0[e] == v0[e] ? fabsf(v0[e]) : INFINITY);
+        mx = fmaxf(mx, v1[e] == v1[e] ? fabsf(v1[e]) : INFINITY);
+      }
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const bool fine = mx <= 3.0e38f;
+      int qe = 0;
+      frexpf(mx > 0.0f && fine ? mx : 1.0f, &qe);   // mx in [2^(qe-1), 2^qe)
+      qe = max(min(5 - qe, 126), -126);
+      const float up = (a.scale_log2 < 0.0f ? -1.0f : 1.0f) * pow2i(qe);
+      if (d == 0)
+        reinterpret_cast<float *>(smem + C::ROWC)[rl] =
+            fine ? fabsf(a.scale_log2) * pow2i(-qe) : __uint_as_float(0x7fc00000u);
+      if (!fine) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v0[e] = v1[e] = 0.0f;
+      }
+      // dims d..d+3 and d+4..d+7: the low or high halves of chunks j and j + 1
+      const int rr = rl & 127, j = (d & 31) >> 2;
+      uint8_t *op = smem + C::Q + (rl >> 7) * C::QTILE + (d >> 6) * C::QHALF + rr * 128 + ((d & 32) >> 2);
+      *reinterpret_cast<uint2 *>(op + ((j ^ (rr & 7)) << 4)) =
+          make_uint2(pack_f16(v0[0] * up, v0[2] * up), pack_f16(v0[1] * up, v0[3] * up));
+      *reinterpret_cast<uint2 *>(op + (((j + 1) ^ (rr & 7)) << 4)) =
+          make_uint2(pack_f16(v1[0] * up, v1[2] * up), pack_f16(v1[1] * up, v1[3] * up));
+    }
+    fence_proxy_async_smem();
+  }
+  if (is_conv) {
     uint32_t bad;
     const int ek = __reduce_max_sync(0xffffffffu, row_exp<HD>(kr, bad));
     const int ev = __reduce_max_sync(0xffffffffu, row_exp<HD>(vr, bad));
@@ -364,338 +410,425 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
   if (vref == kUnset) vref = 0;
   const uint32_t tm = *reinterpret_cast<const uint32_t *>(smem + C::SLOT);
 
+  // Bounded wait of a whole warp for use `use` of barrier b (how often it was
+  // waited for before): its lanes go on, or leave, together.
   bool ok = true;
-  auto wait = [&](int b, int use) {   // `use`: how often this barrier was waited for before
-    if (!ok) return false;
-    if (mbar_wait_sleep(bar(b), use & 1, budget)) return true;
-    atomicOr(a.status, kStatusWaitTimeout);
-    ok = false;
-    return false;
-  };
-
-  // the same for a whole warp: its lanes go on, or leave, together
   auto wait_warp = [&](int b, int use) {
-    wait(b, use);
-    ok = __all_sync(0xffffffffu, ok);
+    if (!__all_sync(0xffffffffu, mbar_wait_sleep(bar(b), use & 1, budget))) {
+      if (lane == 0) atomicOr(a.status, kStatusWaitTimeout);
+      ok = false;
+    }
     return ok;
   };
 
-  float m_run = -INFINITY, l_run = 0.0f;
-  int eref = kUnset;
-  bool poison[2] = {false, false};
-
-  if (warp >= kSoftWarps && warp < kSoftWarps + kConvWarps) {
+  if (is_conv) {
     // ================= dequantize ================================================
+    regs_down<kRegsConv>();
+    regs_traded();
     const int cw = warp - kSoftWarps;
     for (int i = 0; i < n_tiles; i++) {
       const int st = i & 1;
-      if (i >= 2 && !wait_warp(kKFree + st, (i >> 1) - 1)) break;
       uint32_t kbad, vbad;
       const int ke = row_exp<HD>(kr, kbad), ve = row_exp<HD>(vr, vbad);
-      // a non-finite K group keeps its NaN: it reaches its own score only
-      const bool kout = ke != kUnset && (ke > kref + kUp || ke < kref - kDown);
-      const bool vout = ve != kUnset && (ve > vref + kUp || ve < vref - kDown);
-      const bool mark = __any_sync(0xffffffffu, kout || vout);
+      const bool mark = __any_sync(0xffffffffu, (ke != kUnset && (ke > kref + kUp || ke < kref - kDown)) ||
+                                                    (ve != kUnset && (ve > vref + kUp || ve < vref - kDown)));
       const int kx = mark && ke != kUnset ? ke : kref, vx = mark && ve != kUnset ? ve : vref;
+      // a non-finite K group keeps its NaN, which reaches its own score only; a V
+      // group is listed instead
       const uint32_t n0 = __ballot_sync(0xffffffffu, vbad & 1), n1 = __ballot_sync(0xffffffffu, vbad & 2);
-      if (mark) reinterpret_cast<short2 *>(smem + C::EXPS)[(i & 3) * BN + crow] = make_short2(kx, vx);
-      if (lane == 0)
-        reinterpret_cast<int4 *>(smem + C::INFO)[(i & 3) * 4 + cw] = make_int4(mark, n0, n1, 0);
+      if (i >= 2 && !wait_warp(kKFree + st, (i >> 1) - 1)) break;
+      if (mark) reinterpret_cast<short2 *>(smem + C::EXPS)[(i % kInfo) * BN + crow] = make_short2(kx, vx);
+      if (lane == 0) {
+        reinterpret_cast<int *>(smem + C::INFO)[(i % kInfo) * 4 + cw] = (mark ? 1 : 0) | ((n0 | n1) ? 2 : 0);
+        reinterpret_cast<uint2 *>(smem + C::NANS)[(i % kInfo) * 4 + cw] = make_uint2(n0, n1);
+      }
       store_row<HD>(kr, smem + C::K + st * C::TILE, crow, kx, 0u);
-      fetch(kr, kpages, i + 1);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kKFull + st));
+      fetch(kr, kpages, i + 1);
       if (i >= 2 && !wait_warp(kVFree + st, (i >> 1) - 1)) break;
       store_row<HD>(vr, smem + C::V + st * C::TILE, crow, vx, vbad);
-      fetch(vr, vpages, i + 1);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kVFull + st));
+      fetch(vr, vpages, i + 1);
     }
-  } else if (warp == 12) {
+  } else if (warp >= kMmaWarp) {
     // ================= MMAs ======================================================
-    if (lane == 0) {
-      const uint32_t sb = smem_u32(smem);
-      auto scores = [&](int m, int i) {
-        const uint32_t q0 = sb + C::Q + m * C::TILE, k0 = sb + C::K + (i & 1) * C::TILE;
-        const uint32_t d = tm + C::S_COL + 128 * m;
+    regs_down<kRegsMma>();
+    regs_traded();
+    if (warp == kMmaWarp) {
+    // The whole warp walks the tiles, so that descriptors stay in uniform
+    // registers; one lane issues.
+    const bool issuer = elect_one();
+    const uint32_t sb = smem_u32(smem);
+    const uint64_t qd = sdesc(sb + C::Q, 16, 1024, kLayoutSW128);
+    const uint64_t kd = sdesc(sb + C::K, 16, 1024, kLayoutSW128);
+    const uint64_t vd = sdesc(sb + C::V, C::HALF, 1024, kLayoutSW128);
+    // a descriptor's address field counts 16 bytes
+    auto scores = [&](int m, int i) {
+      const uint64_t q = qd + (uint64_t)(m * (C::QTILE >> 4)), k = kd + (uint64_t)((i & 1) * (C::TILE >> 4));
+      const uint32_t d = tm + C::S_COL + 128 * m;
+      if (issuer) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++) {
-          const uint32_t off = (k >> 2) * C::HALF + (k & 3) * 32;
-          mma_f16_ss(d, sdesc(q0 + off, 16, 1024, kLayoutSW128), sdesc(k0 + off, 16, 1024, kLayoutSW128),
-                     idesc_f16(BN, 0), k > 0);
+        for (int s = 0; s < HD / 16; s++) {
+          const uint64_t off = ((s >> 2) * C::HALF + (s & 3) * 32) >> 4;
+          mma_f16_ss(d, q + off, k + off, idesc_f16(BN, 0), s > 0);
         }
         if (i != a.test_stall - 1) mma_commit(bar(kSFull + m));   // test hook: never ready
-      };
-      auto outputs = [&](int m, int i) {
-        const uint32_t v0 = sb + C::V + (i & 1) * C::TILE;
-        const uint32_t p = tm + C::S_COL + 128 * m, d = tm + C::O_COL + HD * m;
-#pragma unroll
-        for (int k = 0; k < BN / 16; k++)
-          mma_f16_ts(d, p + 8 * k, sdesc(v0 + k * 2048, C::HALF, 1024, kLayoutSW128),
-                     idesc_f16(HD, 1), i > 0 || k > 0);
-        if (i == nt[m] - 1) mma_commit(bar(kODone + m));
-      };
-      // tile i's K (V) is released by the last row tile that uses it
-      auto last_user = [&](int i) { return i < nt[1] ? 1 : 0; };
-      if (n_tiles > 0 && wait(kKFull, 0)) {
-        fence_after_sync();
-        for (int m = 0; m < 2; m++)
-          if (nt[m] > 0) scores(m, 0);
-        mma_commit(bar(kKFree));
+        // the tile's K is free when the last row tile that uses it has its scores
+        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kKFree + (i & 1)));
       }
-      for (int i = 0; i < n_tiles && ok; i++) {
-        for (int m = 0; m < 2 && ok; m++) {
-          if (i < nt[m]) {
-            if (!wait(kPFull + m, i)) break;
-            // each tile's V is waited for once
-            if (m == (nt[0] > i ? 0 : 1) && !wait(kVFull + (i & 1), i >> 1)) break;
-            fence_after_sync();
-            outputs(m, i);
-            if (m == last_user(i)) mma_commit(bar(kVFree + (i & 1)));
-          }
-          if (i + 1 < nt[m]) {
-            if (m == (nt[0] > i + 1 ? 0 : 1) && !wait(kKFull + ((i + 1) & 1), (i + 1) >> 1)) break;
-            fence_after_sync();
-            scores(m, i + 1);
-            if (m == last_user(i + 1)) mma_commit(bar(kKFree + ((i + 1) & 1)));
-          }
+    };
+    // PV of tile i, half by half as the weights come; false when a wait ran out
+    auto outputs = [&](int m, int i, int n) {
+      const uint64_t v = vd + (uint64_t)((i & 1) * (C::TILE >> 4));
+      const uint32_t p = tm + C::S_COL + 128 * m, d = tm + C::O_COL + HD * m;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (!wait_warp(kPFull + 2 * m + h, i)) return false;
+        fence_after_sync();
+        if (issuer) {
+#pragma unroll
+          for (int s = h * (BN / 32); s < (h + 1) * (BN / 32); s++)
+            mma_f16_ts(d, p + 8 * s, v + (uint64_t)(s * (2048 >> 4)), idesc_f16(HD, 1), i > 0 || s > 0);
         }
       }
-      // every MMA has ended before the tensor memory is given back
-      mma_commit(bar(kDrain));
-      if (!mbar_wait_sleep(bar(kDrain), 0, budget)) {
-        atomicOr(a.status, kStatusWaitTimeout);
-        ok = false;
+      if (issuer) {
+        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kVFree + (i & 1)));
+        if (i == n - 1) mma_commit(bar(kODone + m));
+      }
+      return true;
+    };
+    // Each tile's K and V is waited for once, ahead of the weights that it is
+    // used behind, so that nothing stands between these and their MMAs.
+    if (n_tiles > 0 && wait_warp(kKFull, 0)) {
+      fence_after_sync();
+      if (nt0 > 0) scores(0, 0);
+      if (nt1 > 0) scores(1, 0);
+    }
+    for (int i = 0; i < n_tiles && ok; i++) {
+      if (i + 1 < n_tiles && !wait_warp(kKFull + ((i + 1) & 1), (i + 1) >> 1)) break;
+      if (!wait_warp(kVFull + (i & 1), i >> 1)) break;
+      if (i < nt0) {
+        if (!outputs(0, i, nt0)) break;
+        if (i + 1 < nt0) scores(0, i + 1);
+      }
+      if (i < nt1) {
+        if (!outputs(1, i, nt1)) break;
+        if (i + 1 < nt1) scores(1, i + 1);
       }
     }
+    // every MMA has ended before the tensor memory is given back
+    if (issuer) mma_commit(bar(kDrain));
     __syncwarp();
+    wait_warp(kDrain, 0);
+    }
   } else {
     // ================= softmax: one row per thread ===============================
+    regs_up<kRegsSoft>();
+    regs_traded();
+    const int mt = warp >> 2;                            // row tile
+    const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
+    const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
+    // score factor: |scale| log2 e / 2^(q exponent), with K's 2^kref
+    float c_row = reinterpret_cast<const float *>(smem + C::ROWC)[r_loc];
+    c_row *= pow2i(kref >> 1);
+    c_row *= pow2i(kref - (kref >> 1));
+    float m_run = -INFINITY, l_run = 0.0f;
+    int eref = kUnset;
+    bool poison0 = false, poison1 = false;   // a non-finite V group was attended
+    bool steady = true;   // of the warp: no row's eref is far from vref
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // tensor-memory lane 32 (warp % 4)
     const uint32_t ts = tm + lanes + C::S_COL + 128 * mt, to = tm + lanes + C::O_COL + HD * mt;
     // positions that every row of this row tile attends
     const int first = it.row0 + 128 * mt, last = min(first + 127, it.row0 + it.rows - 1);
     const int all_hi = min(a.tree ? it.old : it.old + first / a.G + 1, end_pos);
     const int all_lo = a.window > 0 ? max(0, it.old + last / a.G + 1 - a.window) : 0;
-    const int my_tiles = mt ? nt[1] : nt[0];
+    const int my_tiles = mt ? nt1 : nt0;
 
     // O times f. Called between S(i) and P'(i): the commit that announced S(i)
     // covers the MMAs before it, the tile before's PV among them, and tile i's is
     // not issued yet.
     auto scale_out = [&](float f) {
 #pragma unroll 1
-      for (int k = 0; k < HD; k += 32) {
-        uint32_t v[32];
-        tmem_ld32(to + k, v);
+      for (int k = 0; k < HD; k += 16) {
+        uint32_t v[16];
+        tmem_ld16(to + k, v);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-        uint32_t h0[16], h1[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          h0[e] = v[e];
-          h1[e] = v[16 + e];
-        }
-        tmem_st16(to + k, h0);
-        tmem_st16(to + k + 16, h1);
+        for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+        tmem_st16(to + k, v);
       }
+    };
+    // Half h of the tile's weights is in tensor memory (and O is scaled).
+    auto announce = [&](int h) {
       tmem_wait_st();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPFull + 2 * mt + h));
+    };
+    // The scores' maximum xm of a tile (base 2, -inf: none) moves the running
+    // maximum when it passes it by 8; `f` is what the sums so far are scaled by.
+    auto new_max = [&](float xm, float &f) {
+      f = 1.0f;
+      if (xm > m_run + 8.0f) {
+        f = ex2(m_run - xm);
+        m_run = xm;
+        l_run *= f;
+        return true;
+      }
+      return false;
     };
 
-    auto tile = [&](auto masked_tag, auto slow_tag, int i, int marks) {
-      constexpr bool MASKED = decltype(masked_tag)::value, SLOW = decltype(slow_tag)::value;
+    // A tile without marked rows: the row's 128 scores in registers.
+    auto tile_fast = [&](auto masked_tag, int i) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
       const int c0 = base_pos + i * BN;
-      const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + (i & 3) * BN;
+      uint32_t v[4][32];
+#pragma unroll
+      for (int ch = 0; ch < 4; ch++) tmem_ld32(ts + 32 * ch, v[ch]);
+#pragma unroll
+      for (int ch = 0; ch < 4; ch++) wait_ld_of(v[ch]);
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int ch = 0; ch < 4; ch++) {
+          const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (!((on >> e) & 1)) v[ch][e] = 0xff800000u;   // -inf
+        }
+      }
+      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int ch = 0; ch < 4; ch++)
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            t[k] = max3(t[k], __uint_as_float(v[ch][e + 2 * k]), __uint_as_float(v[ch][e + 2 * k + 1]));
+      const float mx = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+      // the maximum of nothing stays -inf (-inf * 0 is NaN)
+      const float xm = mx == -INFINITY ? mx : mx * c_row;
+      if (eref == kUnset) eref = vref;
+      if (__any_sync(0xffffffffu, xm > m_run + 8.0f)) {
+        float f;
+        new_max(xm, f);
+        if (i > 0) scale_out(f);
+      }
+      // the weights carry 2^(vref - eref) whole; the sum takes it off
+      const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run) + (float)(vref - eref);
+      const float2 c2 = make_float2(c_row, c_row), o2 = make_float2(off, off);
+      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+      for (int ch = 0; ch < 4; ch++) {
+        uint32_t p16[16];
+        const uint32_t (&x)[32] = v[ch];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, o2);
+          float2 p = make_float2(ex2(y.x), ex2(y.y));
+          if (MASKED) {   // -inf * 0 where c_row is 0
+            if (x[e] == 0xff800000u) p.x = 0.0f;
+            if (x[e + 1] == 0xff800000u) p.y = 0.0f;
+          }
+          sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], p);
+          p16[e >> 1] = pack_f16(p.x, p.y);
+        }
+        tmem_st16(ts + 16 * ch, p16);
+        if (ch == 1) announce(0);
+      }
+      l_run += (sum[0].x + sum[0].y + sum[1].x + sum[1].y) * pow2i(eref - vref);
+      announce(1);
+    };
+
+    // Any tile: every position with its own powers of two.
+    auto tile_slow = [&](int i, int marks) {
+      const int c0 = base_pos + i * BN;
+      const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + (i % kInfo) * BN;
       float mx = -INFINITY;
       int emax = kUnset;
 #pragma unroll 1
       for (int ch = 0; ch < 4; ch++) {
         uint32_t v[32];
         tmem_ld32(ts + 32 * ch, v);
-        const uint32_t on = MASKED ? mask32(mask, c0 + 32 * ch, end_pos) : 0xffffffffu;
-        tmem_wait_ld();
-        if constexpr (SLOW) {
-          const bool mk = (marks >> ch) & 1;
-#pragma unroll 4
-          for (int e = 0; e < 32; e++) {
-            const short2 x = mk ? ex[32 * ch + e] : make_short2(kref, vref);
-            if ((on >> e) & 1) {
-              mx = fmaxf(mx, __uint_as_float(v[e]) * pow2i(x.x - kref));
-              emax = max(emax, (int)x.y);
-            }
-          }
-        } else {
-          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+        const bool mk = (marks >> ch) & 1;
+        wait_ld_of(v);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float x0 = (!MASKED || ((on >> e) & 1)) ? __uint_as_float(v[e]) : -INFINITY;
-            const float x1 = (!MASKED || ((on >> (e + 1)) & 1)) ? __uint_as_float(v[e + 1]) : -INFINITY;
-            t[(e >> 1) & 3] = max3(t[(e >> 1) & 3], x0, x1);
+        for (int e = 0; e < 32; e++) {
+          const short2 x = mk ? ex[32 * ch + e] : make_short2(kref, vref);
+          if ((on >> e) & 1) {
+            mx = fmaxf(mx, __uint_as_float(v[e]) * pow2i(x.x - kref));
+            emax = max(emax, (int)x.y);
           }
-          mx = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
         }
       }
-      // c_row carries 2^kref; the maximum of nothing stays -inf (-inf * 0 is NaN)
-      const float xm = mx == -INFINITY ? mx : mx * c_row;
-      float f = 1.0f;
-      bool move = false;
-      if (xm > m_run + 8.0f) {
-        f = ex2(m_run - xm);
-        m_run = xm;
-        l_run *= f;
+      float f;
+      bool move = new_max(mx == -INFINITY ? mx : mx * c_row, f);
+      if (emax != kUnset && (eref == kUnset || emax > eref)) {
+        if (eref != kUnset) f *= pow2i(eref - emax);
+        eref = emax;
         move = true;
       }
-      if constexpr (SLOW) {
-        if (emax != kUnset && (eref == kUnset || emax > eref)) {
-          if (eref != kUnset) f *= pow2i(eref - emax);
-          eref = emax;
-          move = true;
-        }
-      } else if (eref == kUnset) {
-        eref = vref;
-      }
       if (i > 0 && __any_sync(0xffffffffu, move)) scale_out(f);
-      // weights of unmarked tiles carry 2^(vref - eref) whole; the sum takes it off
-      float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
-      if (!SLOW) off += (float)(vref - eref);
-      float2 sum = make_float2(0.0f, 0.0f);
+      const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll 1
       for (int ch = 0; ch < 4; ch++) {
         uint32_t v[32], p16[16];
         tmem_ld32(ts + 32 * ch, v);
-        const uint32_t on = MASKED ? mask32(mask, c0 + 32 * ch, end_pos) : 0xffffffffu;
-        tmem_wait_ld();
-        if constexpr (SLOW) {
-          const bool mk = (marks >> ch) & 1;
+        const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+        const bool mk = (marks >> ch) & 1;
+        wait_ld_of(v);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float w[2];
+        for (int e = 0; e < 32; e += 2) {
+          float w[2];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-              const short2 x = mk ? ex[32 * ch + e + u] : make_short2(kref, vref);
-              const bool at = (on >> (e + u)) & 1;
-              const float p = at ? ex2(fmaf(__uint_as_float(v[e + u]) * pow2i(x.x - kref), c_row, off)) : 0.0f;
-              sum.x += p;
-              w[u] = at ? p * pow2i(x.y - eref) : 0.0f;
-            }
-            p16[e >> 1] = pack_f16(w[0], w[1]);
+          for (int u = 0; u < 2; u++) {
+            const short2 x = mk ? ex[32 * ch + e + u] : make_short2(kref, vref);
+            const bool at = (on >> (e + u)) & 1;
+            const float p = at ? ex2(fmaf(__uint_as_float(v[e + u]) * pow2i(x.x - kref), c_row, off)) : 0.0f;
+            l_run += p;
+            w[u] = at ? p * pow2i(x.y - eref) : 0.0f;
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])),
-                                        make_float2(c_row, c_row), make_float2(off, off));
-            float2 p = make_float2(ex2(x.x), ex2(x.y));
-            if (MASKED) {
-              if (!((on >> e) & 1)) p.x = 0.0f;
-              if (!((on >> (e + 1)) & 1)) p.y = 0.0f;
-            }
-            sum = __fadd2_rn(sum, p);
-            p16[e >> 1] = pack_f16(p.x, p.y);
-          }
+          p16[e >> 1] = pack_f16(w[0], w[1]);
         }
         tmem_st16(ts + 16 * ch, p16);
       }
-      l_run += SLOW ? sum.x + sum.y : (sum.x + sum.y) * pow2i(eref - vref);
-      tmem_wait_st();
+      announce(0);
+      announce(1);
     };
 
-    c_row *= pow2i(kref >> 1);   // 2^kref in two factors
-    c_row *= pow2i(kref - (kref >> 1));
     for (int i = 0; i < my_tiles; i++) {
       if (!wait_warp(kSFull + mt, i)) break;
       fence_after_sync();
       const int c0 = base_pos + i * BN;
       const bool full = c0 >= all_lo && c0 + BN <= all_hi;
-      int marks = 0;
-      uint32_t nan_any = 0;
-      const int4 *info = reinterpret_cast<const int4 *>(smem + C::INFO) + (i & 3) * 4;
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const int4 x = info[w];
-        marks |= x.x << w;
-        nan_any |= (uint32_t)x.y | (uint32_t)x.z;
-      }
-      if (nan_any) {
+      // bit 0 of a warp's word: marked rows, bit 1: non-finite V groups
+      const int4 sum = *reinterpret_cast<const int4 *>(smem + C::INFO + (i % kInfo) * 16);
+      const int any = sum.x | sum.y | sum.z | sum.w;
+      if (any & 2) {
+        const uint2 *bad = reinterpret_cast<const uint2 *>(smem + C::NANS) + (i % kInfo) * 4;
         for (int w = 0; w < 4; w++) {
           const uint32_t on = mask32(mask, c0 + 32 * w, end_pos);
-          poison[0] = poison[0] || (on & (uint32_t)info[w].y);
-          poison[1] = poison[1] || (on & (uint32_t)info[w].z);
+          poison0 = poison0 || (on & bad[w].x);
+          poison1 = poison1 || (on & bad[w].y);
         }
       }
-      const bool plain = !marks && __all_sync(0xffffffffu, eref == kUnset || (eref >= vref && eref <= vref + 30));
-      if (!plain) tile(std::true_type{}, std::true_type{}, i, marks);
-      else if (full) tile(std::false_type{}, std::false_type{}, i, 0);
-      else tile(std::true_type{}, std::false_type{}, i, 0);
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPFull + mt));
-    }
-  }
-
-  // ---- results --------------------------------------------------------------------
-  if (warp < kSoftWarps && ok) {
-    const int my_tiles = mt ? nt[1] : nt[0];
-    if (my_tiles > 0) {
-      wait_warp(kODone + mt, 0);
-      fence_after_sync();
-    }
-  }
-  const bool all_ok = __syncthreads_and(ok);
-  if (all_ok && warp < kSoftWarps) {
-    const int my_tiles = mt ? nt[1] : nt[0];
-    const uint32_t to = tm + ((uint32_t)(warp & 3) << 21) + C::O_COL + HD * mt;
-    const bool mine = r_loc < it.rows;
-    const float down = 0.0078125f;   // 2^-kPShift
-    const float L = l_run * down;
-    // O carries 2^(kPShift - eref); in two factors
-    const int e = eref == kUnset ? 0 : eref;
-    const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1));
-#pragma unroll 1
-    for (int j = 0; j < HD / 8; j++) {
-      uint32_t v[8];
-      if (my_tiles > 0) {
-        tmem_ld8(to + 8 * j, v);
-        tmem_wait_ld();
+      if ((any & 1) || !steady) {
+        tile_slow(i, (sum.x & 1) | (sum.y & 1) << 1 | (sum.z & 1) << 2 | (sum.w & 1) << 3);
+        steady = __all_sync(0xffffffffu, eref == kUnset || (eref >= vref && eref <= vref + 30));
+      } else if (full) {
+        tile_fast(std::false_type{}, i);
       } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = 0u;
-      }
-      const int g = j >> 3;
-      float o[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float x = __uint_as_float(v[k]) * f0 * f1;
-        o[k] = poison[g] ? __uint_as_float(0x7fc00000u) : x;
-      }
-      const float lo[4] = {o[0], o[2], o[1], o[3]}, hi[4] = {o[4], o[6], o[5], o[7]};
-      const int d = 64 * g + 4 * (j & 7);
-      if (mine) {
-        if (a.n_splits == 1) {
-          extend_store<T>(a, it, r_loc, d, lo, m_run, L, vec);
-          extend_store<T>(a, it, r_loc, d + 32, hi, m_run, L, vec);
-        } else {
-          const size_t pr = part_row(a, it, it.split, r_loc);
-          *reinterpret_cast<float4 *>(a.part_o + pr * HD + d) = make_float4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<float4 *>(a.part_o + pr * HD + d + 32) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-        }
+        tile_fast(std::true_type{}, i);
       }
     }
-    if (mine && a.n_splits > 1) {
-      const size_t pr = part_row(a, it, it.split, r_loc);
-      a.part_m[pr] = m_run;
-      a.part_l[pr] = L;
+
+    // ---- results ----------------------------------------------------------------
+    if (ok && my_tiles > 0) wait_warp(kODone + mt, 0);
+    // both row tiles are through with K' and V': their space takes the rows on
+    // their way out
+    named_sync(1, kSoftWarps * 32);
+    if (ok) {
+      fence_after_sync();
+      const float down = 0.0078125f;   // 2^-kPShift
+      const float L = l_run * down;
+      // O carries 2^(kPShift - eref); in two factors. Finished rows are divided here.
+      const int e = eref == kUnset ? 0 : eref;
+      const float inv = a.n_splits > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
+      const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1)) * inv;
+      if (r_loc < it.rows) {
+        if (a.n_splits > 1) {
+          const size_t pr = part_row(a, it, it.split, r_loc);
+          a.part_m[pr] = m_run;
+          a.part_l[pr] = L;
+        } else if (a.lse) {
+          extend_lse(a, it, r_loc, m_run, L);
+        }
+      }
+      // A thread's row leaves by way of shared memory, so that whole lines are
+      // stored: up to 256 bytes of a row at a time, 32 rows per warp.
+      uint8_t *stage = smem + C::K + warp * (32 * 256);
+      static_assert(8 * 32 * 256 <= 2 * kStages * C::TILE, "room for the rows of eight warps");
+      const int esize = a.n_splits > 1 ? 4 : 2, per_pass = a.n_splits > 1 ? 64 : HD;
+#pragma unroll 1
+      for (int d0 = 0; d0 < HD; d0 += per_pass) {
+        // 16 columns: dims 4j..4j+7 and 32 on of a 64-dim group
+#pragma unroll 1
+        for (int j = d0 / 8; j < (d0 + per_pass) / 8; j += 2) {
+          uint32_t v[16];
+          if (my_tiles > 0) {
+            tmem_ld16(to + 8 * j, v);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = 0u;
+          }
+          const bool bad = j < 8 ? poison0 : poison1;
+          float o[16];
+#pragma unroll
+          for (int k = 0; k < 16; k++)
+            o[k] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float(v[k]) * f0 * f1;
+          const float lo[8] = {o[0], o[2], o[1], o[3], o[8], o[10], o[9], o[11]};
+          const float hi[8] = {o[4], o[6], o[5], o[7], o[12], o[14], o[13], o[15]};
+          const int d = 64 * (j >> 3) + 4 * (j & 7) - d0;   // within the pass
+          // 16-byte chunks of the row, rotated by the lane
+          auto put = [&](int byte, uint4 x) {
+            *reinterpret_cast<uint4 *>(stage + lane * 256 + ((byte + 16 * lane) & 255)) = x;
+          };
+          if (a.n_splits > 1) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+              put(4 * (d + k), make_uint4(__float_as_uint(lo[k]), __float_as_uint(lo[k + 1]),
+                                          __float_as_uint(lo[k + 2]), __float_as_uint(lo[k + 3])));
+              put(4 * (d + 32 + k), make_uint4(__float_as_uint(hi[k]), __float_as_uint(hi[k + 1]),
+                                               __float_as_uint(hi[k + 2]), __float_as_uint(hi[k + 3])));
+            }
+          } else {
+            put(2 * d, make_uint4(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(lo[4], lo[5]),
+                                  pack2<T>(lo[6], lo[7])));
+            put(2 * d + 64, make_uint4(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]), pack2<T>(hi[4], hi[5]),
+                                       pack2<T>(hi[6], hi[7])));
+          }
+        }
+        __syncwarp();
+        const int cpr = per_pass * esize / 16;   // chunks per row: 8 or 16
+#pragma unroll 4
+        for (int x = lane; x < 32 * cpr; x += 32) {
+          const int rr = x / cpr, ch = x % cpr, r = 128 * mt + 32 * (warp & 3) + rr;
+          if (r >= it.rows) continue;
+          const uint4 y = *reinterpret_cast<const uint4 *>(stage + rr * 256 + ((16 * ch + 16 * rr) & 255));
+          if (a.n_splits > 1) {
+            *reinterpret_cast<uint4 *>(a.part_o + part_row(a, it, it.split, r) * HD + d0 + 4 * ch) = y;
+          } else {
+            T *p = extend_out<T>(a, it, r) + 8 * ch;
+            if (vec) {
+              // 8-byte pieces: rows start on 4-element boundaries
+              reinterpret_cast<uint2 *>(p)[0] = make_uint2(y.x, y.y);
+              reinterpret_cast<uint2 *>(p)[1] = make_uint2(y.z, y.w);
+            } else {
+              const T *e8 = reinterpret_cast<const T *>(&y);
+#pragma unroll
+              for (int k = 0; k < 8; k++) p[k] = e8[k];
+            }
+          }
+        }
+        __syncwarp();
+      }
     }
     fence_before_sync();
+    regs_down<kRegs>();
   }
-  __syncthreads();
+  if (warp >= kSoftWarps) regs_up<kRegs>();   // given back by the softmax warps
+  const bool all_ok = __syncthreads_and(ok);
   fence_after_sync();
-  if (warp == 12) tmem_dealloc(tm, C::COLS);
+  if (warp == kMmaWarp) tmem_dealloc(tm, C::COLS);
   if (a.n_splits > 1) {
     const bool last = extend_arrive_last(a, it.item);
-    if (last && all_ok) extend_merge<HD, T, kThreads>(a, it, vec);
+    if (last && all_ok)
+      extend_merge<HD, T, kThreads>(a, it, vec, reinterpret_cast<float *>(smem), C::EXPS / 4);
   }
 }
 
@@ -710,6 +843,15 @@ int launch_one(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec
     int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                         "extend_umma: smem attribute");
     if (rc) return rc;
+    // the warpgroups trade the launch's registers: they have to add up
+    cudaFuncAttributes at;
+    rc = check_cuda(cudaFuncGetAttributes(&at, fn), "extend_umma: attributes");
+    if (rc) return rc;
+    if (at.numRegs != kRegs) {
+      set_error(EAKV_ERR_INVALID, "extend_umma: built with %d registers per thread, %d expected",
+                at.numRegs, kRegs);
+      return EAKV_ERR_INVALID;
+    }
     attr_done.fetch_or(1ull << (dev & 63), std::memory_order_acq_rel);
   }
   fn<<<n_blocks, kThreads, C::SMEM, s>>>(a, b, vec ? 1 : 0);

@@ -59,7 +59,7 @@ def test_struct_layouts_match_the_header():
 
 class FakeCache:
     """What the argument checks ask of a cache."""
-    n_layers, n_kv_heads, head_dim, device, h, seq_len = 2, 4, 64, 0, 0, 10
+    h, shape = 0, (2, 4, 64, 0)
 
 
 def test_python_checks_refuse_before_the_library():
