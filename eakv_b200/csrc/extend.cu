@@ -27,15 +27,22 @@ constexpr int kSplitPagesF32 = 64, kSplitPages16 = 256, kSplitPagesUmma = 1024;
 // Rows (new tokens x query heads per KV head) up to which 16-bit calls take the
 // warp-level kernel.
 constexpr int kMmaRows = 32;
+constexpr int kTile = 16;
+// Shortest parts worth a CTA, and what an item costs beyond its positions (set-up,
+// results), in pages of the warp-level kernel and tiles of the tcgen05 kernel.
+constexpr int kLeastPages = 6, kLeastTiles = 4;
+constexpr int kOverheadPages = 6, kOverheadTiles = 5;
 
 // One launch's caches and plan: a call's caches with few rows and those with
 // many go to different kernels.
 struct Part {
   bool umma;
   int tiles, launch_tiles;   // row tiles in all and per launch
-  size_t records;            // bytes of split records of one launch
-  int tile_rows, n_splits, split_pages, n_caches;
+  int slots;                 // records of one launch (0: nothing is cut)
+  int tile_rows, unit_pages, run, n_runs, overhead, n_splits, split_units, n_caches;
+  long long units;
   ExtendBatch b;
+  ExtendRuns runs;
 };
 
 int sm_count(int dev) {
@@ -48,18 +55,26 @@ int sm_count(int dev) {
 // bytes. Call with the caches' device current.
 int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool umma, Part &p) {
   p.umma = umma;
-  p.tile_rows = umma ? kExtendUmmaRows : kExtendMmaRows;
+  // the warp-level kernel's tiles: 32 rows where a cache has more than 16 (a page
+  // is converted once for a tile)
+  p.tile_rows = umma ? kExtendUmmaRows : 16;
+  auto mine = [&](int i) {
+    const long long rows = (long long)(t.first[i + 1] - t.first[i]) * a.G;
+    const bool many = a.dtype != EAKV_F32 && t_force_path != 2 && (rows > kMmaRows || t_force_path == 3);
+    return rows > 0 && many == umma;
+  };
+  for (int i = 0; i < a.n_caches && !umma; i++)
+    if (mine(i) && (long long)(t.first[i + 1] - t.first[i]) * a.G > 16) p.tile_rows = kTile;
   p.n_caches = 0;
-  p.records = 0;
-  p.n_splits = p.split_pages = 1;
+  p.slots = p.run = p.n_runs = p.overhead = 0;
+  p.units = 0;
+  p.n_splits = p.split_units = 1;
+  p.unit_pages = umma ? 2 : 1;   // the tcgen05 kernel's tiles are two pages
   const int heads = a.geom.n_heads;
   long long tiles = 0;
-  int max_pages = 1;
   for (int i = 0; i < a.n_caches; i++) {
+    if (!mine(i)) continue;
     const int n = t.first[i + 1] - t.first[i];
-    const bool many = a.dtype != EAKV_F32 && t_force_path != 2 &&
-                      ((long long)n * a.G > kMmaRows || t_force_path == 3);
-    if (n == 0 || many != umma) continue;
     const int k = p.n_caches++;
     p.b.base[k] = t.base[i];
     p.b.old[k] = t.pos[i];
@@ -67,50 +82,82 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
     p.b.n_new[k] = n;
     p.b.tile0[k] = (int)tiles;
     tiles += ((long long)n * a.G + p.tile_rows - 1) / p.tile_rows;
-    long long span = (long long)t.pos[i] + n;   // positions a tile may attend
-    if (a.window > 0) {
-      // its tokens' windows (a tree's tokens may look ahead within n)
-      const long long w = (long long)a.window + (tree ? n : p.tile_rows / a.G + 1);
-      if (w < span) span = w + kPagePositions;    // not page-aligned
+    if (tiles * heads > (1ll << 30)) {
+      set_error(EAKV_ERR_INVALID, "extend_attention: more than 2^30 tiles of rows");
+      return EAKV_ERR_INVALID;
     }
-    const int pages = (int)((span + kPagePositions - 1) / kPagePositions);
-    if (pages > max_pages) max_pages = pages;
   }
   for (int i = p.n_caches; i <= kMaxBatch; i++) p.b.tile0[i] = (int)tiles;
   p.tiles = p.launch_tiles = (int)tiles;
   if (p.tiles == 0) return EAKV_OK;
-  if (tiles * heads > (1ll << 30)) {
-    set_error(EAKV_ERR_INVALID, "extend_attention: more than 2^30 tiles of rows");
-    return EAKV_ERR_INVALID;
-  }
-  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype);
+  // units of a tile's items, and of all
+  auto units_of = [&](int k, int tile) {
+    const int row0 = (tile - p.b.tile0[k]) * p.tile_rows, all = p.b.n_new[k] * a.G;
+    const int rows = all - row0 < p.tile_rows ? all - row0 : p.tile_rows;
+    const ExtRange r = extend_range(row0, rows, a.G, p.b.old[k], p.b.n_new[k], a.window, tree);
+    return (r.pages + p.unit_pages - 1) / p.unit_pages;
+  };
+  const int overhead = umma ? kOverheadTiles : kOverheadPages;
+  long long units = 0;   // with the items' overheads
+  int max_units = 1;
+  for (int k = 0; k < p.n_caches; k++)
+    for (int i = p.b.tile0[k]; i < p.b.tile0[k + 1]; i++) {
+      const int u = units_of(k, i);
+      units += (long long)(u + overhead) * heads;
+      if (u > max_units) max_units = u;
+    }
+  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype, p.tile_rows);
   if (per_sm <= 0) return EAKV_ERR_INVALID;   // recorded by the lookup
-  const int cap = umma ? kSplitPagesUmma : a.dtype == EAKV_F32 ? kSplitPagesF32 : kSplitPages16;
-  const int lo = (max_pages + cap - 1) / cap;
-  int hi = max_pages / 2;   // two pages at least: one per warp, or one tile
-  if (hi < lo) hi = lo;
-  if (hi > 4096) hi = 4096;
-  int ns = t_force_splits > 0 ? t_force_splits
-                              : choose_splits(tiles * heads, max_pages, lo, hi, per_sm, sm_count(device));
-  if (ns > max_pages) ns = max_pages;
-  if (ns < 1) ns = 1;
-  p.split_pages = (max_pages + ns - 1) / ns;
-  if (umma) p.split_pages += p.split_pages & 1;   // tiles of two pages
-  p.n_splits = (max_pages + p.split_pages - 1) / p.split_pages;
+  const int cap = umma ? kSplitPagesUmma / 2 : a.dtype == EAKV_F32 ? kSplitPagesF32 : kSplitPages16;
+  const int least = umma ? kLeastTiles : kLeastPages;
+  const long long resident = (long long)per_sm * sm_count(device), items = tiles * heads;
+  long long run = (units + resident - 1) / resident;
+  if (run < least + overhead) run = least + overhead;
+  // splits that fit on the GPU at once, against a run
+  long long fit = resident / items;
+  if (fit > max_units / least) fit = max_units / least;
+  if (fit < 1) fit = 1;
+  const bool even = items * fit <= resident &&
+                    (max_units + fit - 1) / fit + overhead <= run + run / 8 && (max_units + fit - 1) / fit <= cap;
+  if (t_force_splits == 0 && !even && run <= cap && (units + run - 1) / run <= kMaxRuns) {
+    p.overhead = overhead;
+    p.units = units;
+    p.run = (int)run;
+    p.n_runs = (int)((units + run - 1) / run);
+    // start of every run: walk the tiles
+    long long at = 0;   // units before the tile
+    int r = 0;
+    for (int k = 0; k < p.n_caches; k++)
+      for (int i = p.b.tile0[k]; i < p.b.tile0[k + 1]; i++) {
+        const long long u = (long long)(units_of(k, i) + overhead) * heads;
+        for (; r < p.n_runs && (long long)r * p.run < at + u; r++)
+          p.runs.start[r] = make_int2(i, (int)((long long)r * p.run - at));
+        at += u;
+      }
+    p.slots = p.n_runs > 1 ? 2 * p.n_runs : 0;
+    return EAKV_OK;
+  }
+  int ns = t_force_splits > 0 ? t_force_splits : even ? (int)fit : (max_units + cap - 1) / cap;
+  if (ns > max_units) ns = max_units;
+  p.split_units = (max_units + ns - 1) / ns;
+  p.n_splits = (max_units + p.split_units - 1) / p.split_units;
   if (p.n_splits > 1) {
     if (p.launch_tiles > kSplitItems / heads) p.launch_tiles = kSplitItems / heads;
-    p.records = (size_t)p.launch_tiles * heads * p.n_splits * p.tile_rows *
-                (a.geom.gpd * 64 + 2) * sizeof(float);
+    // bounds the records of a launch
+    while ((long long)p.launch_tiles * heads * p.n_splits * p.tile_rows > (1ll << 22) && p.launch_tiles > 1)
+      p.launch_tiles = (p.launch_tiles + 1) / 2;
+    p.slots = p.launch_tiles * heads * p.n_splits;
   }
-  // a launch's blocks: fewer row tiles per launch where splits would pass 2^30
-  while ((long long)p.launch_tiles * heads * p.n_splits > (1ll << 30) && p.launch_tiles > 1)
-    p.launch_tiles = (p.launch_tiles + 1) / 2;
   return EAKV_OK;
 }
 
+size_t record_bytes(const ExtendArgs &a, const Part &p) {
+  return (size_t)p.slots * p.tile_rows * (a.geom.gpd * 64 + 2) * sizeof(float);
+}
+
 // Workspace bytes of both parts, which run one after the other on it.
-size_t workspace_of(const Part (&p)[2]) {
-  const size_t r = p[0].records > p[1].records ? p[0].records : p[1].records;
+size_t workspace_of(const ExtendArgs &a, const Part (&p)[2]) {
+  const size_t r0 = record_bytes(a, p[0]), r1 = record_bytes(a, p[1]), r = r0 > r1 ? r0 : r1;
   return r ? kCounterBytes + r : 0;
 }
 
@@ -159,7 +206,7 @@ int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const
   DeviceGuard g(caches[0]->device);
   Part p[2];
   for (int k = 0; k < 2 && !rc; k++) rc = plan(a, b, caches[0]->device, tree != 0, k == 0, p[k]);
-  if (!rc) *bytes = workspace_of(p);
+  if (!rc) *bytes = workspace_of(a, p);
   return rc;
 }
 
@@ -198,7 +245,7 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
   for (int k = 0; k < 2 && !rc; k++) rc = plan(a, b, c0->device, tree != nullptr, k == 0, p[k]);
   if (rc) return rc;
   cudaStream_t s = stream ? (cudaStream_t)stream : c0->stream;
-  const size_t need = workspace_of(p);
+  const size_t need = workspace_of(a, p);
   void *data = nullptr;
   if (need && workspace) {
     if (workspace_bytes < need) {
@@ -221,18 +268,22 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
   for (int k = 0; k < 2; k++) {   // the long ones first
     a.n_caches = p[k].n_caches;
     a.tile_rows = p[k].tile_rows;
+    a.unit_pages = p[k].unit_pages;
+    a.run = p[k].run;
+    a.units = p[k].units;
+    a.overhead = p[k].overhead;
     a.n_splits = p[k].n_splits;
-    a.split_pages = p[k].split_pages;
-    const size_t rows = (size_t)p[k].launch_tiles * a.geom.n_heads * a.n_splits * a.tile_rows;
+    a.split_units = p[k].split_units;
+    const size_t rows = (size_t)p[k].slots * a.tile_rows;
     a.part_o = (float *)data;
     a.part_m = a.part_o + rows * c0->head_dim;
     a.part_l = a.part_m + rows;
     for (int t0 = 0; t0 < p[k].tiles && !rc; t0 += p[k].launch_tiles) {
       a.tile_lo = t0;
       a.tile_hi = t0 + p[k].launch_tiles < p[k].tiles ? t0 + p[k].launch_tiles : p[k].tiles;
-      const int blocks = (a.tile_hi - a.tile_lo) * a.geom.n_heads * a.n_splits;
-      rc = p[k].umma ? extend_umma_launch(a, p[k].b, blocks, vec, s)
-                     : extend_mma_launch(a, p[k].b, blocks, vec, s);
+      const int blocks = a.run ? p[k].n_runs : (a.tile_hi - a.tile_lo) * a.geom.n_heads * a.n_splits;
+      rc = p[k].umma ? extend_umma_launch(a, p[k].b, p[k].runs, blocks, vec, s)
+                     : extend_mma_launch(a, p[k].b, p[k].runs, blocks, vec, s);
     }
   }
   return rc;

@@ -3,9 +3,23 @@
 //
 // A row is a (token, query head) pair of one KV head: row r of a cache's KV
 // head h is token r / G, query head h*G + r % G (G query heads per KV head).
-// A work item is (cache, KV head, tile of rows, split): the rows of a tile are
-// neighbours, so their causal limits nearly agree, and every row of the tile
-// is served by the one read of a page.
+// An item is (tile of rows, KV head): the rows of a tile are neighbours, so
+// their causal limits nearly agree, and every row of the tile is served by the
+// one read of a page. An item's positions are counted in units of unit_pages
+// pages.
+//
+// Two ways of cutting the items up. Balanced: all units of all items in one
+// row, cut into as many equal runs as CTAs fit on the GPU at once; a CTA works
+// through the (parts of) items in its run. With whole waves of equal splits
+// instead, the last wave is rarely full: 2048 tokens behind 32768 positions ran
+// 1.40 ms (4 splits, 7 rounds), 1.35 (1 split, 1.7 rounds), 1.06 balanced. An item
+// starts with `overhead' units of nothing, its set-up and results, so that a run of
+// many short items is no longer than one of few long ones. Splits: every item cut
+// into n_splits parts, one CTA each, where these fit on the GPU at once and
+// are no longer than a run would be, or where a run would be longer than the
+// precision of the sums allows.
+// Parts of an item that is cut leave records, which the part that finishes
+// last merges.
 #pragma once
 #include "decode_common.cuh"
 #include "tokens.cuh"
@@ -25,11 +39,15 @@ struct ExtendArgs {
   unsigned wait_budget;
   int test_stall;
   // plan
-  int tile_rows;             // rows of a work item
-  int tile_lo, tile_hi;      // row tiles of this launch
-  int n_splits, split_pages;
-  unsigned *cnt;             // one counter per item, zero between calls
-  float *part_o, *part_m, *part_l;   // [item][split][row of the tile]..., see part_row
+  int tile_rows;             // rows of a tile
+  int unit_pages;
+  int run;                   // balanced: units of a CTA's run (0: splits)
+  int overhead;              // balanced: units that an item counts beyond its own
+  long long units;           // balanced: of all items
+  int tile_lo, tile_hi;      // splits: row tiles of this launch
+  int n_splits, split_units;
+  unsigned *cnt;             // counters of cut items, zero between calls
+  float *part_o, *part_m, *part_l;   // records [slot][row of the tile]...
 };
 
 // The caches of one launch, all with new tokens.
@@ -41,58 +59,160 @@ struct ExtendBatch {
   int tile0[kMaxBatch + 1];  // first row tile of each cache, over one KV head
 };
 
+// Where the runs of a balanced launch start: row tile, and units behind the
+// start of its KV head 0.
+constexpr int kMaxRuns = 768;
+struct ExtendRuns {
+  int2 start[kMaxRuns];
+};
+
+// Positions [lo, hi) that some row of rows [row0, row0 + rows) of a cache may
+// attend, and the pages that hold them.
+struct ExtRange {
+  int lo, hi, pg0, pages;
+};
+__host__ __device__ inline ExtRange extend_range(int row0, int rows, int G, int old, int n_new,
+                                                 int window, bool tree) {
+  ExtRange r;
+  const int t_first = row0 / G, t_last = (row0 + rows - 1) / G;
+  r.lo = window > 0 && old + t_first + 1 > window ? old + t_first + 1 - window : 0;
+  r.hi = tree ? old + n_new : old + t_last + 1;
+  r.pg0 = r.lo / kPagePositions;
+  r.pages = (r.hi + kPagePositions - 1) / kPagePositions - r.pg0;
+  return r;
+}
+
+// A CTA's part of an item.
 struct ExtItem {
-  int b, h, split;
-  int item;        // index without the split
+  int b, h;
   int row0, rows;  // rows of the tile, within the (cache, KV head)
   int old, tok0;   // position of the cache's first new token, its packed index
   int n_new;
   int lo, hi;      // positions that some row of the tile may attend: [lo, hi)
   int all_lo, all_hi;   // positions every row attends: [all_lo, all_hi)
-  int pg0, npages; // pages of this split
+  int pg0, npages; // pages of this part
+  // records: the item's parts, this one's slot, the slots of part p > 0
+  // (slot_p0 + p * slot_step) and of part 0, its counter
+  int n_parts, slot, slot0, slot_p0, slot_step, counter;
+  int state;       // 1: a part, 0: behind the last one, -1: addresses outside the cache
 };
 
-// blockIdx.x -> (tile, head, split), splits fastest, then heads; the last
-// tiles of a prompt, which attend the most, start first.
-__device__ __forceinline__ ExtItem extend_item(const ExtendArgs &a, const ExtendBatch &batch) {
-  ExtItem it;
-  int bid = blockIdx.x;
-  it.split = bid % a.n_splits;
-  it.item = bid / a.n_splits;
-  bid = it.item;
-  it.h = bid % a.geom.n_heads;
-  const int tile = a.tile_hi - 1 - bid / a.geom.n_heads;
-  int lo = 0, hi = a.n_caches - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (batch.tile0[mid] <= tile) lo = mid;
-    else hi = mid - 1;
-  }
-  it.b = lo;
-  it.old = batch.old[lo];
-  it.tok0 = batch.first[lo];
-  it.n_new = batch.n_new[lo];
-  it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
-  it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
-  const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
-  it.lo = a.window > 0 ? max(0, it.old + t_first + 1 - a.window) : 0;
-  it.hi = a.tree ? it.old + it.n_new : it.old + t_last + 1;
-  it.all_lo = a.window > 0 ? max(0, it.old + t_last + 1 - a.window) : 0;
-  it.all_hi = a.tree ? it.old : it.old + t_first + 1;
-  const int P0 = it.lo / kPagePositions;
-  const int P1 = (it.hi + kPagePositions - 1) / kPagePositions;
-  it.pg0 = min(P0 + it.split * a.split_pages, P1);
-  const int pg1 = min(P1, it.pg0 + a.split_pages);
-  it.npages = pg1 > it.pg0 ? pg1 - it.pg0 : 0;
-  return it;
-}
+// A CTA's walk through its parts of items, in shared memory: thread 0 takes the
+// steps, the next one ahead of the barrier that ends a part, so that all threads
+// find it behind that.
+struct ExtWalk {
+  int tile, rem, left;   // next: tile, units behind its KV head 0; units left of the run
+  ExtItem item[2];       // of even and odd parts
 
-__device__ __forceinline__ bool extend_item_ok(const ExtendArgs &a, const ExtItem &it) {
-  const bool ok = it.b >= 0 && it.b < a.n_caches && it.h < a.geom.n_heads && it.rows >= 1 &&
-                  it.row0 >= 0 && it.pg0 >= 0 && it.pg0 + it.npages <= a.geom.n_pages;
-  if (!ok && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
-  return ok;
-}
+  __device__ __forceinline__ void begin(const ExtendArgs &a, const ExtendBatch &batch,
+                                        const ExtendRuns &runs) {
+    if (a.run > 0) {
+      const int2 s = runs.start[blockIdx.x];
+      tile = s.x;
+      rem = s.y;
+      left = (int)min((long long)a.run, a.units - (long long)blockIdx.x * a.run);
+    } else {
+      left = 1;
+    }
+    next(a, batch, 0);
+  }
+
+  // Part `p` into item[p & 1]; false behind the last one.
+  __device__ __forceinline__ bool next(const ExtendArgs &a, const ExtendBatch &batch, int p) {
+    ExtItem &out = item[p & 1];
+    ExtItem it;
+    for (;;) {
+    if (left <= 0) {
+      out.state = 0;
+      return false;
+    }
+    int split = 0, item = 0;
+    if (a.run == 0) {
+      // splits fastest, then heads; the last tiles of a prompt, which attend the
+      // most, start first
+      split = blockIdx.x % a.n_splits;
+      item = blockIdx.x / a.n_splits;
+      it.h = item % a.geom.n_heads;
+      tile = a.tile_hi - 1 - item / a.geom.n_heads;
+    }
+    int lo = 0, hi = a.n_caches - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (batch.tile0[mid] <= tile) lo = mid;
+      else hi = mid - 1;
+    }
+    it.b = lo;
+    it.old = batch.old[lo];
+    it.tok0 = batch.first[lo];
+    it.n_new = batch.n_new[lo];
+    it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
+    it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
+    const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window, a.tree != nullptr);
+    const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
+    it.lo = r.lo;
+    it.hi = r.hi;
+    it.all_lo = a.window > 0 ? max(0, it.old + t_last + 1 - a.window) : 0;
+    it.all_hi = a.tree ? it.old : it.old + t_first + 1;
+    const int units = (r.pages + a.unit_pages - 1) / a.unit_pages;
+    int u0, u1;
+    if (a.run > 0) {
+      // [overhead | units], head after head
+      const int len = a.overhead + units;
+      it.h = rem / len;
+      const int x0 = rem - it.h * len, x1 = min(len, x0 + left);
+      // the item's place in the row of all units: this run's end less what is left
+      const long long end = min((long long)(blockIdx.x + 1) * a.run, a.units);
+      const long long at = end - left - x0 + a.overhead;
+      left -= x1 - x0;
+      rem += x1 - x0;
+      if (rem >= len * a.geom.n_heads) {
+        tile++;
+        rem = 0;
+      }
+      u0 = max(x0 - a.overhead, 0);
+      u1 = x1 - a.overhead;
+      if (u1 <= 0) continue;   // only the item's overhead: another run has its units
+      const int first = (int)(at / a.run), last = (int)((at + units - 1) / a.run);
+      it.n_parts = last - first + 1;
+      // two slots per CTA: a part that begins inside its item, and one that begins it
+      it.slot0 = 2 * first + 1;
+      it.slot_p0 = 2 * first;
+      it.slot_step = 2;
+      it.slot = u0 == 0 ? it.slot0 : 2 * blockIdx.x;
+      it.counter = first;   // only the last item that starts in a run is cut at its end
+    } else {
+      u0 = min(split * a.split_units, units);
+      u1 = min(u0 + a.split_units, units);
+      it.n_parts = a.n_splits;
+      it.slot0 = it.slot_p0 = item * a.n_splits;
+      it.slot_step = 1;
+      it.slot = it.slot0 + split;
+      it.counter = item;
+      left = 0;
+    }
+    it.pg0 = r.pg0 + u0 * a.unit_pages;
+    it.npages = min(u1 * a.unit_pages, r.pages) - u0 * a.unit_pages;
+    if (it.npages < 0) it.npages = 0;
+    const bool ok = it.b >= 0 && it.b < a.n_caches && it.h >= 0 && it.h < a.geom.n_heads && it.rows >= 1 &&
+                    it.row0 >= 0 && it.pg0 >= 0 && it.pg0 + it.npages <= a.geom.n_pages;
+    if (!ok) atomicOr(a.status, kStatusBadIndex);
+    it.state = ok ? 1 : -1;
+    out = it;
+    return true;
+    }
+  }
+
+  // Parts from p on that nobody works on, after a wait ran out or at a bad item:
+  // they arrive all the same, without records, so that the counters are back at
+  // zero after the launch.
+  __device__ __forceinline__ void abandon(const ExtendArgs &a, const ExtendBatch &batch, int p) {
+    for (; item[p & 1].state != 0; p++) {
+      const ExtItem &it = item[p & 1];
+      if (it.n_parts > 1) atomicInc(a.cnt + it.counter, (unsigned)it.n_parts - 1);
+      next(a, batch, p + 1);
+    }
+  }
+};
 
 // What one row attends: positions [lo, hi), and with a tree, of those from
 // `old` on only the ones whose bit is set.
@@ -121,25 +241,30 @@ __device__ __forceinline__ RowMask row_mask(const ExtendArgs &a, const ExtItem &
   return m;
 }
 
-// Partial records of a split: row r of (item, split).
-__device__ __forceinline__ size_t part_row(const ExtendArgs &a, const ExtItem &it, int split, int r) {
-  return ((size_t)it.item * a.n_splits + split) * a.tile_rows + r;
+// Record of row r in a slot, and the slot of part p of the item.
+__device__ __forceinline__ size_t part_row(const ExtendArgs &a, int slot, int r) {
+  return (size_t)slot * a.tile_rows + r;
+}
+__device__ __forceinline__ int part_slot(const ExtItem &it, int p) {
+  return p == 0 ? it.slot0 : it.slot_p0 + p * it.slot_step;
 }
 
-// Arrival of a work item's CTA on its counter, as in decode_common.cuh: true
-// for the last of the item's splits, with the other splits' records visible.
-__device__ __forceinline__ bool extend_arrive_last(const ExtendArgs &a, int item) {
-  __shared__ int s_last;
+// Arrival of a part on its item's counter, as in decode_common.cuh: true for
+// the last of the item's parts, with the other parts' records visible. Called
+// by NT threads that meet on named barrier `id`; *last is shared.
+template <int NT>
+__device__ __forceinline__ bool extend_arrive_last(const ExtendArgs &a, const ExtItem &it, int *last,
+                                                   int id) {
   __threadfence();
-  __syncthreads();
+  named_sync(id, NT);
   if (threadIdx.x == 0) {
-    const unsigned n = (unsigned)a.n_splits;
-    s_last = atomicInc(a.cnt + item, n - 1) == n - 1;
+    const unsigned n = (unsigned)it.n_parts;
+    *reinterpret_cast<volatile int *>(last) = atomicInc(a.cnt + it.counter, n - 1) == n - 1;
   }
-  __syncthreads();
-  const bool last = s_last != 0;
-  if (last) __threadfence();
-  return last;
+  named_sync(id, NT);
+  const bool r = *reinterpret_cast<volatile int *>(last) != 0;
+  if (r) __threadfence();
+  return r;
 }
 
 // Weight of a record with maximum m under the common maximum M. A record
@@ -148,6 +273,28 @@ __device__ __forceinline__ bool extend_arrive_last(const ExtendArgs &a, int item
 __device__ __forceinline__ float part_weight(float m, float M) {
   return m == -INFINITY ? 1.0f : ex2(m - M);
 }
+
+// Element offset of every n-th row of the item's tile in a buffer of rows, from
+// row r on (the last row when that lies behind it), without a division per row.
+struct RowWalk {
+  long long at, plain, wrapped;   // offset; its step, and the step into another token
+  int h, dh, G;                   // query head within the KV head's group, its step
+  __device__ __forceinline__ RowWalk(const ExtendArgs &a, const ExtItem &it, const Rows &b, int r, int n) {
+    const int row = it.row0 + min(r, it.rows - 1), t = row / a.G;
+    G = a.G;
+    h = row - t * G;
+    at = (long long)(it.tok0 + t) * b.token_stride + (long long)(it.h * G + h) * b.head_stride;
+    const int dt = n / G;
+    dh = n - dt * G;
+    plain = dt * b.token_stride + dh * b.head_stride;
+    wrapped = plain + b.token_stride - G * b.head_stride;
+  }
+  __device__ __forceinline__ void step() {
+    const bool wrap = h + dh >= G;
+    at += wrap ? wrapped : plain;
+    h += wrap ? dh - G : dh;
+  }
+};
 
 // Output row of row r of the item's tile.
 template <typename T>
@@ -179,21 +326,20 @@ __device__ __forceinline__ void extend_store(const ExtendArgs &a, const ExtItem 
   if (a.lse && d == 0) extend_lse(a, it, r, M, L);
 }
 
-// The last CTA of an item: rows merged over the splits, in split order, four
-// dims per thread at a time. `ws` is free shared memory of ws_floats: the
-// splits' weights of a row are worked out once into it, and the records' loads
-// then depend on nothing.
+// The last part of an item: rows merged over the parts, in their order, four
+// dims per thread at a time, by NT threads that meet on named barrier `id`. `ws`
+// is free shared memory of ws_floats: the parts' weights of a row are worked out
+// once into it, and the records' loads then depend on nothing.
 template <int HD, typename T, int NT>
 __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem &it, bool vec, float *ws,
-                                             int ws_floats) {
-  const int ns = a.n_splits;
+                                             int ws_floats, int id) {
+  const int ns = it.n_parts;
   float *m_s = ws, *l_s = ws + it.rows, *f_s = ws + 2 * it.rows;   // [rows], [rows], [rows][ns]
   const bool staged = (ns + 2) * it.rows <= ws_floats;
-  __syncthreads();
   if (staged) {
     for (int x = threadIdx.x; x < it.rows * ns; x += NT)
-      f_s[x] = __ldcg(a.part_m + part_row(a, it, x % ns, x / ns));
-    __syncthreads();
+      f_s[x] = __ldcg(a.part_m + part_row(a, part_slot(it, x % ns), x / ns));
+    named_sync(id, NT);
     for (int r = threadIdx.x; r < it.rows; r += NT) {
       float M = -INFINITY, L = 0.0f;
       for (int s = 0; s < ns; s++) M = fmaxf(M, f_s[r * ns + s]);
@@ -201,12 +347,12 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
       for (int s = 0; s < ns; s++) {
         const float f = part_weight(f_s[r * ns + s], M);
         f_s[r * ns + s] = f;
-        L = fmaf(f, __ldcg(a.part_l + part_row(a, it, s, r)), L);
+        L = fmaf(f, __ldcg(a.part_l + part_row(a, part_slot(it, s), r)), L);
       }
       m_s[r] = M;
       l_s[r] = L;
     }
-    __syncthreads();
+    named_sync(id, NT);
   }
   for (int x = threadIdx.x; x < it.rows * (HD / 4); x += NT) {
     const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
@@ -215,12 +361,12 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
       M = m_s[r];
       L = l_s[r];
     } else {
-      for (int s = 0; s < ns; s++) M = fmaxf(M, __ldcg(a.part_m + part_row(a, it, s, r)));
+      for (int s = 0; s < ns; s++) M = fmaxf(M, __ldcg(a.part_m + part_row(a, part_slot(it, s), r)));
     }
     float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = 0; s < ns; s++) {
-      const size_t pr = part_row(a, it, s, r);
+      const size_t pr = part_row(a, part_slot(it, s), r);
       const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + pr * HD + d));
       float f;
       if (staged) {
@@ -238,14 +384,13 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
   }
 }
 
-// extend_mma.cu
-constexpr int kExtendMmaRows = 16;
-int extend_mma_resident(int head_dim, int dtype);
-int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec,
-                      cudaStream_t s);
+// extend_mma.cu: tile_rows 16 or 32
+int extend_mma_resident(int head_dim, int dtype, int tile_rows);
+int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
+                      bool vec, cudaStream_t s);
 // extend_umma.cu: 16-bit types
 constexpr int kExtendUmmaRows = 256;
-int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec,
-                       cudaStream_t s);
+int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
+                       bool vec, cudaStream_t s);
 
 }  // namespace eakv

@@ -29,7 +29,7 @@
 // Non-finite V groups are kept out of the products (0 NaN is NaN) and
 // listed by position; a row that attends one gets NaN in the group's dims.
 //
-// Roles (16 warps, the last three idle). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
+// Roles (16 warps, the last two idle). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
 // per row; the weights go over S, and O is scaled when a maximum moves. Warps 8-11: dequantize, one thread per position: its K
 // and V rows come from global memory a tile ahead in registers and leave as
 // 16-byte stores in the 128-byte swizzle. A 32-bit word of nibbles becomes one
@@ -63,6 +63,8 @@ constexpr int kStages = 2;                    // K and V operands in flight
 constexpr int kInfo = 4;
 constexpr int kSoftWarps = 8, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kWalkWarp = kMmaWarp + 1;
+constexpr int kWorkThreads = (kWalkWarp + 1) * 32;
 constexpr int kThreads = (kSoftWarps + kConvWarps + 4) * 32;   // four warpgroups, the last mostly idle
 // Registers per thread: the launch gives each thread kRegs, and the warpgroups
 // trade them (512 threads x 128 = 128 x (2 kRegsSoft + kRegsConv + kRegsMma)).
@@ -91,10 +93,12 @@ struct WCfg {
   static constexpr int NANS = INFO + kInfo * 16;             // uint2 [kInfo][4 warps]
   static constexpr int ROWC = NANS + kInfo * 32;         // float [256]: score factor of a row
   static constexpr int BARS = ROWC + 256 * 4;
-  static constexpr int SLOT = BARS + 8 * 18;
-  static constexpr int RED = SLOT + 8;                 // int2 [4]
-  static constexpr int END = RED + 32;
+  static constexpr int SLOT = BARS + 8 * 18;           // tensor-memory base, `a wait ran out', merge flag
+  static constexpr int RED = SLOT + 16;                // int2 [4]
+  static constexpr int WALK = RED + 32;                // ExtWalk
+  static constexpr int END = WALK + 256;
   static constexpr int SMEM = END + 1024;              // alignment slack
+  static_assert(sizeof(ExtWalk) <= 256, "room for the walk");
   // tensor memory columns
   static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
   static_assert(BARS % 8 == 0 && ROWC % 16 == 0 && SLOT % 8 == 0, "alignment");
@@ -271,29 +275,16 @@ __device__ __forceinline__ uint32_t mask32(const RowMask &m, int c0, int end) {
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ ExtendBatch batch,
-                   const int vec) {
+                   const __grid_constant__ ExtendRuns runs, const int vec) {
   using C = WCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t bars = smem_u32(smem + C::BARS);
   auto bar = [&](int i) { return bars + 8 * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const ExtItem it = extend_item(a, batch);
-  if (!extend_item_ok(a, it)) {
-    if (a.n_splits > 1) extend_arrive_last(a, it.item);
-    return;
-  }
   const uint32_t budget = min(a.wait_budget, 1u << 18);
-  const int base_pos = it.pg0 * kPagePositions;
-  const int end_pos = (it.pg0 + it.npages) * kPagePositions;   // of this split
-  // tiles of each row tile
-  auto tiles_of = [&](int m) {
-    if (it.rows <= 128 * m) return 0;
-    const int last = min(it.row0 + 128 * m + 127, it.row0 + it.rows - 1);
-    const int hi = min(a.tree ? it.hi : it.old + last / a.G + 1, end_pos);
-    return hi > base_pos ? (hi - base_pos + BN - 1) / BN : 0;
-  };
-  const int nt0 = tiles_of(0), nt1 = tiles_of(1), n_tiles = max(nt0, nt1);
+  ExtWalk &walk = *reinterpret_cast<ExtWalk *>(smem + C::WALK);
+  volatile int *failed = reinterpret_cast<volatile int *>(smem + C::SLOT + 4);
 
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(smem + C::SLOT), C::COLS);
@@ -312,102 +303,12 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     }
     mbar_init(bar(kDrain), 1);
     fence_mbar_init();
-  }
-
-  // ---- dequantizing threads: the first tile, and the references -----------------
-  const int crow = threadIdx.x & 127;             // position row of a converter thread
-  const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, it.pg0) * C::PB +
-                          (size_t)(crow / kPagePositions) * C::PB;
-  const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
-  RawRow<HD> kr, vr;
-  // This thread's row of tile i, zeros when no row of the item may attend it.
-  auto fetch = [&](RawRow<HD> &r, const uint8_t *pages, int i) {
-    const int p = base_pos + i * BN + crow;
-    if (i < n_tiles && p >= it.lo && p < it.hi && p < end_pos) {
-      load_row<HD>(r, pages + (size_t)i * (2 * C::PB), crow % kPagePositions);
-    } else {
-#pragma unroll
-      for (int k = 0; k < HD / 32; k++) r.w[k] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int k = 0; k < 2 * C::NG; k++) r.sb[k] = 0.0f;
-    }
-  };
-  const bool is_conv = warp >= kSoftWarps && warp < kSoftWarps + kConvWarps;
-  if (is_conv) {
-    fetch(kr, kpages, 0);
-    fetch(vr, vpages, 0);
-  }
-
-  // ---- Q' ------------------------------------------------------------------------
-  // A row is HD/8 lanes of eight dims each; its power of two goes into ROWC with
-  // the scale.
-  if (warp < kSoftWarps) {
-    constexpr int LPR = HD / 8, RPW = 32 / LPR;   // lanes per row, rows per warp and step
-    const int d = 8 * (lane % LPR);
-#pragma unroll 8
-    for (int s = 0; s < 32 / RPW; s++) {
-      const int rl = 32 * warp + s * RPW + lane / LPR;
-      const int row = it.row0 + min(rl, it.rows - 1);
-      const T *qp = reinterpret_cast<const T *>(a.q.data) +
-                    (long long)(it.tok0 + row / a.G) * a.q.token_stride +
-                    (long long)(it.h * a.G + row % a.G) * a.q.head_stride + d;
-      float v0[4], v1[4];
-      if (vec) {
-        load4<T, true>(qp, v0);
-        load4<T, true>(qp + 4, v1);
-      } else {
-        load4<T, false>(qp, v0);
-        load4<T, false>(qp + 4, v1);
-      }
-      float mx = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        // NaN counts as an infinity
-        mx = fmaxf(mx, v0[e] == v0[e] ? fabsf(v0[e]) : INFINITY);
-        mx = fmaxf(mx, v1[e] == v1[e] ? fabsf(v1[e]) : INFINITY);
-      }
-#pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const bool fine = mx <= 3.0e38f;
-      int qe = 0;
-      frexpf(mx > 0.0f && fine ? mx : 1.0f, &qe);   // mx in [2^(qe-1), 2^qe)
-      qe = max(min(5 - qe, 126), -126);
-      const float up = (a.scale_log2 < 0.0f ? -1.0f : 1.0f) * pow2i(qe);
-      if (d == 0)
-        reinterpret_cast<float *>(smem + C::ROWC)[rl] =
-            fine ? fabsf(a.scale_log2) * pow2i(-qe) : __uint_as_float(0x7fc00000u);
-      if (!fine) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v0[e] = v1[e] = 0.0f;
-      }
-      // dims d..d+3 and d+4..d+7: the low or high halves of chunks j and j + 1
-      const int rr = rl & 127, j = (d & 31) >> 2;
-      uint8_t *op = smem + C::Q + (rl >> 7) * C::QTILE + (d >> 6) * C::QHALF + rr * 128 + ((d & 32) >> 2);
-      *reinterpret_cast<uint2 *>(op + ((j ^ (rr & 7)) << 4)) =
-          make_uint2(pack_f16(v0[0] * up, v0[2] * up), pack_f16(v0[1] * up, v0[3] * up));
-      *reinterpret_cast<uint2 *>(op + (((j + 1) ^ (rr & 7)) << 4)) =
-          make_uint2(pack_f16(v1[0] * up, v1[2] * up), pack_f16(v1[1] * up, v1[3] * up));
-    }
-    fence_proxy_async_smem();
-  }
-  if (is_conv) {
-    uint32_t bad;
-    const int ek = __reduce_max_sync(0xffffffffu, row_exp<HD>(kr, bad));
-    const int ev = __reduce_max_sync(0xffffffffu, row_exp<HD>(vr, bad));
-    if (lane == 0) reinterpret_cast<int2 *>(smem + C::RED)[warp - kSoftWarps] = make_int2(ek, ev);
+    *failed = 0;
+    walk.begin(a, batch, runs);
   }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  int kref = kUnset, vref = kUnset;
-#pragma unroll
-  for (int w = 0; w < kConvWarps; w++) {
-    const int2 e = reinterpret_cast<const int2 *>(smem + C::RED)[w];
-    kref = max(kref, e.x);
-    vref = max(vref, e.y);
-  }
-  if (kref == kUnset) kref = 0;
-  if (vref == kUnset) vref = 0;
   const uint32_t tm = *reinterpret_cast<const uint32_t *>(smem + C::SLOT);
 
   // Bounded wait of a whole warp for use `use` of barrier b (how often it was
@@ -415,50 +316,121 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
   bool ok = true;
   auto wait_warp = [&](int b, int use) {
     if (!__all_sync(0xffffffffu, mbar_wait_sleep(bar(b), use & 1, budget))) {
-      if (lane == 0) atomicOr(a.status, kStatusWaitTimeout);
+      if (lane == 0) {
+        atomicOr(a.status, kStatusWaitTimeout);
+        *failed = 1;
+      }
       ok = false;
     }
     return ok;
   };
+  // Every role walks the same parts of items. They meet twice in each: when Q'
+  // and the references are there, and when nothing of the part is in use any
+  // more.
+  auto meet = [&] { named_sync(3, kWorkThreads); };
+  // Positions of part p, and its tiles for each row tile; false behind the last
+  // part, or at one outside its cache.
+  int base_pos, end_pos, nt0, nt1, n_tiles;
+  auto begin_part = [&](const ExtItem &it) {
+    if (it.state <= 0) return false;
+    base_pos = it.pg0 * kPagePositions;
+    end_pos = (it.pg0 + it.npages) * kPagePositions;
+    auto tiles_of = [&](int m) {
+      if (it.rows <= 128 * m) return 0;
+      const int last = min(it.row0 + 128 * m + 127, it.row0 + it.rows - 1);
+      const int hi = min(a.tree ? it.hi : it.old + last / a.G + 1, end_pos);
+      return hi > base_pos ? (hi - base_pos + BN - 1) / BN : 0;
+    };
+    nt0 = tiles_of(0);
+    nt1 = tiles_of(1);
+    n_tiles = max(nt0, nt1);
+    return true;
+  };
+  // references of the part, from the dequantizing warps' maxima
+  int kref, vref;
+  auto references = [&] {
+    kref = vref = kUnset;
+#pragma unroll
+    for (int w = 0; w < kConvWarps; w++) {
+      const int2 e = reinterpret_cast<const int2 *>(smem + C::RED)[w];
+      kref = max(kref, e.x);
+      vref = max(vref, e.y);
+    }
+    if (kref == kUnset) kref = 0;
+    if (vref == kUnset) vref = 0;
+  };
 
-  if (is_conv) {
+  if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ================= dequantize ================================================
     regs_down<kRegsConv>();
     regs_traded();
-    const int cw = warp - kSoftWarps;
-    for (int i = 0; i < n_tiles; i++) {
-      const int st = i & 1;
-      uint32_t kbad, vbad;
-      const int ke = row_exp<HD>(kr, kbad), ve = row_exp<HD>(vr, vbad);
-      const bool mark = __any_sync(0xffffffffu, (ke != kUnset && (ke > kref + kUp || ke < kref - kDown)) ||
-                                                    (ve != kUnset && (ve > vref + kUp || ve < vref - kDown)));
-      const int kx = mark && ke != kUnset ? ke : kref, vx = mark && ve != kUnset ? ve : vref;
-      // a non-finite K group keeps its NaN, which reaches its own score only; a V
-      // group is listed instead
-      const uint32_t n0 = __ballot_sync(0xffffffffu, vbad & 1), n1 = __ballot_sync(0xffffffffu, vbad & 2);
-      if (i >= 2 && !wait_warp(kKFree + st, (i >> 1) - 1)) break;
-      if (mark) reinterpret_cast<short2 *>(smem + C::EXPS)[(i % kInfo) * BN + crow] = make_short2(kx, vx);
-      if (lane == 0) {
-        reinterpret_cast<int *>(smem + C::INFO)[(i % kInfo) * 4 + cw] = (mark ? 1 : 0) | ((n0 | n1) ? 2 : 0);
-        reinterpret_cast<uint2 *>(smem + C::NANS)[(i % kInfo) * 4 + cw] = make_uint2(n0, n1);
+    const int cw = warp - kSoftWarps, crow = threadIdx.x & 127;   // its position in a tile
+    int done = 0;   // tiles of the parts before
+    for (int part = 0;; part++) {
+      const ExtItem &it = walk.item[part & 1];
+      if (!begin_part(it)) break;
+      const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, it.pg0) * C::PB +
+                              (size_t)(crow / kPagePositions) * C::PB;
+      const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
+      RawRow<HD> kr, vr;
+      // This thread's row of tile i, zeros when no row of the item may attend it.
+      auto fetch = [&](RawRow<HD> &r, const uint8_t *pages, int i) {
+        const int p = base_pos + i * BN + crow;
+        if (i < n_tiles && p >= it.lo && p < it.hi && p < end_pos) {
+          load_row<HD>(r, pages + (size_t)i * (2 * C::PB), crow % kPagePositions);
+        } else {
+#pragma unroll
+          for (int k = 0; k < HD / 32; k++) r.w[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 2 * C::NG; k++) r.sb[k] = 0.0f;
+        }
+      };
+      fetch(kr, kpages, 0);
+      fetch(vr, vpages, 0);
+      uint32_t bad;
+      const int ek = __reduce_max_sync(0xffffffffu, row_exp<HD>(kr, bad));
+      const int ev = __reduce_max_sync(0xffffffffu, row_exp<HD>(vr, bad));
+      if (lane == 0) reinterpret_cast<int2 *>(smem + C::RED)[cw] = make_int2(ek, ev);
+      meet();
+      references();
+      for (int i = 0; i < n_tiles; i++) {
+        const int n = done + i, st = n & 1;
+        uint32_t kbad, vbad;
+        const int ke = row_exp<HD>(kr, kbad), ve = row_exp<HD>(vr, vbad);
+        const bool mark = __any_sync(0xffffffffu, (ke != kUnset && (ke > kref + kUp || ke < kref - kDown)) ||
+                                                      (ve != kUnset && (ve > vref + kUp || ve < vref - kDown)));
+        const int kx = mark && ke != kUnset ? ke : kref, vx = mark && ve != kUnset ? ve : vref;
+        // a non-finite K group keeps its NaN, which reaches its own score only; a V
+        // group is listed instead
+        const uint32_t n0 = __ballot_sync(0xffffffffu, vbad & 1), n1 = __ballot_sync(0xffffffffu, vbad & 2);
+        if (n >= 2 && !wait_warp(kKFree + st, (n >> 1) - 1)) break;
+        if (mark) reinterpret_cast<short2 *>(smem + C::EXPS)[(n % kInfo) * BN + crow] = make_short2(kx, vx);
+        if (lane == 0) {
+          reinterpret_cast<int *>(smem + C::INFO)[(n % kInfo) * 4 + cw] = (mark ? 1 : 0) | ((n0 | n1) ? 2 : 0);
+          reinterpret_cast<uint2 *>(smem + C::NANS)[(n % kInfo) * 4 + cw] = make_uint2(n0, n1);
+        }
+        store_row<HD>(kr, smem + C::K + st * C::TILE, crow, kx, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kKFull + st));
+        fetch(kr, kpages, i + 1);
+        if (n >= 2 && !wait_warp(kVFree + st, (n >> 1) - 1)) break;
+        store_row<HD>(vr, smem + C::V + st * C::TILE, crow, vx, vbad);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kVFull + st));
+        fetch(vr, vpages, i + 1);
       }
-      store_row<HD>(kr, smem + C::K + st * C::TILE, crow, kx, 0u);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kKFull + st));
-      fetch(kr, kpages, i + 1);
-      if (i >= 2 && !wait_warp(kVFree + st, (i >> 1) - 1)) break;
-      store_row<HD>(vr, smem + C::V + st * C::TILE, crow, vx, vbad);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kVFull + st));
-      fetch(vr, vpages, i + 1);
+      done += n_tiles;
+      meet();
+      if (*failed) break;
     }
   } else if (warp >= kMmaWarp) {
     // ================= MMAs ======================================================
     regs_down<kRegsMma>();
     regs_traded();
     if (warp == kMmaWarp) {
+    int done = 0, done0 = 0, done1 = 0;   // tiles of the parts before, of each row tile
     // The whole warp walks the tiles, so that descriptors stay in uniform
     // registers; one lane issues.
     const bool issuer = elect_one();
@@ -468,7 +440,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     const uint64_t vd = sdesc(sb + C::V, C::HALF, 1024, kLayoutSW128);
     // a descriptor's address field counts 16 bytes
     auto scores = [&](int m, int i) {
-      const uint64_t q = qd + (uint64_t)(m * (C::QTILE >> 4)), k = kd + (uint64_t)((i & 1) * (C::TILE >> 4));
+      const uint64_t q = qd + (uint64_t)(m * (C::QTILE >> 4)), k = kd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
       const uint32_t d = tm + C::S_COL + 128 * m;
       if (issuer) {
 #pragma unroll
@@ -478,16 +450,16 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         }
         if (i != a.test_stall - 1) mma_commit(bar(kSFull + m));   // test hook: never ready
         // the tile's K is free when the last row tile that uses it has its scores
-        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kKFree + (i & 1)));
+        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kKFree + ((done + i) & 1)));
       }
     };
     // PV of tile i, half by half as the weights come; false when a wait ran out
     auto outputs = [&](int m, int i, int n) {
-      const uint64_t v = vd + (uint64_t)((i & 1) * (C::TILE >> 4));
+      const uint64_t v = vd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
       const uint32_t p = tm + C::S_COL + 128 * m, d = tm + C::O_COL + HD * m;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        if (!wait_warp(kPFull + 2 * m + h, i)) return false;
+        if (!wait_warp(kPFull + 2 * m + h, (m ? done1 : done0) + i)) return false;
         fence_after_sync();
         if (issuer) {
 #pragma unroll
@@ -496,21 +468,25 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         }
       }
       if (issuer) {
-        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kVFree + (i & 1)));
+        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kVFree + ((done + i) & 1)));
         if (i == n - 1) mma_commit(bar(kODone + m));
       }
       return true;
     };
     // Each tile's K and V is waited for once, ahead of the weights that it is
     // used behind, so that nothing stands between these and their MMAs.
-    if (n_tiles > 0 && wait_warp(kKFull, 0)) {
+    for (int part = 0;; part++) {
+      const ExtItem &it = walk.item[part & 1];
+      if (!begin_part(it)) break;
+    meet();
+    if (n_tiles > 0 && wait_warp(kKFull + (done & 1), done >> 1)) {
       fence_after_sync();
       if (nt0 > 0) scores(0, 0);
       if (nt1 > 0) scores(1, 0);
     }
     for (int i = 0; i < n_tiles && ok; i++) {
-      if (i + 1 < n_tiles && !wait_warp(kKFull + ((i + 1) & 1), (i + 1) >> 1)) break;
-      if (!wait_warp(kVFull + (i & 1), i >> 1)) break;
+      if (i + 1 < n_tiles && !wait_warp(kKFull + ((done + i + 1) & 1), (done + i + 1) >> 1)) break;
+      if (!wait_warp(kVFull + ((done + i) & 1), (done + i) >> 1)) break;
       if (i < nt0) {
         if (!outputs(0, i, nt0)) break;
         if (i + 1 < nt0) scores(0, i + 1);
@@ -520,16 +496,103 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         if (i + 1 < nt1) scores(1, i + 1);
       }
     }
+    done += n_tiles;
+    done0 += nt0;
+    done1 += nt1;
+    meet();
+    if (*failed) break;
+    }
     // every MMA has ended before the tensor memory is given back
     if (issuer) mma_commit(bar(kDrain));
     __syncwarp();
     wait_warp(kDrain, 0);
+    } else if (warp == kWalkWarp) {
+      // ================= walk: the next part, while this one is worked on ===========
+      int part = 0;
+      for (; walk.item[part & 1].state > 0; part++) {
+        meet();
+        if (lane == 0) walk.next(a, batch, part + 1);
+        meet();
+        if (*failed) {
+          const ExtItem &it = walk.item[part & 1];
+          const bool arrived = it.n_parts == 1 || *reinterpret_cast<volatile int *>(smem + C::SLOT + 12);
+          if (lane == 0 && !arrived) atomicInc(a.cnt + it.counter, (unsigned)it.n_parts - 1);
+          part++;
+          break;
+        }
+      }
+      if (lane == 0) walk.abandon(a, batch, part);
     }
   } else {
     // ================= softmax: one row per thread ===============================
     regs_up<kRegsSoft>();
     regs_traded();
     const int mt = warp >> 2;                            // row tile
+    // tiles of the parts before: of this row tile, of both; parts with tiles
+    int done = 0, all_done = 0, parts = 0;
+    for (int part = 0;; part++) {
+      const ExtItem &it = walk.item[part & 1];
+      if (!begin_part(it)) break;
+      // ---- Q' ----------------------------------------------------------------------
+      // A row is HD/8 lanes of eight dims each; its power of two goes into ROWC
+      // with the scale. Rows behind the last repeat it.
+      {
+        constexpr int LPR = HD / 8, RPW = 32 / LPR;   // lanes per row, rows per warp and step
+        const int d = 8 * (lane % LPR);
+        const int rl0 = 32 * warp + lane / LPR;
+        RowWalk row(a, it, a.q, rl0, RPW);
+        const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        const int j = (d & 31) >> 2;
+        uint8_t *op = smem + C::Q + mt * C::QTILE + (d >> 6) * C::QHALF + ((d & 32) >> 2);
+        // kBatch rows' loads before the first is looked at
+        auto rows = [&](auto vec_tag) {
+          constexpr int kBatch = 8;
+#pragma unroll 1
+          for (int s0 = 0; s0 < 32 / RPW; s0 += kBatch) {
+            float v[kBatch][2][4];
+#pragma unroll
+            for (int s = 0; s < kBatch; s++) {
+              const T *qp = reinterpret_cast<const T *>(a.q.data) + row.at + d;
+              load4<T, decltype(vec_tag)::value>(qp, v[s][0]);
+              load4<T, decltype(vec_tag)::value>(qp + 4, v[s][1]);
+              if (rl0 + (s0 + s + 1) * RPW < it.rows) row.step();
+            }
+#pragma unroll
+            for (int s = 0; s < kBatch; s++) {
+              const int rl = rl0 + (s0 + s) * RPW, rr = rl & 127;
+              float (&v0)[4] = v[s][0], (&v1)[4] = v[s][1];
+              // largest magnitude as bits: infinities and NaN come out on top
+              uint32_t mx = 0;
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                mx = max(mx, max(__float_as_uint(v0[e]) & 0x7fffffffu, __float_as_uint(v1[e]) & 0x7fffffffu));
+#pragma unroll
+              for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const bool fine = mx < 0x7f800000u;
+              // mx in [2^(e-1), 2^e), e = (mx >> 23) - 126; times 2^(5 - e)
+              const int qe = mx == 0 || !fine ? 0 : max(min(131 - (int)(mx >> 23), 126), -126);
+              const float up = fine ? sign * pow2i(qe) : 0.0f;
+              if (d == 0)
+                reinterpret_cast<float *>(smem + C::ROWC)[rl] =
+                    fine ? fabsf(a.scale_log2) * pow2i(-qe) : __uint_as_float(0x7fc00000u);
+              if (!fine) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v0[e] = v1[e] = 0.0f;
+              }
+              // dims d..d+3 and d+4..d+7: the low or high halves of chunks j and j + 1
+              *reinterpret_cast<uint2 *>(op + rr * 128 + ((j ^ (rr & 7)) << 4)) =
+                  make_uint2(pack_f16(v0[0] * up, v0[2] * up), pack_f16(v0[1] * up, v0[3] * up));
+              *reinterpret_cast<uint2 *>(op + rr * 128 + (((j + 1) ^ (rr & 7)) << 4)) =
+                  make_uint2(pack_f16(v1[0] * up, v1[2] * up), pack_f16(v1[1] * up, v1[3] * up));
+            }
+          }
+        };
+        if (vec) rows(std::true_type{});
+        else rows(std::false_type{});
+        fence_proxy_async_smem();
+      }
+    meet();
+    references();
     const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
     const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
     // score factor: |scale| log2 e / 2^(q exponent), with K's 2^kref
@@ -646,7 +709,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     // Any tile: every position with its own powers of two.
     auto tile_slow = [&](int i, int marks) {
       const int c0 = base_pos + i * BN;
-      const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + (i % kInfo) * BN;
+      const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + ((all_done + i) % kInfo) * BN;
       float mx = -INFINITY;
       int emax = kUnset;
 #pragma unroll 1
@@ -701,15 +764,15 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     };
 
     for (int i = 0; i < my_tiles; i++) {
-      if (!wait_warp(kSFull + mt, i)) break;
+      if (!wait_warp(kSFull + mt, done + i)) break;
       fence_after_sync();
       const int c0 = base_pos + i * BN;
       const bool full = c0 >= all_lo && c0 + BN <= all_hi;
       // bit 0 of a warp's word: marked rows, bit 1: non-finite V groups
-      const int4 sum = *reinterpret_cast<const int4 *>(smem + C::INFO + (i % kInfo) * 16);
+      const int4 sum = *reinterpret_cast<const int4 *>(smem + C::INFO + ((all_done + i) % kInfo) * 16);
       const int any = sum.x | sum.y | sum.z | sum.w;
       if (any & 2) {
-        const uint2 *bad = reinterpret_cast<const uint2 *>(smem + C::NANS) + (i % kInfo) * 4;
+        const uint2 *bad = reinterpret_cast<const uint2 *>(smem + C::NANS) + ((all_done + i) % kInfo) * 4;
         for (int w = 0; w < 4; w++) {
           const uint32_t on = mask32(mask, c0 + 32 * w, end_pos);
           poison0 = poison0 || (on & bad[w].x);
@@ -727,7 +790,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     }
 
     // ---- results ----------------------------------------------------------------
-    if (ok && my_tiles > 0) wait_warp(kODone + mt, 0);
+    if (ok && my_tiles > 0) wait_warp(kODone + mt, parts);
     // both row tiles are through with K' and V': their space takes the rows on
     // their way out
     named_sync(1, kSoftWarps * 32);
@@ -737,11 +800,11 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       const float L = l_run * down;
       // O carries 2^(kPShift - eref); in two factors. Finished rows are divided here.
       const int e = eref == kUnset ? 0 : eref;
-      const float inv = a.n_splits > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
+      const float inv = it.n_parts > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
       const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1)) * inv;
       if (r_loc < it.rows) {
-        if (a.n_splits > 1) {
-          const size_t pr = part_row(a, it, it.split, r_loc);
+        if (it.n_parts > 1) {
+          const size_t pr = part_row(a, it.slot, r_loc);
           a.part_m[pr] = m_run;
           a.part_l[pr] = L;
         } else if (a.lse) {
@@ -752,11 +815,12 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       // stored: up to 256 bytes of a row at a time, 32 rows per warp.
       uint8_t *stage = smem + C::K + warp * (32 * 256);
       static_assert(8 * 32 * 256 <= 2 * kStages * C::TILE, "room for the rows of eight warps");
-      const int esize = a.n_splits > 1 ? 4 : 2, per_pass = a.n_splits > 1 ? 64 : HD;
+      const int per_pass = it.n_parts > 1 ? 64 : HD;
+      const bool spoiled = __any_sync(0xffffffffu, poison0 || poison1);
 #pragma unroll 1
       for (int d0 = 0; d0 < HD; d0 += per_pass) {
         // 16 columns: dims 4j..4j+7 and 32 on of a 64-dim group
-#pragma unroll 1
+#pragma unroll 2
         for (int j = d0 / 8; j < (d0 + per_pass) / 8; j += 2) {
           uint32_t v[16];
           if (my_tiles > 0) {
@@ -766,11 +830,13 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
 #pragma unroll
             for (int k = 0; k < 16; k++) v[k] = 0u;
           }
-          const bool bad = j < 8 ? poison0 : poison1;
           float o[16];
 #pragma unroll
-          for (int k = 0; k < 16; k++)
-            o[k] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float(v[k]) * f0 * f1;
+          for (int k = 0; k < 16; k++) o[k] = __uint_as_float(v[k]) * f0 * f1;
+          if (spoiled && (j < 8 ? poison0 : poison1)) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = __uint_as_float(0x7fc00000u);
+          }
           const float lo[8] = {o[0], o[2], o[1], o[3], o[8], o[10], o[9], o[11]};
           const float hi[8] = {o[4], o[6], o[5], o[7], o[12], o[14], o[13], o[15]};
           const int d = 64 * (j >> 3) + 4 * (j & 7) - d0;   // within the pass
@@ -778,7 +844,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
           auto put = [&](int byte, uint4 x) {
             *reinterpret_cast<uint4 *>(stage + lane * 256 + ((byte + 16 * lane) & 255)) = x;
           };
-          if (a.n_splits > 1) {
+          if (it.n_parts > 1) {
 #pragma unroll
             for (int k = 0; k < 8; k += 4) {
               put(4 * (d + k), make_uint4(__float_as_uint(lo[k]), __float_as_uint(lo[k + 1]),
@@ -794,16 +860,24 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
           }
         }
         __syncwarp();
-        const int cpr = per_pass * esize / 16;   // chunks per row: 8 or 16
+        // whole rows again: a lane's chunk of rows rr0, rr0 + rows per step, ...
+        const bool record = it.n_parts > 1;
+        const int cpr = record ? 16 : HD / 8;   // chunks of a row
+        const int ch = lane & (cpr - 1), step = 32 / cpr, rr0 = lane / cpr;
+        const int n_rows = it.rows - 32 * warp;   // of this warp (row tiles are 4 warps of 32 rows)
+        float *po = a.part_o + part_row(a, it.slot, 32 * warp) * HD + d0 + 4 * ch;
+        RowWalk row(a, it, a.out, 32 * warp + rr0, step);
+        auto chunk = [&](int rr) {
+          return *reinterpret_cast<const uint4 *>(stage + rr * 256 + ((16 * ch + 16 * rr) & 255));
+        };
+        if (record) {
 #pragma unroll 4
-        for (int x = lane; x < 32 * cpr; x += 32) {
-          const int rr = x / cpr, ch = x % cpr, r = 128 * mt + 32 * (warp & 3) + rr;
-          if (r >= it.rows) continue;
-          const uint4 y = *reinterpret_cast<const uint4 *>(stage + rr * 256 + ((16 * ch + 16 * rr) & 255));
-          if (a.n_splits > 1) {
-            *reinterpret_cast<uint4 *>(a.part_o + part_row(a, it, it.split, r) * HD + d0 + 4 * ch) = y;
-          } else {
-            T *p = extend_out<T>(a, it, r) + 8 * ch;
+          for (int rr = rr0; rr < min(32, n_rows); rr += step) *reinterpret_cast<uint4 *>(po + rr * HD) = chunk(rr);
+        } else {
+#pragma unroll 4
+          for (int rr = rr0; rr < min(32, n_rows); rr += step) {
+            T *p = reinterpret_cast<T *>(a.out.data) + row.at + 8 * ch;
+            const uint4 y = chunk(rr);
             if (vec) {
               // 8-byte pieces: rows start on 4-element boundaries
               reinterpret_cast<uint2 *>(p)[0] = make_uint2(y.x, y.y);
@@ -813,27 +887,40 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
 #pragma unroll
               for (int k = 0; k < 8; k++) p[k] = e8[k];
             }
+            row.step();
           }
         }
         __syncwarp();
       }
     }
+    if (it.n_parts > 1) {
+      // warps that gave up leave their mark ahead of this barrier
+      volatile int *said = reinterpret_cast<volatile int *>(smem + C::SLOT + 12);
+      named_sync(1, kSoftWarps * 32);
+      if (threadIdx.x == 0) *said = !*failed;
+      named_sync(1, kSoftWarps * 32);
+      if (*said && extend_arrive_last<kSoftWarps * 32>(a, it, reinterpret_cast<int *>(smem + C::SLOT + 8), 1))
+        extend_merge<HD, T, kSoftWarps * 32>(a, it, vec, reinterpret_cast<float *>(smem + C::K),
+                                             2 * kStages * C::TILE / 4, 1);
+    }
+    done += my_tiles;
+    all_done += n_tiles;
+    parts += my_tiles > 0;
     fence_before_sync();
+    meet();
+    fence_after_sync();
+    if (*failed) break;
+    }
     regs_down<kRegs>();
   }
   if (warp >= kSoftWarps) regs_up<kRegs>();   // given back by the softmax warps
-  const bool all_ok = __syncthreads_and(ok);
-  fence_after_sync();
+  __syncthreads();
   if (warp == kMmaWarp) tmem_dealloc(tm, C::COLS);
-  if (a.n_splits > 1) {
-    const bool last = extend_arrive_last(a, it.item);
-    if (last && all_ok)
-      extend_merge<HD, T, kThreads>(a, it, vec, reinterpret_cast<float *>(smem), C::EXPS / 4);
-  }
 }
 
 template <int HD, typename T>
-int launch_one(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec, cudaStream_t s) {
+int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks, bool vec,
+               cudaStream_t s) {
   using C = WCfg<HD>;
   auto fn = extend_umma_kernel<HD, T>;
   static std::atomic<unsigned long long> attr_done{0};   // one bit per device
@@ -854,19 +941,19 @@ int launch_one(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec
     }
     attr_done.fetch_or(1ull << (dev & 63), std::memory_order_acq_rel);
   }
-  fn<<<n_blocks, kThreads, C::SMEM, s>>>(a, b, vec ? 1 : 0);
+  fn<<<n_blocks, kThreads, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
   return check_cuda(cudaGetLastError(), "extend_umma launch");
 }
 
 }  // namespace
 
-int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, int n_blocks, bool vec,
-                       cudaStream_t s) {
+int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
+                       bool vec, cudaStream_t s) {
   if (a.geom.gpd == 2)
-    return a.dtype == EAKV_F16 ? launch_one<128, __half>(a, b, n_blocks, vec, s)
-                               : launch_one<128, __nv_bfloat16>(a, b, n_blocks, vec, s);
-  return a.dtype == EAKV_F16 ? launch_one<64, __half>(a, b, n_blocks, vec, s)
-                             : launch_one<64, __nv_bfloat16>(a, b, n_blocks, vec, s);
+    return a.dtype == EAKV_F16 ? launch_one<128, __half>(a, b, runs, n_blocks, vec, s)
+                               : launch_one<128, __nv_bfloat16>(a, b, runs, n_blocks, vec, s);
+  return a.dtype == EAKV_F16 ? launch_one<64, __half>(a, b, runs, n_blocks, vec, s)
+                             : launch_one<64, __nv_bfloat16>(a, b, runs, n_blocks, vec, s);
 }
 
 }  // namespace eakv
