@@ -117,8 +117,11 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
   long long fit = resident / items;
   if (fit > max_units / least) fit = max_units / least;
   if (fit < 1) fit = 1;
-  const bool even = items * fit <= resident &&
-                    (max_units + fit - 1) / fit + overhead <= run + run / 8 && (max_units + fit - 1) / fit <= cap;
+  // or whole items, where there are enough of them for the last to end together
+  // (at 4.5 items per CTA 136 us against 187 in runs, at 1.7 1.14 ms against 1.05)
+  const bool even = (items * fit <= resident && (max_units + fit - 1) / fit + overhead <= run + run / 8 &&
+                     (max_units + fit - 1) / fit <= cap) ||
+                    (items >= 4 * resident && max_units <= cap);
   if (t_force_splits == 0 && !even && run <= cap && (units + run - 1) / run <= kMaxRuns) {
     p.overhead = overhead;
     p.units = units;

@@ -209,7 +209,7 @@ typedef struct {
 /* Rotary positions. The first rot_dim dims of a head (a multiple of 8) are
  * rot_dim/2 pairs: (i, i + rot_dim/2), or (2i, 2i+1) when interleaved. Pair
  * i of a token turns by the angle whose cosine and sine are at
- * [position][i] of the f32 tables [n_rows][rot_dim/2], with the token's
+ * [position][i] of the f32 tables [n_rows][rot_dim/2] (16-byte aligned), with the token's
  * position on the axis that pair i follows: the first sections[0] pairs
  * follow axis 0, the next sections[1] axis 1, and so on (one axis for text;
  * time, height and width for images and video). positions is device
