@@ -121,8 +121,10 @@ __device__ __forceinline__ float quantize4(const float (&x)[16], uint8_t *pp, ui
   if (__all_sync(0xffffffffu, tame && !nan)) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const uint32_t lo = __float_as_uint(__fadd_rz(__fadd_rn(__fmul_rn(__fsub_rn(x[e], mn), inv), 0.5f), 8388608.0f));
-      const uint32_t hi = __float_as_uint(__fadd_rz(__fadd_rn(__fmul_rn(__fsub_rn(x[8 + e], mn), inv), 0.5f), 8388608.0f));
+      const float q0 = __fadd_rn(__fmul_rn(__fsub_rn(x[e], mn), inv), 0.5f);
+      const float q1 = __fadd_rn(__fmul_rn(__fsub_rn(x[8 + e], mn), inv), 0.5f);
+      const uint32_t lo = __float_as_uint(__fadd_rz(q0, 8388608.0f));
+      const uint32_t hi = __float_as_uint(__fadd_rz(q1, 8388608.0f));
       // lo and hi are 0x4B00000q: byte e of the word is 16 q_hi + q_lo
       w[e >> 2] += ((hi << 4) + lo) << (8 * (e & 3));
     }

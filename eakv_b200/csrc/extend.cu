@@ -27,7 +27,6 @@ constexpr int kSplitPagesF32 = 64, kSplitPages16 = 256, kSplitPagesUmma = 1024;
 // Rows (new tokens x query heads per KV head) up to which 16-bit calls take the
 // warp-level kernel.
 constexpr int kMmaRows = 32;
-constexpr int kTile = 16;
 // Shortest parts worth a CTA, and what an item costs beyond its positions (set-up,
 // results), in pages of the warp-level kernel and tiles of the tcgen05 kernel.
 constexpr int kLeastPages = 6, kLeastTiles = 4;
@@ -55,16 +54,12 @@ int sm_count(int dev) {
 // bytes. Call with the caches' device current.
 int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool umma, Part &p) {
   p.umma = umma;
-  // the warp-level kernel's tiles: 32 rows where a cache has more than 16 (a page
-  // is converted once for a tile)
-  p.tile_rows = umma ? kExtendUmmaRows : 16;
+  p.tile_rows = umma ? kExtendUmmaRows : kExtendMmaRows;
   auto mine = [&](int i) {
     const long long rows = (long long)(t.first[i + 1] - t.first[i]) * a.G;
     const bool many = a.dtype != EAKV_F32 && t_force_path != 2 && (rows > kMmaRows || t_force_path == 3);
     return rows > 0 && many == umma;
   };
-  for (int i = 0; i < a.n_caches && !umma; i++)
-    if (mine(i) && (long long)(t.first[i + 1] - t.first[i]) * a.G > 16) p.tile_rows = kTile;
   p.n_caches = 0;
   p.slots = p.run = p.n_runs = p.overhead = 0;
   p.units = 0;
@@ -106,7 +101,7 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
       units += (long long)(u + overhead) * heads;
       if (u > max_units) max_units = u;
     }
-  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype, p.tile_rows);
+  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype);
   if (per_sm <= 0) return EAKV_ERR_INVALID;   // recorded by the lookup
   const int cap = umma ? kSplitPagesUmma / 2 : a.dtype == EAKV_F32 ? kSplitPagesF32 : kSplitPages16;
   const int least = umma ? kLeastTiles : kLeastPages;

@@ -122,93 +122,93 @@ struct ExtWalk {
     ExtItem &out = item[p & 1];
     ExtItem it;
     for (;;) {
-    if (left <= 0) {
-      out.state = 0;
-      return false;
-    }
-    int split = 0, item = 0;
-    if (a.run == 0) {
-      // splits fastest, then heads; the last tiles of a prompt, which attend the
-      // most, start first
-      split = blockIdx.x % a.n_splits;
-      item = blockIdx.x / a.n_splits;
-      it.h = item % a.geom.n_heads;
-      tile = a.tile_hi - 1 - item / a.geom.n_heads;
-    }
-    int lo = 0, hi = a.n_caches - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (batch.tile0[mid] <= tile) lo = mid;
-      else hi = mid - 1;
-    }
-    it.b = lo;
-    it.old = batch.old[lo];
-    it.tok0 = batch.first[lo];
-    it.n_new = batch.n_new[lo];
-    it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
-    it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
-    const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window, a.tree != nullptr);
-    const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
-    it.lo = r.lo;
-    it.hi = r.hi;
-    it.all_lo = a.window > 0 ? max(0, it.old + t_last + 1 - a.window) : 0;
-    it.all_hi = a.tree ? it.old : it.old + t_first + 1;
-    const int units = (r.pages + a.unit_pages - 1) / a.unit_pages;
-    int u0, u1;
-    if (a.run > 0) {
-      // [overhead | units], head after head
-      const int len = a.overhead + units;
-      it.h = rem / len;
-      const int x0 = rem - it.h * len, x1 = min(len, x0 + left);
-      // the item's place in the row of all units: this run's end less what is left
-      const long long end = min((long long)(blockIdx.x + 1) * a.run, a.units);
-      const long long at = end - left - x0 + a.overhead;
-      left -= x1 - x0;
-      rem += x1 - x0;
-      if (rem >= len * a.geom.n_heads) {
-        tile++;
-        rem = 0;
+      if (left <= 0) {
+        out.state = 0;
+        return false;
       }
-      u0 = max(x0 - a.overhead, 0);
-      u1 = x1 - a.overhead;
-      if (u1 <= 0) continue;   // only the item's overhead: another run has its units
-      const int first = (int)(at / a.run), last = (int)((at + units - 1) / a.run);
-      it.n_parts = last - first + 1;
-      // two slots per CTA: a part that begins inside its item, and one that begins it
-      it.slot0 = 2 * first + 1;
-      it.slot_p0 = 2 * first;
-      it.slot_step = 2;
-      it.slot = u0 == 0 ? it.slot0 : 2 * blockIdx.x;
-      it.counter = first;   // only the last item that starts in a run is cut at its end
-    } else {
-      u0 = min(split * a.split_units, units);
-      u1 = min(u0 + a.split_units, units);
-      it.n_parts = a.n_splits;
-      it.slot0 = it.slot_p0 = item * a.n_splits;
-      it.slot_step = 1;
-      it.slot = it.slot0 + split;
-      it.counter = item;
-      left = 0;
-    }
-    it.pg0 = r.pg0 + u0 * a.unit_pages;
-    it.npages = min(u1 * a.unit_pages, r.pages) - u0 * a.unit_pages;
-    if (it.npages < 0) it.npages = 0;
-    const bool ok = it.b >= 0 && it.b < a.n_caches && it.h >= 0 && it.h < a.geom.n_heads && it.rows >= 1 &&
-                    it.row0 >= 0 && it.pg0 >= 0 && it.pg0 + it.npages <= a.geom.n_pages;
-    if (!ok) atomicOr(a.status, kStatusBadIndex);
-    it.state = ok ? 1 : -1;
-    out = it;
-    return true;
+      int split = 0, item = 0;
+      if (a.run == 0) {
+        // splits fastest, then heads; the last tiles of a prompt, which attend the
+        // most, start first
+        split = blockIdx.x % a.n_splits;
+        item = blockIdx.x / a.n_splits;
+        it.h = item % a.geom.n_heads;
+        tile = a.tile_hi - 1 - item / a.geom.n_heads;
+      }
+      int lo = 0, hi = a.n_caches - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (batch.tile0[mid] <= tile) lo = mid;
+        else hi = mid - 1;
+      }
+      it.b = lo;
+      it.old = batch.old[lo];
+      it.tok0 = batch.first[lo];
+      it.n_new = batch.n_new[lo];
+      it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
+      it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
+      const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window, a.tree != nullptr);
+      const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
+      it.lo = r.lo;
+      it.hi = r.hi;
+      it.all_lo = a.window > 0 ? max(0, it.old + t_last + 1 - a.window) : 0;
+      it.all_hi = a.tree ? it.old : it.old + t_first + 1;
+      const int units = (r.pages + a.unit_pages - 1) / a.unit_pages;
+      int u0, u1;
+      if (a.run > 0) {
+        // [overhead | units], head after head
+        const int len = a.overhead + units;
+        it.h = rem / len;
+        const int x0 = rem - it.h * len, x1 = min(len, x0 + left);
+        // the item's place in the row of all units: this run's end less what is left
+        const long long end = min((long long)(blockIdx.x + 1) * a.run, a.units);
+        const long long at = end - left - x0 + a.overhead;
+        left -= x1 - x0;
+        rem += x1 - x0;
+        if (rem >= len * a.geom.n_heads) {
+          tile++;
+          rem = 0;
+        }
+        u0 = max(x0 - a.overhead, 0);
+        u1 = x1 - a.overhead;
+        if (u1 <= 0) continue;   // only the item's overhead: another run has its units
+        const int first = (int)(at / a.run), last = (int)((at + units - 1) / a.run);
+        it.n_parts = last - first + 1;
+        // two slots per CTA: a part that begins inside its item, and one that begins it
+        it.slot0 = 2 * first + 1;
+        it.slot_p0 = 2 * first;
+        it.slot_step = 2;
+        it.slot = u0 == 0 ? it.slot0 : 2 * blockIdx.x;
+        it.counter = first;   // only the last item that starts in a run is cut at its end
+      } else {
+        u0 = min(split * a.split_units, units);
+        u1 = min(u0 + a.split_units, units);
+        it.n_parts = a.n_splits;
+        it.slot0 = it.slot_p0 = item * a.n_splits;
+        it.slot_step = 1;
+        it.slot = it.slot0 + split;
+        it.counter = item;
+        left = 0;
+      }
+      it.pg0 = r.pg0 + u0 * a.unit_pages;
+      it.npages = min(u1 * a.unit_pages, r.pages) - u0 * a.unit_pages;
+      if (it.npages < 0) it.npages = 0;
+      const bool ok = it.b >= 0 && it.b < a.n_caches && it.h >= 0 && it.h < a.geom.n_heads && it.rows >= 1 &&
+                      it.row0 >= 0 && it.pg0 >= 0 && it.pg0 + it.npages <= a.geom.n_pages;
+      if (!ok) atomicOr(a.status, kStatusBadIndex);
+      it.state = ok ? 1 : -1;
+      out = it;
+      return true;
     }
   }
 
   // Parts from p on that nobody works on, after a wait ran out or at a bad item:
   // they arrive all the same, without records, so that the counters are back at
   // zero after the launch.
+  // item[p & 1] stays as it is: other threads may still look at it.
   __device__ __forceinline__ void abandon(const ExtendArgs &a, const ExtendBatch &batch, int p) {
-    for (; item[p & 1].state != 0; p++) {
-      const ExtItem &it = item[p & 1];
-      if (it.n_parts > 1) atomicInc(a.cnt + it.counter, (unsigned)it.n_parts - 1);
+    for (const ExtItem *it = &item[p & 1]; it->state != 0; it = &item[(p + 1) & 1]) {
+      if (it->n_parts > 1) atomicInc(a.cnt + it->counter, (unsigned)it->n_parts - 1);
       next(a, batch, p + 1);
     }
   }
@@ -384,8 +384,9 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
   }
 }
 
-// extend_mma.cu: tile_rows 16 or 32
-int extend_mma_resident(int head_dim, int dtype, int tile_rows);
+// extend_mma.cu
+constexpr int kExtendMmaRows = 16;
+int extend_mma_resident(int head_dim, int dtype);
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                       bool vec, cudaStream_t s);
 // extend_umma.cu: 16-bit types

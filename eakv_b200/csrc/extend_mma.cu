@@ -39,14 +39,13 @@
 namespace eakv {
 namespace {
 
-// MT: tiles of 16 rows per CTA.
-template <int HD, int LIMBS, int MT>
+template <int HD, int LIMBS>
 struct XCfg {
-  static constexpr int R = 16 * MT;
+  static constexpr int R = kExtendMmaRows;
   static constexpr int NG = HD / 64;
   static constexpr int NW = 4;
   static constexpr int THREADS = NW * 32;
-  static constexpr int MINB = MT == 1 ? 3 : 2;                // CTAs per SM
+  static constexpr int MINB = 3;                                // CTAs per SM
   static constexpr int NIB = kPagePositions * NG * 32;
   static constexpr int PB = kPagePositions * NG * 40;
   static constexpr int NSTAGE = HD == 128 ? 5 : 8;              // pages in flight
@@ -56,14 +55,12 @@ struct XCfg {
   static constexpr int MAIN = RING > MERGE ? RING : MERGE;
   static constexpr int QOFF = MAIN + 2 * NSTAGE * 8;            // q rows [R][HD] f32
   static constexpr int STATOFF = QOFF + R * HD * 4;             // [R] max|q|, [R][NG] sums
-  // the A fragments of q stay in registers for one tile of one limb
-  static constexpr bool QREG = false;
   // K enters as 16 (64 + n), the offset taken off by the sums' start: four
   // operations per two pairs less than centring, and the sums run within
   // 64 sum |q| of zero, 2^-18 of it lost (one-limb types)
   static constexpr bool KRAW = LIMBS == 1;
-  static constexpr int FRAGOFF = STATOFF + R * (1 + NG) * 4;    // [step][tile][limb][lane]
-  static constexpr int FRAGS = QREG ? 0 : LIMBS * MT * 4 * NG * 32 * 16;
+  static constexpr int FRAGOFF = STATOFF + R * (1 + NG) * 4;    // [step][limb][lane]
+  static constexpr int FRAGS = LIMBS * 4 * NG * 32 * 16;
   static constexpr int SMEM = FRAGOFF + FRAGS;
   static_assert(MAIN % 16 == 0 && FRAGOFF % 16 == 0, "alignment");
 };
@@ -123,12 +120,12 @@ __device__ __noinline__ void abandon_walk(ExtWalk &walk, const ExtendArgs &a, co
   walk.abandon(a, batch, p);
 }
 
-template <int HD, int LIMBS, int MT, typename T>
-__global__ void __launch_bounds__(XCfg<HD, LIMBS, MT>::THREADS, XCfg<HD, LIMBS, MT>::MINB)
+template <int HD, int LIMBS, typename T>
+__global__ void __launch_bounds__(XCfg<HD, LIMBS>::THREADS, XCfg<HD, LIMBS>::MINB)
 extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ ExtendBatch batch,
                   const __grid_constant__ ExtendRuns runs, const int vec) {
-  using C = XCfg<HD, LIMBS, MT>;
-  constexpr int NG = C::NG, R = C::R, NR = 2 * MT;   // NR: rows of a lane, g + 8 r
+  using C = XCfg<HD, LIMBS>;
+  constexpr int NG = C::NG, R = C::R, NR = 2;   // NR: rows of a lane, g + 8 r
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last_part;
   __shared__ ExtWalk walk;
@@ -151,101 +148,99 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
   int *last_req = reinterpret_cast<int *>(&bars[C::NSTAGE]) + C::NSTAGE;
   int done = 0;   // pages of the parts before: stages and phases go on
   for (int part = 0;; part++) {
-  const ExtItem &it = walk.item[part & 1];
-  if (it.state <= 0) {
-    if (threadIdx.x == 0 && it.state < 0) abandon_walk(walk, a, batch, part);
-    return;
-  }
-  const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
-  const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
-  auto issue = [&](int i) {
-    if (i == a.test_stall - 1) return;   // test hook: this stage's wait runs out
-    const int st = (done + i) % C::NSTAGE;
-    const uint32_t full = smem_u32(&bars[st]);
-    mbar_arrive_expect_tx(full, 2 * C::PB);
-    const uint32_t dst = smem_u32(smem + st * C::STAGE_BYTES);
-    bulk_g2s(dst, kpages + (size_t)(it.pg0 + i) * C::PB, C::PB, full);
-    bulk_g2s(dst + C::PB, vpages + (size_t)(it.pg0 + i) * C::PB, C::PB, full);
-    publish_requested(&last_req[st], done + i);
-  };
-  if (threadIdx.x == 0)
-    for (int i = 0; i < it.npages && i < C::NSTAGE; i++) issue(i);
+    const ExtItem &it = walk.item[part & 1];
+    if (it.state <= 0) {
+      if (threadIdx.x == 0 && it.state < 0) abandon_walk(walk, a, batch, part);
+      return;
+    }
+    const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
+    const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
+    auto issue = [&](int i) {
+      if (i == a.test_stall - 1) return;   // test hook: this stage's wait runs out
+      const int st = (done + i) % C::NSTAGE;
+      const uint32_t full = smem_u32(&bars[st]);
+      mbar_arrive_expect_tx(full, 2 * C::PB);
+      const uint32_t dst = smem_u32(smem + st * C::STAGE_BYTES);
+      bulk_g2s(dst, kpages + (size_t)(it.pg0 + i) * C::PB, C::PB, full);
+      bulk_g2s(dst + C::PB, vpages + (size_t)(it.pg0 + i) * C::PB, C::PB, full);
+      publish_requested(&last_req[st], done + i);
+    };
+    if (threadIdx.x == 0)
+      for (int i = 0; i < it.npages && i < C::NSTAGE; i++) issue(i);
 
-  // ---- the tile's q rows: f32 in shared memory, row maxima and group sums ------
-  for (int x = threadIdx.x; x < R * (HD / 4); x += C::THREADS) {
-    const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r < it.rows) {
-      const int row = it.row0 + r;
-      const T *p = reinterpret_cast<const T *>(a.q.data) +
-                   (long long)(it.tok0 + row / a.G) * a.q.token_stride +
-                   (long long)(it.h * a.G + row % a.G) * a.q.head_stride + d;
-      if (vec) load4<T, true>(p, v);
-      else load4<T, false>(p, v);
+    // ---- the tile's q rows: f32 in shared memory, row maxima and group sums ------
+    for (int x = threadIdx.x; x < R * (HD / 4); x += C::THREADS) {
+      const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < it.rows) {
+        const int row = it.row0 + r;
+        const T *p = reinterpret_cast<const T *>(a.q.data) +
+                     (long long)(it.tok0 + row / a.G) * a.q.token_stride +
+                     (long long)(it.h * a.G + row % a.G) * a.q.head_stride + d;
+        if (vec) load4<T, true>(p, v);
+        else load4<T, false>(p, v);
+      }
+      *reinterpret_cast<float4 *>(q_s + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
     }
-    *reinterpret_cast<float4 *>(q_s + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-  __syncthreads();
-  for (int r = warp; r < R; r += C::NW) {
-    float mx = 0.0f;
-    bool bad = false;
+    __syncthreads();
+    for (int r = warp; r < R; r += C::NW) {
+      float mx = 0.0f;
+      bool bad = false;
 #pragma unroll
-    for (int gg = 0; gg < NG; gg++) {
-      const float v0 = q_s[r * HD + 64 * gg + lane], v1 = q_s[r * HD + 64 * gg + 32 + lane];
-      mx = fmaxf(mx, fmaxf(fabsf(v0), fabsf(v1)));
-      bad = bad || v0 != v0 || v1 != v1;
-      float sm = v0 + v1;
+      for (int gg = 0; gg < NG; gg++) {
+        const float v0 = q_s[r * HD + 64 * gg + lane], v1 = q_s[r * HD + 64 * gg + 32 + lane];
+        mx = fmaxf(mx, fmaxf(fabsf(v0), fabsf(v1)));
+        bad = bad || v0 != v0 || v1 != v1;
+        float sm = v0 + v1;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sm += __shfl_xor_sync(0xffffffffu, sm, o);
-      if (lane == 0) stat_s[R + r * NG + gg] = sm;
+        for (int o = 16; o > 0; o >>= 1) sm += __shfl_xor_sync(0xffffffffu, sm, o);
+        if (lane == 0) stat_s[R + r * NG + gg] = sm;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      bad = __any_sync(0xffffffffu, bad);
+      if (lane == 0) stat_s[r] = bad ? INFINITY : mx;
     }
+    __syncthreads();
+    // rows g + 8 r of this lane
+    float rowfac[NR], qsum[NR][NG], kstart[NR][NG];
+    RowMask mask[NR];
+    {
+      float up[NR];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) stat_s[r] = bad ? INFINITY : mx;
-  }
-  __syncthreads();
-  // rows g + 8 r of this lane
-  float rowfac[NR], qsum[NR][NG], kstart[NR][NG];
-  RowMask mask[NR];
-  uint32_t aq[C::QREG ? NG * 4 : 1][4];
-  {
-    float up[NR];
+      for (int r = 0; r < NR; r++) {
+        const float hmax = stat_s[g + 8 * r];
+        const bool fine = hmax <= 3.0e38f;
+        int e = 0;
+        frexpf(hmax > 0.0f && fine ? hmax : 1.0f, &e);          // hmax in [2^(e-1), 2^e)
+        const int qe = max(min(5 - e, 126), -126);
+        up[r] = fine ? __uint_as_float((uint32_t)(127 + qe) << 23) : 0.0f;
+        // a row with an infinity or NaN in q has NaN scores
+        rowfac[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - qe) << 23)
+                         : __uint_as_float(0x7fc00000u);
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-      const float hmax = stat_s[g + 8 * r];
-      const bool fine = hmax <= 3.0e38f;
-      int e = 0;
-      frexpf(hmax > 0.0f && fine ? hmax : 1.0f, &e);          // hmax in [2^(e-1), 2^e)
-      const int qe = max(min(5 - e, 126), -126);
-      up[r] = fine ? __uint_as_float((uint32_t)(127 + qe) << 23) : 0.0f;
-      // a row with an infinity or NaN in q has NaN scores
-      rowfac[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - qe) << 23)
-                       : __uint_as_float(0x7fc00000u);
+        for (int gg = 0; gg < NG; gg++)
+          qsum[r][gg] = fine ? stat_s[R + (g + 8 * r) * NG + gg] * up[r] : 0.0f;
+        mask[r] = row_mask(a, it, it.row0 + g + 8 * r);
+      }
+      // A fragments of k-step s = (word j, byte parity par) of group gg: dims
+      // d = 64 gg + 8c + 4j + par and d + 2 (low nibbles), d + 32 and d + 34 (high
+      // nibbles, held times 16)
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++)
-        qsum[r][gg] = fine ? stat_s[R + (g + 8 * r) * NG + gg] * up[r] : 0.0f;
-      mask[r] = row_mask(a, it, it.row0 + g + 8 * r);
-    }
-    // A fragments of k-step s = (word j, byte parity par) of group gg: dims
-    // d = 64 gg + 8c + 4j + par and d + 2 (low nibbles), d + 32 and d + 34 (high
-    // nibbles, held times 16)
+      for (int r = 0; r < NR; r++)
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+        for (int gg = 0; gg < NG; gg++) kstart[r][gg] = 0.0f;
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++) kstart[r][gg] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NG * 4; s++) {
-      const int d = 64 * (s >> 2) + 8 * c + 4 * ((s >> 1) & 1) + (s & 1);
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
+      for (int s = 0; s < NG * 4; s++) {
+        const int d = 64 * (s >> 2) + 8 * c + 4 * ((s >> 1) & 1) + (s & 1);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // k & 1: row, k >> 1: high nibbles
-          const int r = 2 * m + (k & 1);
+          const int r = k & 1;
           const float *p = q_s + (g + 8 * r) * HD + d + 32 * (k >> 1);
           const float f = up[r] * (C::KRAW || (k >> 1) ? 0.0625f : 1.0f);
-          const float x0 = up[r] == 0.0f ? 0.0f : p[0] * f, x1 = up[r] == 0.0f ? 0.0f : p[2] * f;   // inf * 0
+          const float x0 = up[r] == 0.0f ? 0.0f : p[0] * f;   // inf * 0
+          const float x1 = up[r] == 0.0f ? 0.0f : p[2] * f;
           hi[k] = pack_f16(x0, x1);
           if (C::KRAW) {
             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
@@ -253,219 +248,208 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           }
           lo[k] = LIMBS == 2 ? pack_rest(x0, x1, hi[k]) : 0u;
         }
-        if constexpr (C::QREG) {
-#pragma unroll
-          for (int k = 0; k < 4; k++) aq[s][k] = hi[k];
-        } else if (s % C::NW == warp) {
-          uint4 *f = frag_s + ((s * MT + m) * LIMBS) * 32 + lane;
+        if (s % C::NW == warp) {
+          uint4 *f = frag_s + s * LIMBS * 32 + lane;
           f[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           if (LIMBS == 2) f[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
     }
-  }
-  if (C::KRAW) {
+    if (C::KRAW) {
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+      for (int r = 0; r < NR; r++)
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++) {
-        kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 1);
-        kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 2);
-      }
-  }
-  if (!C::QREG) __syncthreads();
+        for (int gg = 0; gg < NG; gg++) {
+          kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 1);
+          kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 2);
+        }
+    }
+    __syncthreads();
 
-  float o[MT][NG][8][4];
-#pragma unroll
-  for (int m = 0; m < MT; m++)
+    float o[NG][8][4];
 #pragma unroll
     for (int gg = 0; gg < NG; gg++)
 #pragma unroll
       for (int n = 0; n < 8; n++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[m][gg][n][k] = 0.0f;
-  float m_run[NR], m_eff[NR], l_run[NR], pb[NR][NG];
-  // Everything a row sums is divided by a power of two near the largest V scale
-  // the row has attended (eref: its biased exponent, -6 before the first), by
-  // way of the exponential's argument (m_eff); it moves like the maximum, when a
-  // scale passes it by 2^6, so that p s stays below 2^8 2^7.
-  int eref[NR];
-#pragma unroll
-  for (int r = 0; r < NR; r++) {
-    m_run[r] = -INFINITY;
-    m_eff[r] = l_run[r] = 0.0f;
-    eref[r] = -6;
-#pragma unroll
-    for (int gg = 0; gg < NG; gg++) pb[r][gg] = 0.0f;
-  }
-
-  // page_ex: largest exponent of a V scale of the page (full pages)
-  auto step = [&](auto full_tag, const uint8_t *ks, int page_pos0, int p0, int page_ex) {
-    constexpr bool FULL = decltype(full_tag)::value;
-    const uint8_t *vsm = ks + C::PB;
-    bool on[NR][4];
-    float sk[4][NG], bk[4][NG];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
-      if (!FULL) {
-#pragma unroll
-        for (int r = 0; r < NR; r++) on[r][j] = mask[r].attends(page_pos0 + tp);
-      }
-      if constexpr (NG == 2) {
-        const float4 k4 = *reinterpret_cast<const float4 *>(ks + C::NIB + tp * 16);
-        sk[j][0] = k4.x; bk[j][0] = k4.y; sk[j][1] = k4.z; bk[j][1] = k4.w;
-      } else {
-        const float2 k2 = *reinterpret_cast<const float2 *>(ks + C::NIB + tp * 8);
-        sk[j][0] = k2.x; bk[j][0] = k2.y;
-      }
-#pragma unroll
-      for (int gg = 0; gg < NG && !C::KRAW; gg++) bk[j][gg] = fmaf(8.0f, sk[j][gg], bk[j][gg]);
-    }
-    // ---- scores --------------------------------------------------------------
-    float sc[NR][4];
-    {
-      float dk[2][MT][NG][4];
-#pragma unroll
-      for (int gg = 0; gg < NG; gg++) {
-        uint2 wv[2];
-#pragma unroll
-        for (int tile = 0; tile < 2; tile++) {
-          wv[tile] = *reinterpret_cast<const uint2 *>(ks + (p0 + 8 * tile + g) * (HD / 2) + 8 * c + 32 * gg);
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) dk[tile][m][gg][k] = C::KRAW ? kstart[2 * m + (k >> 1)][gg] : 0.0f;
-        }
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          uint32_t b0[2], b1[2];
-#pragma unroll
-          for (int tile = 0; tile < 2; tile++) {
-            const uint32_t w = (s >> 1) ? wv[tile].y : wv[tile].x;
-            const uint32_t y = (s & 1) ? w >> 8 : w;
-            b0[tile] = C::KRAW ? raw_hi((s & 1) ? w >> 4 : w << 4) : nib_lo(y);
-            b1[tile] = C::KRAW ? raw_hi(y) : nib_hi(y);
-          }
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int l = 0; l < LIMBS; l++) {
-              const uint4 f = frag_s[(((4 * gg + s) * MT + m) * LIMBS + l) * 32 + lane];
-              const uint32_t af[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-              for (int tile = 0; tile < 2; tile++) mma(dk[tile][m][gg], af, b0[tile], b1[tile]);
-            }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-          float u = 0.0f;
-#pragma unroll
-          for (int gg = 0; gg < NG; gg++) {
-            u = fmaf(dk[j >> 1][r >> 1][gg][2 * (r & 1) + (j & 1)], sk[j][gg], u);
-            u = fmaf(qsum[r][gg], bk[j][gg], u);
-          }
-          u *= rowfac[r];
-          sc[r][j] = (FULL || on[r][j]) ? u : -INFINITY;
-        }
-    }
-    float sv[4][NG], bv[4][NG];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
-      if constexpr (NG == 2) {
-        const float4 v4 = *reinterpret_cast<const float4 *>(vsm + C::NIB + tp * 16);
-        sv[j][0] = v4.x; bv[j][0] = v4.y; sv[j][1] = v4.z; bv[j][1] = v4.w;
-      } else {
-        const float2 v2 = *reinterpret_cast<const float2 *>(vsm + C::NIB + tp * 8);
-        sv[j][0] = v2.x; bv[j][0] = v2.y;
-      }
-#pragma unroll
-      for (int gg = 0; gg < NG; gg++) bv[j][gg] = fmaf(8.0f, sv[j][gg], bv[j][gg]);
-    }
-    // ---- online softmax, base 2, lazy maximum -----------------------------------
-    // A row moves when a score passes its maximum by 8, or a V scale that it
-    // attends passes its reference by 2^6 (scales are negative only in damaged
-    // files; NaN is passed over).
-    bool move = false;
-    float lm[NR];
-    int ex[NR];
+        for (int k = 0; k < 4; k++) o[gg][n][k] = 0.0f;
+    float m_run[NR], m_eff[NR], l_run[NR], pb[NR][NG];
+    // Everything a row sums is divided by a power of two near the largest V scale
+    // the row has attended (eref: its biased exponent, -6 before the first), by
+    // way of the exponential's argument (m_eff); it moves like the maximum, when a
+    // scale passes it by 2^6, so that p s stays below 2^8 2^7.
+    int eref[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-      lm[r] = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
-      if (FULL) {
-        ex[r] = page_ex;
-      } else {
-        float sx = 0.0f;
+      m_run[r] = -INFINITY;
+      m_eff[r] = l_run[r] = 0.0f;
+      eref[r] = -6;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          float s = fabsf(sv[j][0]);
-          if (NG == 2) s = fmaxf(s, fabsf(sv[j][NG - 1]));
-          if (on[r][j]) sx = fmaxf(sx, s);
-        }
-        ex[r] = (int)(__float_as_uint(sx) >> 23);
-      }
-      move = move || lm[r] > m_run[r] + 8.0f || ex[r] > eref[r] + 6;
+      for (int gg = 0; gg < NG; gg++) pb[r][gg] = 0.0f;
     }
-    if (__any_sync(0xffffffffu, move)) {
+
+    // page_ex: largest exponent of a V scale of the page (full pages)
+    auto step = [&](auto full_tag, const uint8_t *ks, int page_pos0, int p0, int page_ex) {
+      constexpr bool FULL = decltype(full_tag)::value;
+      const uint8_t *vsm = ks + C::PB;
+      bool on[NR][4];
+      float sk[4][NG], bk[4][NG];
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
-        float t = lm[r];
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        int x = ex[r];
-        if (!FULL && x >= 253) {   // without the infinite ones
-          x = 0;
+      for (int j = 0; j < 4; j++) {
+        const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
+        if (!FULL) {
 #pragma unroll
-          for (int j = 0; j < 4; j++)
+          for (int r = 0; r < NR; r++) on[r][j] = mask[r].attends(page_pos0 + tp);
+        }
+        if constexpr (NG == 2) {
+          const float4 k4 = *reinterpret_cast<const float4 *>(ks + C::NIB + tp * 16);
+          sk[j][0] = k4.x; bk[j][0] = k4.y; sk[j][1] = k4.z; bk[j][1] = k4.w;
+        } else {
+          const float2 k2 = *reinterpret_cast<const float2 *>(ks + C::NIB + tp * 8);
+          sk[j][0] = k2.x; bk[j][0] = k2.y;
+        }
+#pragma unroll
+        for (int gg = 0; gg < NG && !C::KRAW; gg++) bk[j][gg] = fmaf(8.0f, sk[j][gg], bk[j][gg]);
+      }
+      // ---- scores --------------------------------------------------------------
+      float sc[NR][4];
+      {
+        float dk[2][NG][4];
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++) {
+          uint2 wv[2];
+#pragma unroll
+          for (int tile = 0; tile < 2; tile++) {
+            wv[tile] = *reinterpret_cast<const uint2 *>(ks + (p0 + 8 * tile + g) * (HD / 2) + 8 * c + 32 * gg);
+#pragma unroll
+            for (int k = 0; k < 4; k++) dk[tile][gg][k] = C::KRAW ? kstart[k >> 1][gg] : 0.0f;
+          }
+#pragma unroll
+          for (int s = 0; s < 4; s++) {
+            uint32_t b0[2], b1[2];
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++) {
+              const uint32_t w = (s >> 1) ? wv[tile].y : wv[tile].x;
+              const uint32_t y = (s & 1) ? w >> 8 : w;
+              b0[tile] = C::KRAW ? raw_hi((s & 1) ? w >> 4 : w << 4) : nib_lo(y);
+              b1[tile] = C::KRAW ? raw_hi(y) : nib_hi(y);
+            }
+#pragma unroll
+            for (int l = 0; l < LIMBS; l++) {
+              const uint4 f = frag_s[((4 * gg + s) * LIMBS + l) * 32 + lane];
+              const uint32_t af[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int tile = 0; tile < 2; tile++) mma(dk[tile][gg], af, b0[tile], b1[tile]);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int r = 0; r < NR; r++) {
+            float u = 0.0f;
 #pragma unroll
             for (int gg = 0; gg < NG; gg++) {
-              const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
-              if (on[r][j] && e1 < 255) x = max(x, min(e1, 252));
+              u = fmaf(dk[j >> 1][gg][2 * r + (j & 1)], sk[j][gg], u);
+              u = fmaf(qsum[r][gg], bk[j][gg], u);
             }
+            u *= rowfac[r];
+            sc[r][j] = (FULL || on[r][j]) ? u : -INFINITY;
+          }
+      }
+      float sv[4][NG], bv[4][NG];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
+        if constexpr (NG == 2) {
+          const float4 v4 = *reinterpret_cast<const float4 *>(vsm + C::NIB + tp * 16);
+          sv[j][0] = v4.x; bv[j][0] = v4.y; sv[j][1] = v4.z; bv[j][1] = v4.w;
+        } else {
+          const float2 v2 = *reinterpret_cast<const float2 *>(vsm + C::NIB + tp * 8);
+          sv[j][0] = v2.x; bv[j][0] = v2.y;
         }
-        x = max(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = max(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        const bool mv = t > m_run[r] + 8.0f, me = x > eref[r] + 6;
-        if (mv || me) {
-          float alpha = mv ? ex2(m_run[r] - t) : 1.0f;
-          if (mv) m_run[r] = t;
-          // before the first reference all sums are zero, or NaN
-          if (me && eref[r] > 0) alpha *= __uint_as_float((uint32_t)max(127 + eref[r] - x, 0) << 23);
-          if (me) eref[r] = x;
-          m_eff[r] = (m_run[r] == -INFINITY ? 0.0f : m_run[r]) + (eref[r] > 0 ? (float)(eref[r] - 127) : 0.0f);
-          l_run[r] *= alpha;
 #pragma unroll
-          for (int gg = 0; gg < NG; gg++) {
-            pb[r][gg] *= alpha;
+        for (int gg = 0; gg < NG; gg++) bv[j][gg] = fmaf(8.0f, sv[j][gg], bv[j][gg]);
+      }
+      // ---- online softmax, base 2, lazy maximum -----------------------------------
+      // A row moves when a score passes its maximum by 8, or a V scale that it
+      // attends passes its reference by 2^6 (scales are negative only in damaged
+      // files; NaN is passed over).
+      bool move = false;
+      float lm[NR];
+      int ex[NR];
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
-              o[r >> 1][gg][n][2 * (r & 1)] *= alpha;
-              o[r >> 1][gg][n][2 * (r & 1) + 1] *= alpha;
+      for (int r = 0; r < NR; r++) {
+        lm[r] = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
+        if (FULL) {
+          ex[r] = page_ex;
+        } else {
+          float sx = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float s = fabsf(sv[j][0]);
+            if (NG == 2) s = fmaxf(s, fabsf(sv[j][NG - 1]));
+            if (on[r][j]) sx = fmaxf(sx, s);
+          }
+          ex[r] = (int)(__float_as_uint(sx) >> 23);
+        }
+        move = move || lm[r] > m_run[r] + 8.0f || ex[r] > eref[r] + 6;
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          float t = lm[r];
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+          int x = ex[r];
+          if (!FULL && x >= 253) {   // without the infinite ones
+            x = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int gg = 0; gg < NG; gg++) {
+                const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
+                if (on[r][j] && e1 < 255) x = max(x, min(e1, 252));
+              }
+          }
+          x = max(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = max(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          const bool mv = t > m_run[r] + 8.0f, me = x > eref[r] + 6;
+          if (mv || me) {
+            float alpha = mv ? ex2(m_run[r] - t) : 1.0f;
+            if (mv) m_run[r] = t;
+            // before the first reference all sums are zero, or NaN
+            if (me && eref[r] > 0) alpha *= __uint_as_float((uint32_t)max(127 + eref[r] - x, 0) << 23);
+            if (me) eref[r] = x;
+            m_eff[r] = (m_run[r] == -INFINITY ? 0.0f : m_run[r]) +
+                       (eref[r] > 0 ? (float)(eref[r] - 127) : 0.0f);
+            l_run[r] *= alpha;
+#pragma unroll
+            for (int gg = 0; gg < NG; gg++) {
+              pb[r][gg] *= alpha;
+#pragma unroll
+              for (int n = 0; n < 8; n++) {
+                o[gg][n][2 * r] *= alpha;
+                o[gg][n][2 * r + 1] *= alpha;
+              }
             }
           }
         }
       }
-    }
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+      for (int r = 0; r < NR; r++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        sc[r][j] = ex2(sc[r][j] - m_eff[r]);   // the weights from here on
-        l_run[r] += sc[r][j];
-      }
-    // ---- outputs -------------------------------------------------------------
+        for (int j = 0; j < 4; j++) {
+          sc[r][j] = ex2(sc[r][j] - m_eff[r]);   // the weights from here on
+          l_run[r] += sc[r][j];
+        }
+      // ---- outputs -------------------------------------------------------------
 #pragma unroll
-    for (int gg = 0; gg < NG; gg++) {
-      uint32_t ah[MT][4], al[MT][4];
-#pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int gg = 0; gg < NG; gg++) {
+        uint32_t ah[4], al[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // k & 1: row, k >> 1: positions 2c+8, 2c+9
-          const int r = 2 * m + (k & 1);
+          const int r = k & 1;
           float x[2];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
@@ -474,157 +458,154 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
             x[e] = (FULL || on[r][j]) ? sc[r][j] * sv[j][gg] : 0.0f;
             if (FULL || on[r][j]) pb[r][gg] = fmaf(sc[r][j], bv[j][gg], pb[r][gg]);
           }
-          ah[m][k] = pack_f16(x[0], x[1]);
-          al[m][k] = LIMBS == 2 ? pack_rest(x[0], x[1], ah[m][k]) : 0u;
+          ah[k] = pack_f16(x[0], x[1]);
+          al[k] = LIMBS == 2 ? pack_rest(x[0], x[1], ah[k]) : 0u;
         }
-      // V bytes: lane (g, c) receives bytes 16w + 2g, + 1 of positions 2c, 2c+1
-      // (x[2w]) and 2c+8, 2c+9 (x[2w+1])
-      uint32_t x[4];
-      {
-        const int t = lane >> 3, r = lane & 7;
-        ldsm_x4_trans(x, smem_u32(vsm + (p0 + 8 * (t & 1) + r) * (HD / 2) + 32 * gg + 16 * (t >> 1)));
-      }
+        // V bytes: lane (g, c) receives bytes 16w + 2g, + 1 of positions 2c, 2c+1
+        // (x[2w]) and 2c+8, 2c+9 (x[2w+1])
+        uint32_t x[4];
+        {
+          const int t = lane >> 3, r = lane & 7;
+          ldsm_x4_trans(x, smem_u32(vsm + (p0 + 8 * (t & 1) + r) * (HD / 2) + 32 * gg + 16 * (t >> 1)));
+        }
 #pragma unroll
-      for (int n = 0; n < 8; n++) {   // n = 4w + 2 parity + (high nibbles)
-        const int w = n >> 2, par = (n >> 1) & 1;
-        const uint32_t y0 = par ? x[2 * w] >> 8 : x[2 * w];
-        const uint32_t y1 = par ? x[2 * w + 1] >> 8 : x[2 * w + 1];
-        const uint32_t b0 = (n & 1) ? nib_hi(y0) : nib_lo(y0);
-        const uint32_t b1 = (n & 1) ? nib_hi(y1) : nib_lo(y1);
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          mma(o[m][gg][n], ah[m], b0, b1);
-          if constexpr (LIMBS == 2) mma(o[m][gg][n], al[m], b0, b1);
+        for (int n = 0; n < 8; n++) {   // n = 4w + 2 parity + (high nibbles)
+          const int w = n >> 2, par = (n >> 1) & 1;
+          const uint32_t y0 = par ? x[2 * w] >> 8 : x[2 * w];
+          const uint32_t y1 = par ? x[2 * w + 1] >> 8 : x[2 * w + 1];
+          const uint32_t b0 = (n & 1) ? nib_hi(y0) : nib_lo(y0);
+          const uint32_t b1 = (n & 1) ? nib_hi(y1) : nib_lo(y1);
+          mma(o[gg][n], ah, b0, b1);
+          if constexpr (LIMBS == 2) mma(o[gg][n], al, b0, b1);
         }
       }
-    }
-  };
+    };
 
-  bool ok = true;
-  for (int i = warp; i < it.npages; i += C::NW) {
-    const int st = (done + i) % C::NSTAGE;
-    if (!wait_requested(&last_req[st], done + i, a.wait_budget) ||
-        !mbar_wait(smem_u32(&bars[st]), ((done + i) / C::NSTAGE) & 1, a.wait_budget)) {
-      atomicOr(a.status, kStatusWaitTimeout);
-      ok = false;
-      break;
-    }
-    const uint8_t *ks = smem + st * C::STAGE_BYTES;
-    const int page_pos0 = (it.pg0 + i) * kPagePositions;
-    const bool full = page_pos0 >= it.all_lo && page_pos0 + kPagePositions <= it.all_hi;
-    if (full) {
-      // finite scales only: what an infinite one reaches is NaN anyway
-      int ex = 0;
-#pragma unroll
-      for (int k = 0; k < 2 * NG; k++) {
-        const uint32_t b = *reinterpret_cast<const uint32_t *>(ks + C::PB + C::NIB + 8 * (lane + 32 * k));
-        const int e = (int)(b >> 23) & 255;
-        ex = max(ex, e < 255 ? min(e, 252) : 0);
+    bool ok = true;
+    for (int i = warp; i < it.npages; i += C::NW) {
+      const int st = (done + i) % C::NSTAGE;
+      if (!wait_requested(&last_req[st], done + i, a.wait_budget) ||
+          !mbar_wait(smem_u32(&bars[st]), ((done + i) / C::NSTAGE) & 1, a.wait_budget)) {
+        atomicOr(a.status, kStatusWaitTimeout);
+        ok = false;
+        break;
       }
-      ex = __reduce_max_sync(0xffffffffu, ex);
+      const uint8_t *ks = smem + st * C::STAGE_BYTES;
+      const int page_pos0 = (it.pg0 + i) * kPagePositions;
+      const bool full = page_pos0 >= it.all_lo && page_pos0 + kPagePositions <= it.all_hi;
+      if (full) {
+        // finite scales only: what an infinite one reaches is NaN anyway
+        int ex = 0;
+#pragma unroll
+        for (int k = 0; k < 2 * NG; k++) {
+          const uint32_t b = *reinterpret_cast<const uint32_t *>(ks + C::PB + C::NIB + 8 * (lane + 32 * k));
+          const int e = (int)(b >> 23) & 255;
+          ex = max(ex, e < 255 ? min(e, 252) : 0);
+        }
+        ex = __reduce_max_sync(0xffffffffu, ex);
 #pragma unroll 1
-      for (int s = 0; s < kPagePositions / 16; s++) step(std::true_type{}, ks, page_pos0, 16 * s, ex);
-    } else {
+        for (int s = 0; s < kPagePositions / 16; s++) step(std::true_type{}, ks, page_pos0, 16 * s, ex);
+      } else {
 #pragma unroll 1
-      for (int s = 0; s < kPagePositions / 16; s++) step(std::false_type{}, ks, page_pos0, 16 * s, 0);
+        for (int s = 0; s < kPagePositions / 16; s++) step(std::false_type{}, ks, page_pos0, 16 * s, 0);
+      }
+      __syncwarp();
+      if (lane == 0 && stage_release_last(reinterpret_cast<int *>(&bars[C::NSTAGE]) + st, 1) &&
+          i + C::NSTAGE < it.npages)
+        issue(i + C::NSTAGE);
     }
-    __syncwarp();
-    if (lane == 0 && stage_release_last(reinterpret_cast<int *>(&bars[C::NSTAGE]) + st, 1) &&
-        i + C::NSTAGE < it.npages)
-      issue(i + C::NSTAGE);
-  }
-  if (!__syncthreads_and(ok)) {
-    if (threadIdx.x == 0) {
+    if (!__syncthreads_and(ok)) {
+      if (threadIdx.x == 0) {
+        drain_stages(bars, last_req, C::NSTAGE, a.wait_budget);
+        abandon_walk(walk, a, batch, part);
+      }
+      return;
+    }
+    if (threadIdx.x == 0 && !stages_idle(bars, last_req, C::NSTAGE)) {
+      atomicOr(a.status, kStatusLateCopy);
       drain_stages(bars, last_req, C::NSTAGE, a.wait_budget);
-      abandon_walk(walk, a, batch, part);
     }
-    return;
-  }
-  if (threadIdx.x == 0 && !stages_idle(bars, last_req, C::NSTAGE)) {
-    atomicOr(a.status, kStatusLateCopy);
-    drain_stages(bars, last_req, C::NSTAGE, a.wait_budget);
-  }
 
-  // ---- the warps' sums meet in the (now idle) ring ---------------------------------
-  __syncthreads();
-  float *mw = reinterpret_cast<float *>(smem);   // [NW][R]
-  float *lw = mw + C::NW * R;
-  float *ow = lw + C::NW * R;                    // [NW][R][HD]
+    // ---- the warps' sums meet in the (now idle) ring ---------------------------------
+    __syncthreads();
+    float *mw = reinterpret_cast<float *>(smem);   // [NW][R]
+    float *lw = mw + C::NW * R;
+    float *ow = lw + C::NW * R;                    // [NW][R][HD]
 #pragma unroll
-  for (int r = 0; r < NR; r++) {
-    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+    for (int r = 0; r < NR; r++) {
+      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
 #pragma unroll
-    for (int gg = 0; gg < NG; gg++) {
-      pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 1);
-      pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 2);
+      for (int gg = 0; gg < NG; gg++) {
+        pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 1);
+        pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 2);
+      }
+      const int row = warp * R + g + 8 * r;
+      const float vs = eref[r] > 0 ? __uint_as_float((uint32_t)eref[r] << 23) : 1.0f;
+      if (c == 0) {
+        mw[row] = m_run[r];
+        lw[row] = l_run[r] * vs;
+      }
+#pragma unroll
+      for (int gg = 0; gg < NG; gg++)
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+          for (int hi = 0; hi < 2; hi++) {
+            const float f = hi ? vs * 0.0625f : vs, b = pb[r][gg] * vs;
+            const float (&e0)[4] = o[gg][4 * w + hi], (&e1)[4] = o[gg][4 * w + 2 + hi];
+            const int k = 2 * r;
+            *reinterpret_cast<float4 *>(ow + row * HD + 64 * gg + 32 * hi + 16 * w + 4 * c) =
+                make_float4(fmaf(e0[k], f, b), fmaf(e1[k], f, b), fmaf(e0[k + 1], f, b), fmaf(e1[k + 1], f, b));
+          }
     }
-    const int row = warp * R + g + 8 * r;
-    const float vs = eref[r] > 0 ? __uint_as_float((uint32_t)eref[r] << 23) : 1.0f;
-    if (c == 0) {
-      mw[row] = m_run[r];
-      lw[row] = l_run[r] * vs;
-    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < it.rows * (HD / 4); x += C::THREADS) {
+      const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
+      float M = -INFINITY;
 #pragma unroll
-    for (int gg = 0; gg < NG; gg++)
+      for (int w = 0; w < C::NW; w++) M = fmaxf(M, mw[w * R + r]);
+      float O[4] = {0.0f, 0.0f, 0.0f, 0.0f}, L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 2; w++)
-#pragma unroll
-        for (int hi = 0; hi < 2; hi++) {
-          const float f = hi ? vs * 0.0625f : vs, b = pb[r][gg] * vs;
-          const float (&e0)[4] = o[r >> 1][gg][4 * w + hi], (&e1)[4] = o[r >> 1][gg][4 * w + 2 + hi];
-          const int k = 2 * (r & 1);
-          *reinterpret_cast<float4 *>(ow + row * HD + 64 * gg + 32 * hi + 16 * w + 4 * c) =
-              make_float4(fmaf(e0[k], f, b), fmaf(e1[k], f, b), fmaf(e0[k + 1], f, b), fmaf(e1[k + 1], f, b));
+      for (int w = 0; w < C::NW; w++) {
+        const float f = part_weight(mw[w * R + r], M);
+        const float4 v = *reinterpret_cast<const float4 *>(ow + (w * R + r) * HD + d);
+        L = fmaf(f, lw[w * R + r], L);
+        O[0] = fmaf(f, v.x, O[0]);
+        O[1] = fmaf(f, v.y, O[1]);
+        O[2] = fmaf(f, v.z, O[2]);
+        O[3] = fmaf(f, v.w, O[3]);
+      }
+      if (it.n_parts == 1) {
+        extend_store<T>(a, it, r, d, O, M, L, vec);
+      } else {
+        const size_t pr = part_row(a, it.slot, r);
+        *reinterpret_cast<float4 *>(a.part_o + pr * HD + d) = make_float4(O[0], O[1], O[2], O[3]);
+        if (d == 0) {
+          a.part_m[pr] = M;
+          a.part_l[pr] = L;
         }
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < it.rows * (HD / 4); x += C::THREADS) {
-    const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < C::NW; w++) M = fmaxf(M, mw[w * R + r]);
-    float O[4] = {0.0f, 0.0f, 0.0f, 0.0f}, L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < C::NW; w++) {
-      const float f = part_weight(mw[w * R + r], M);
-      const float4 v = *reinterpret_cast<const float4 *>(ow + (w * R + r) * HD + d);
-      L = fmaf(f, lw[w * R + r], L);
-      O[0] = fmaf(f, v.x, O[0]);
-      O[1] = fmaf(f, v.y, O[1]);
-      O[2] = fmaf(f, v.z, O[2]);
-      O[3] = fmaf(f, v.w, O[3]);
-    }
-    if (it.n_parts == 1) {
-      extend_store<T>(a, it, r, d, O, M, L, vec);
-    } else {
-      const size_t pr = part_row(a, it.slot, r);
-      *reinterpret_cast<float4 *>(a.part_o + pr * HD + d) = make_float4(O[0], O[1], O[2], O[3]);
-      if (d == 0) {
-        a.part_m[pr] = M;
-        a.part_l[pr] = L;
       }
     }
-  }
-  if (it.n_parts > 1 && extend_arrive_last<C::THREADS>(a, it, &last_part, 1))
-    extend_merge<HD, T, C::THREADS>(a, it, vec, reinterpret_cast<float *>(smem), C::MAIN / 4, 1);
-  // the ring takes copies again
-  done += it.npages;
-  fence_proxy_async_smem();
-  if (threadIdx.x == 0) step_walk(walk, a, batch, part + 1);
-  __syncthreads();
+    if (it.n_parts > 1 && extend_arrive_last<C::THREADS>(a, it, &last_part, 1))
+      extend_merge<HD, T, C::THREADS>(a, it, vec, reinterpret_cast<float *>(smem), C::MAIN / 4, 1);
+    // the ring takes copies again
+    done += it.npages;
+    fence_proxy_async_smem();
+    if (threadIdx.x == 0) step_walk(walk, a, batch, part + 1);
+    __syncthreads();
   }
 }
 
-template <int HD, int LIMBS, int MT, typename T>
+template <int HD, int LIMBS, typename T>
 int resident_one() {
-  using C = XCfg<HD, LIMBS, MT>;
+  using C = XCfg<HD, LIMBS>;
   static std::atomic<int> cached[64];
   int dev = 0;
   cudaGetDevice(&dev);
   const int hit = cached[dev & 63].load(std::memory_order_relaxed);
   if (hit) return hit;
-  auto fn = extend_mma_kernel<HD, LIMBS, MT, T>;
+  auto fn = extend_mma_kernel<HD, LIMBS, T>;
   if (check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                  "extend: smem attribute"))
     return 0;
@@ -635,28 +616,25 @@ int resident_one() {
   return per_sm;
 }
 
-template <int HD, int LIMBS, int MT, typename T>
+template <int HD, int LIMBS, typename T>
 int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks, bool vec,
                cudaStream_t s) {
-  using C = XCfg<HD, LIMBS, MT>;
-  extend_mma_kernel<HD, LIMBS, MT, T><<<n_blocks, C::THREADS, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
+  using C = XCfg<HD, LIMBS>;
+  extend_mma_kernel<HD, LIMBS, T><<<n_blocks, C::THREADS, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
   return check_cuda(cudaGetLastError(), "extend_mma launch");
 }
 
 // f(launch or resident functions of the instance that serves the arguments)
 template <int HD, typename F>
-int pick(int dtype, int mt, F f) {
-  if (dtype == EAKV_F32)
-    return mt == 2 ? f.template operator()<HD, 2, 2, float>() : f.template operator()<HD, 2, 1, float>();
-  if (dtype == EAKV_F16)
-    return mt == 2 ? f.template operator()<HD, 1, 2, __half>() : f.template operator()<HD, 1, 1, __half>();
-  return mt == 2 ? f.template operator()<HD, 1, 2, __nv_bfloat16>()
-                 : f.template operator()<HD, 1, 1, __nv_bfloat16>();
+int pick(int dtype, F f) {
+  if (dtype == EAKV_F32) return f.template operator()<HD, 2, float>();
+  if (dtype == EAKV_F16) return f.template operator()<HD, 1, __half>();
+  return f.template operator()<HD, 1, __nv_bfloat16>();
 }
 
 struct Resident {
-  template <int HD, int LIMBS, int MT, typename T> int operator()() const {
-    return resident_one<HD, LIMBS, MT, T>();
+  template <int HD, int LIMBS, typename T> int operator()() const {
+    return resident_one<HD, LIMBS, T>();
   }
 };
 struct Launch {
@@ -666,8 +644,8 @@ struct Launch {
   int n_blocks;
   bool vec;
   cudaStream_t s;
-  template <int HD, int LIMBS, int MT, typename T> int operator()() const {
-    return launch_one<HD, LIMBS, MT, T>(a, b, runs, n_blocks, vec, s);
+  template <int HD, int LIMBS, typename T> int operator()() const {
+    return launch_one<HD, LIMBS, T>(a, b, runs, n_blocks, vec, s);
   }
 };
 
@@ -675,15 +653,14 @@ struct Launch {
 
 // CTAs per SM of the kernel for this shape on the current device (0: error).
 // Sets the kernel's shared-memory limit, so it comes before the launch.
-int extend_mma_resident(int head_dim, int dtype, int tile_rows) {
-  return head_dim == 128 ? pick<128>(dtype, tile_rows / 16, Resident{})
-                         : pick<64>(dtype, tile_rows / 16, Resident{});
+int extend_mma_resident(int head_dim, int dtype) {
+  return head_dim == 128 ? pick<128>(dtype, Resident{}) : pick<64>(dtype, Resident{});
 }
 
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                       bool vec, cudaStream_t s) {
   const Launch f{a, b, runs, n_blocks, vec, s};
-  return a.geom.gpd == 2 ? pick<128>(a.dtype, a.tile_rows / 16, f) : pick<64>(a.dtype, a.tile_rows / 16, f);
+  return a.geom.gpd == 2 ? pick<128>(a.dtype, f) : pick<64>(a.dtype, f);
 }
 
 }  // namespace eakv

@@ -29,17 +29,28 @@
 // Non-finite V groups are kept out of the products (0 NaN is NaN) and
 // listed by position; a row that attends one gets NaN in the group's dims.
 //
-// Roles (16 warps, the last two idle). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
-// per row; the weights go over S, and O is scaled when a maximum moves. Warps 8-11: dequantize, one thread per position: its K
-// and V rows come from global memory a tile ahead in registers and leave as
-// 16-byte stores in the 128-byte swizzle. A 32-bit word of nibbles becomes one
-// 16-byte chunk [d, d+2, d+1, d+3, d+32, d+34, d+33, d+35] (the pairs that one mask
-// selects); Q' is stored in the same order and the output's columns are read back
-// in it, so the order costs nothing. Warp 12 issues the MMAs: for tile i, PV of
-// row tile 0, S(i+1) of row tile 0, the same for row tile 1, so one row tile's
-// softmax runs under the other's MMAs. P' of a tile lies over its S (tensor
-// memory: 2 x 128 columns of S, 2 x 128 of O: all 512); the tensor pipe runs the
-// MMAs in order.
+// Roles (16 warps). Warps 0-3 and 4-7: softmax of row tile 0 and 1, one thread
+// per row, its 128 scores in registers; the weights go over S, and O is scaled
+// when a maximum moves. Warps 8-11: dequantize, one thread per position: its K and
+// V rows come from global memory a tile ahead in registers and leave as 16-byte
+// stores in the 128-byte swizzle. A 32-bit word of nibbles becomes one 16-byte
+// chunk [d, d+2, d+1, d+3, d+32, d+34, d+33, d+35] (the pairs that one mask selects);
+// Q' is stored in the same order and the output's columns are read back in it, so
+// the order costs nothing. Warp 12 issues the MMAs: for tile i, PV of row tile 0,
+// S(i+1) of row tile 0, the same for row tile 1, so one row tile's softmax runs
+// under the other's MMAs; PV starts on the first half of a tile's weights. Warp 13
+// finds the CTA's next part while this one is worked on; the last two only fill
+// their warpgroup. P' of a tile lies over its S (tensor memory: 2 x 128 columns of S,
+// 2 x 128 of O: all 512); the tensor pipe runs the MMAs in order. The softmax
+// warpgroups take registers from the other two.
+//
+// Bound: the tensor pipe, whose operands come from shared memory at its full rate
+// (S = Q'K' reads 128 bytes a cycle) next to the dequantizing stores: 2048 tokens
+// of 32 heads (8 KV heads, head_dim 128) behind 32768 positions in 1.05 ms,
+// 1.08 PFLOP/s. Tried and slower: tiles of 64 positions with two S buffers (its
+// MMAs are 1.4 times slower per value), one pass over the scores in place of the
+// registers, exponentials by polynomial on the FMA pipe for a quarter or half of
+// them (the exponentials are not what it waits for).
 //
 // All hand-overs are mbarriers with bounded, suspending waits; one that runs
 // out sets the status word, and every role leaves at its next wait.
@@ -91,13 +102,14 @@ struct WCfg {
   static constexpr int EXPS = V + kStages * TILE;            // short2 [kInfo][BN]: K, V
   static constexpr int INFO = EXPS + kInfo * BN * 4;         // int [kInfo][4 warps]
   static constexpr int NANS = INFO + kInfo * 16;             // uint2 [kInfo][4 warps]
-  static constexpr int ROWC = NANS + kInfo * 32;         // float [256]: score factor of a row
+  static constexpr int ROWC = NANS + kInfo * 32;             // float [256]: score factor of a row
   static constexpr int BARS = ROWC + 256 * 4;
-  static constexpr int SLOT = BARS + 8 * 18;           // tensor-memory base, `a wait ran out', merge flag
-  static constexpr int RED = SLOT + 16;                // int2 [4]
-  static constexpr int WALK = RED + 32;                // ExtWalk
+  // tensor-memory base, `a wait ran out', the item's last part, `its arrival is said'
+  static constexpr int SLOT = BARS + 8 * 18;
+  static constexpr int RED = SLOT + 16;                      // int2 [4 warps]: largest exponents
+  static constexpr int WALK = RED + 32;                      // ExtWalk
   static constexpr int END = WALK + 256;
-  static constexpr int SMEM = END + 1024;              // alignment slack
+  static constexpr int SMEM = END + 1024;                    // alignment slack
   static_assert(sizeof(ExtWalk) <= 256, "room for the walk");
   // tensor memory columns
   static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
@@ -430,82 +442,83 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     regs_down<kRegsMma>();
     regs_traded();
     if (warp == kMmaWarp) {
-    int done = 0, done0 = 0, done1 = 0;   // tiles of the parts before, of each row tile
-    // The whole warp walks the tiles, so that descriptors stay in uniform
-    // registers; one lane issues.
-    const bool issuer = elect_one();
-    const uint32_t sb = smem_u32(smem);
-    const uint64_t qd = sdesc(sb + C::Q, 16, 1024, kLayoutSW128);
-    const uint64_t kd = sdesc(sb + C::K, 16, 1024, kLayoutSW128);
-    const uint64_t vd = sdesc(sb + C::V, C::HALF, 1024, kLayoutSW128);
-    // a descriptor's address field counts 16 bytes
-    auto scores = [&](int m, int i) {
-      const uint64_t q = qd + (uint64_t)(m * (C::QTILE >> 4)), k = kd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
-      const uint32_t d = tm + C::S_COL + 128 * m;
-      if (issuer) {
-#pragma unroll
-        for (int s = 0; s < HD / 16; s++) {
-          const uint64_t off = ((s >> 2) * C::HALF + (s & 3) * 32) >> 4;
-          mma_f16_ss(d, q + off, k + off, idesc_f16(BN, 0), s > 0);
-        }
-        if (i != a.test_stall - 1) mma_commit(bar(kSFull + m));   // test hook: never ready
-        // the tile's K is free when the last row tile that uses it has its scores
-        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kKFree + ((done + i) & 1)));
-      }
-    };
-    // PV of tile i, half by half as the weights come; false when a wait ran out
-    auto outputs = [&](int m, int i, int n) {
-      const uint64_t v = vd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
-      const uint32_t p = tm + C::S_COL + 128 * m, d = tm + C::O_COL + HD * m;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (!wait_warp(kPFull + 2 * m + h, (m ? done1 : done0) + i)) return false;
-        fence_after_sync();
+      int done = 0, done0 = 0, done1 = 0;   // tiles of the parts before, of each row tile
+      // The whole warp walks the tiles, so that descriptors stay in uniform
+      // registers; one lane issues.
+      const bool issuer = elect_one();
+      const uint32_t sb = smem_u32(smem);
+      const uint64_t qd = sdesc(sb + C::Q, 16, 1024, kLayoutSW128);
+      const uint64_t kd = sdesc(sb + C::K, 16, 1024, kLayoutSW128);
+      const uint64_t vd = sdesc(sb + C::V, C::HALF, 1024, kLayoutSW128);
+      // a descriptor's address field counts 16 bytes
+      auto scores = [&](int m, int i) {
+        const uint64_t q = qd + (uint64_t)(m * (C::QTILE >> 4));
+        const uint64_t k = kd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
+        const uint32_t d = tm + C::S_COL + 128 * m;
         if (issuer) {
 #pragma unroll
-          for (int s = h * (BN / 32); s < (h + 1) * (BN / 32); s++)
-            mma_f16_ts(d, p + 8 * s, v + (uint64_t)(s * (2048 >> 4)), idesc_f16(HD, 1), i > 0 || s > 0);
+          for (int s = 0; s < HD / 16; s++) {
+            const uint64_t off = ((s >> 2) * C::HALF + (s & 3) * 32) >> 4;
+            mma_f16_ss(d, q + off, k + off, idesc_f16(BN, 0), s > 0);
+          }
+          if (i != a.test_stall - 1) mma_commit(bar(kSFull + m));   // test hook: never ready
+          // the tile's K is free when the last row tile that uses it has its scores
+          if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kKFree + ((done + i) & 1)));
         }
+      };
+      // PV of tile i, half by half as the weights come; false when a wait ran out
+      auto outputs = [&](int m, int i, int n) {
+        const uint64_t v = vd + (uint64_t)(((done + i) & 1) * (C::TILE >> 4));
+        const uint32_t p = tm + C::S_COL + 128 * m, d = tm + C::O_COL + HD * m;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (!wait_warp(kPFull + 2 * m + h, (m ? done1 : done0) + i)) return false;
+          fence_after_sync();
+          if (issuer) {
+#pragma unroll
+            for (int s = h * (BN / 32); s < (h + 1) * (BN / 32); s++)
+              mma_f16_ts(d, p + 8 * s, v + (uint64_t)(s * (2048 >> 4)), idesc_f16(HD, 1), i > 0 || s > 0);
+          }
+        }
+        if (issuer) {
+          if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kVFree + ((done + i) & 1)));
+          if (i == n - 1) mma_commit(bar(kODone + m));
+        }
+        return true;
+      };
+      // Each tile's K and V is waited for once, ahead of the weights that it is
+      // used behind, so that nothing stands between these and their MMAs.
+      for (int part = 0;; part++) {
+        const ExtItem &it = walk.item[part & 1];
+        if (!begin_part(it)) break;
+        meet();
+        if (n_tiles > 0 && wait_warp(kKFull + (done & 1), done >> 1)) {
+          fence_after_sync();
+          if (nt0 > 0) scores(0, 0);
+          if (nt1 > 0) scores(1, 0);
+        }
+        for (int i = 0; i < n_tiles && ok; i++) {
+          if (i + 1 < n_tiles && !wait_warp(kKFull + ((done + i + 1) & 1), (done + i + 1) >> 1)) break;
+          if (!wait_warp(kVFull + ((done + i) & 1), (done + i) >> 1)) break;
+          if (i < nt0) {
+            if (!outputs(0, i, nt0)) break;
+            if (i + 1 < nt0) scores(0, i + 1);
+          }
+          if (i < nt1) {
+            if (!outputs(1, i, nt1)) break;
+            if (i + 1 < nt1) scores(1, i + 1);
+          }
+        }
+        done += n_tiles;
+        done0 += nt0;
+        done1 += nt1;
+        meet();
+        if (*failed) break;
       }
-      if (issuer) {
-        if (m == (i < nt1 ? 1 : 0)) mma_commit(bar(kVFree + ((done + i) & 1)));
-        if (i == n - 1) mma_commit(bar(kODone + m));
-      }
-      return true;
-    };
-    // Each tile's K and V is waited for once, ahead of the weights that it is
-    // used behind, so that nothing stands between these and their MMAs.
-    for (int part = 0;; part++) {
-      const ExtItem &it = walk.item[part & 1];
-      if (!begin_part(it)) break;
-    meet();
-    if (n_tiles > 0 && wait_warp(kKFull + (done & 1), done >> 1)) {
-      fence_after_sync();
-      if (nt0 > 0) scores(0, 0);
-      if (nt1 > 0) scores(1, 0);
-    }
-    for (int i = 0; i < n_tiles && ok; i++) {
-      if (i + 1 < n_tiles && !wait_warp(kKFull + ((done + i + 1) & 1), (done + i + 1) >> 1)) break;
-      if (!wait_warp(kVFull + ((done + i) & 1), (done + i) >> 1)) break;
-      if (i < nt0) {
-        if (!outputs(0, i, nt0)) break;
-        if (i + 1 < nt0) scores(0, i + 1);
-      }
-      if (i < nt1) {
-        if (!outputs(1, i, nt1)) break;
-        if (i + 1 < nt1) scores(1, i + 1);
-      }
-    }
-    done += n_tiles;
-    done0 += nt0;
-    done1 += nt1;
-    meet();
-    if (*failed) break;
-    }
-    // every MMA has ended before the tensor memory is given back
-    if (issuer) mma_commit(bar(kDrain));
-    __syncwarp();
-    wait_warp(kDrain, 0);
+      // every MMA has ended before the tensor memory is given back
+      if (issuer) mma_commit(bar(kDrain));
+      __syncwarp();
+      wait_warp(kDrain, 0);
     } else if (warp == kWalkWarp) {
       // ================= walk: the next part, while this one is worked on ===========
       int part = 0;
@@ -591,325 +604,326 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         else rows(std::false_type{});
         fence_proxy_async_smem();
       }
-    meet();
-    references();
-    const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
-    const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
-    // score factor: |scale| log2 e / 2^(q exponent), with K's 2^kref
-    float c_row = reinterpret_cast<const float *>(smem + C::ROWC)[r_loc];
-    c_row *= pow2i(kref >> 1);
-    c_row *= pow2i(kref - (kref >> 1));
-    float m_run = -INFINITY, l_run = 0.0f;
-    int eref = kUnset;
-    bool poison0 = false, poison1 = false;   // a non-finite V group was attended
-    bool steady = true;   // of the warp: no row's eref is far from vref
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // tensor-memory lane 32 (warp % 4)
-    const uint32_t ts = tm + lanes + C::S_COL + 128 * mt, to = tm + lanes + C::O_COL + HD * mt;
-    // positions that every row of this row tile attends
-    const int first = it.row0 + 128 * mt, last = min(first + 127, it.row0 + it.rows - 1);
-    const int all_hi = min(a.tree ? it.old : it.old + first / a.G + 1, end_pos);
-    const int all_lo = a.window > 0 ? max(0, it.old + last / a.G + 1 - a.window) : 0;
-    const int my_tiles = mt ? nt1 : nt0;
+      meet();
+      references();
+      const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
+      const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
+      // score factor: |scale| log2 e / 2^(q exponent), with K's 2^kref
+      float c_row = reinterpret_cast<const float *>(smem + C::ROWC)[r_loc];
+      c_row *= pow2i(kref >> 1);
+      c_row *= pow2i(kref - (kref >> 1));
+      float m_run = -INFINITY, l_run = 0.0f;
+      int eref = kUnset;
+      bool poison0 = false, poison1 = false;   // a non-finite V group was attended
+      bool steady = true;   // of the warp: no row's eref is far from vref
+      const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // tensor-memory lane 32 (warp % 4)
+      const uint32_t ts = tm + lanes + C::S_COL + 128 * mt, to = tm + lanes + C::O_COL + HD * mt;
+      // positions that every row of this row tile attends
+      const int first = it.row0 + 128 * mt, last = min(first + 127, it.row0 + it.rows - 1);
+      const int all_hi = min(a.tree ? it.old : it.old + first / a.G + 1, end_pos);
+      const int all_lo = a.window > 0 ? max(0, it.old + last / a.G + 1 - a.window) : 0;
+      const int my_tiles = mt ? nt1 : nt0;
 
-    // O times f. Called between S(i) and P'(i): the commit that announced S(i)
-    // covers the MMAs before it, the tile before's PV among them, and tile i's is
-    // not issued yet.
-    auto scale_out = [&](float f) {
+      // O times f. Called between S(i) and P'(i): the commit that announced S(i)
+      // covers the MMAs before it, the tile before's PV among them, and tile i's is
+      // not issued yet.
+      auto scale_out = [&](float f) {
 #pragma unroll 1
-      for (int k = 0; k < HD; k += 16) {
-        uint32_t v[16];
-        tmem_ld16(to + k, v);
-        tmem_wait_ld();
+        for (int k = 0; k < HD; k += 16) {
+          uint32_t v[16];
+          tmem_ld16(to + k, v);
+          tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-        tmem_st16(to + k, v);
-      }
-    };
-    // Half h of the tile's weights is in tensor memory (and O is scaled).
-    auto announce = [&](int h) {
-      tmem_wait_st();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPFull + 2 * mt + h));
-    };
-    // The scores' maximum xm of a tile (base 2, -inf: none) moves the running
-    // maximum when it passes it by 8; `f` is what the sums so far are scaled by.
-    auto new_max = [&](float xm, float &f) {
-      f = 1.0f;
-      if (xm > m_run + 8.0f) {
-        f = ex2(m_run - xm);
-        m_run = xm;
-        l_run *= f;
-        return true;
-      }
-      return false;
-    };
+          for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+          tmem_st16(to + k, v);
+        }
+      };
+      // Half h of the tile's weights is in tensor memory (and O is scaled).
+      auto announce = [&](int h) {
+        tmem_wait_st();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPFull + 2 * mt + h));
+      };
+      // The scores' maximum xm of a tile (base 2, -inf: none) moves the running
+      // maximum when it passes it by 8; `f` is what the sums so far are scaled by.
+      auto new_max = [&](float xm, float &f) {
+        f = 1.0f;
+        if (xm > m_run + 8.0f) {
+          f = ex2(m_run - xm);
+          m_run = xm;
+          l_run *= f;
+          return true;
+        }
+        return false;
+      };
 
-    // A tile without marked rows: the row's 128 scores in registers.
-    auto tile_fast = [&](auto masked_tag, int i) {
-      constexpr bool MASKED = decltype(masked_tag)::value;
-      const int c0 = base_pos + i * BN;
-      uint32_t v[4][32];
+      // A tile without marked rows: the row's 128 scores in registers.
+      auto tile_fast = [&](auto masked_tag, int i) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        const int c0 = base_pos + i * BN;
+        uint32_t v[4][32];
 #pragma unroll
-      for (int ch = 0; ch < 4; ch++) tmem_ld32(ts + 32 * ch, v[ch]);
+        for (int ch = 0; ch < 4; ch++) tmem_ld32(ts + 32 * ch, v[ch]);
 #pragma unroll
-      for (int ch = 0; ch < 4; ch++) wait_ld_of(v[ch]);
-      if constexpr (MASKED) {
+        for (int ch = 0; ch < 4; ch++) wait_ld_of(v[ch]);
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int ch = 0; ch < 4; ch++) {
+            const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (!((on >> e) & 1)) v[ch][e] = 0xff800000u;   // -inf
+          }
+        }
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int ch = 0; ch < 4; ch++)
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              t[k] = max3(t[k], __uint_as_float(v[ch][e + 2 * k]), __uint_as_float(v[ch][e + 2 * k + 1]));
+        const float mx = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+        // the maximum of nothing stays -inf (-inf * 0 is NaN)
+        const float xm = mx == -INFINITY ? mx : mx * c_row;
+        if (eref == kUnset) eref = vref;
+        if (__any_sync(0xffffffffu, xm > m_run + 8.0f)) {
+          float f;
+          new_max(xm, f);
+          if (i > 0) scale_out(f);
+        }
+        // the weights carry 2^(vref - eref) whole; the sum takes it off
+        const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run) + (float)(vref - eref);
+        const float2 c2 = make_float2(c_row, c_row), o2 = make_float2(off, off);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int ch = 0; ch < 4; ch++) {
+          uint32_t p16[16];
+          const uint32_t (&x)[32] = v[ch];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, o2);
+            float2 p = make_float2(ex2(y.x), ex2(y.y));
+            if (MASKED) {   // -inf * 0 where c_row is 0
+              if (x[e] == 0xff800000u) p.x = 0.0f;
+              if (x[e + 1] == 0xff800000u) p.y = 0.0f;
+            }
+            sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], p);
+            p16[e >> 1] = pack_f16(p.x, p.y);
+          }
+          tmem_st16(ts + 16 * ch, p16);
+          if (ch == 1) announce(0);
+        }
+        l_run += (sum[0].x + sum[0].y + sum[1].x + sum[1].y) * pow2i(eref - vref);
+        announce(1);
+      };
+
+      // Any tile: every position with its own powers of two.
+      auto tile_slow = [&](int i, int marks) {
+        const int c0 = base_pos + i * BN;
+        const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + ((all_done + i) % kInfo) * BN;
+        float mx = -INFINITY;
+        int emax = kUnset;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ch++) {
+          uint32_t v[32];
+          tmem_ld32(ts + 32 * ch, v);
           const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+          const bool mk = (marks >> ch) & 1;
+          wait_ld_of(v);
 #pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (!((on >> e) & 1)) v[ch][e] = 0xff800000u;   // -inf
+          for (int e = 0; e < 32; e++) {
+            const short2 x = mk ? ex[32 * ch + e] : make_short2(kref, vref);
+            if ((on >> e) & 1) {
+              mx = fmaxf(mx, __uint_as_float(v[e]) * pow2i(x.x - kref));
+              emax = max(emax, (int)x.y);
+            }
+          }
         }
-      }
-      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int ch = 0; ch < 4; ch++)
-#pragma unroll
-        for (int e = 0; e < 32; e += 8)
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            t[k] = max3(t[k], __uint_as_float(v[ch][e + 2 * k]), __uint_as_float(v[ch][e + 2 * k + 1]));
-      const float mx = fmaxf(max3(t[0], t[1], t[2]), t[3]);
-      // the maximum of nothing stays -inf (-inf * 0 is NaN)
-      const float xm = mx == -INFINITY ? mx : mx * c_row;
-      if (eref == kUnset) eref = vref;
-      if (__any_sync(0xffffffffu, xm > m_run + 8.0f)) {
         float f;
-        new_max(xm, f);
-        if (i > 0) scale_out(f);
-      }
-      // the weights carry 2^(vref - eref) whole; the sum takes it off
-      const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run) + (float)(vref - eref);
-      const float2 c2 = make_float2(c_row, c_row), o2 = make_float2(off, off);
-      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-      for (int ch = 0; ch < 4; ch++) {
-        uint32_t p16[16];
-        const uint32_t (&x)[32] = v[ch];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, o2);
-          float2 p = make_float2(ex2(y.x), ex2(y.y));
-          if (MASKED) {   // -inf * 0 where c_row is 0
-            if (x[e] == 0xff800000u) p.x = 0.0f;
-            if (x[e + 1] == 0xff800000u) p.y = 0.0f;
-          }
-          sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], p);
-          p16[e >> 1] = pack_f16(p.x, p.y);
+        bool move = new_max(mx == -INFINITY ? mx : mx * c_row, f);
+        if (emax != kUnset && (eref == kUnset || emax > eref)) {
+          if (eref != kUnset) f *= pow2i(eref - emax);
+          eref = emax;
+          move = true;
         }
-        tmem_st16(ts + 16 * ch, p16);
-        if (ch == 1) announce(0);
-      }
-      l_run += (sum[0].x + sum[0].y + sum[1].x + sum[1].y) * pow2i(eref - vref);
-      announce(1);
-    };
-
-    // Any tile: every position with its own powers of two.
-    auto tile_slow = [&](int i, int marks) {
-      const int c0 = base_pos + i * BN;
-      const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + ((all_done + i) % kInfo) * BN;
-      float mx = -INFINITY;
-      int emax = kUnset;
+        if (i > 0 && __any_sync(0xffffffffu, move)) scale_out(f);
+        const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll 1
-      for (int ch = 0; ch < 4; ch++) {
-        uint32_t v[32];
-        tmem_ld32(ts + 32 * ch, v);
-        const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
-        const bool mk = (marks >> ch) & 1;
-        wait_ld_of(v);
+        for (int ch = 0; ch < 4; ch++) {
+          uint32_t v[32], p16[16];
+          tmem_ld32(ts + 32 * ch, v);
+          const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
+          const bool mk = (marks >> ch) & 1;
+          wait_ld_of(v);
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const short2 x = mk ? ex[32 * ch + e] : make_short2(kref, vref);
-          if ((on >> e) & 1) {
-            mx = fmaxf(mx, __uint_as_float(v[e]) * pow2i(x.x - kref));
-            emax = max(emax, (int)x.y);
-          }
-        }
-      }
-      float f;
-      bool move = new_max(mx == -INFINITY ? mx : mx * c_row, f);
-      if (emax != kUnset && (eref == kUnset || emax > eref)) {
-        if (eref != kUnset) f *= pow2i(eref - emax);
-        eref = emax;
-        move = true;
-      }
-      if (i > 0 && __any_sync(0xffffffffu, move)) scale_out(f);
-      const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
-#pragma unroll 1
-      for (int ch = 0; ch < 4; ch++) {
-        uint32_t v[32], p16[16];
-        tmem_ld32(ts + 32 * ch, v);
-        const uint32_t on = mask32(mask, c0 + 32 * ch, end_pos);
-        const bool mk = (marks >> ch) & 1;
-        wait_ld_of(v);
+          for (int e = 0; e < 32; e += 2) {
+            float w[2];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float w[2];
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const short2 x = mk ? ex[32 * ch + e + u] : make_short2(kref, vref);
-            const bool at = (on >> (e + u)) & 1;
-            const float p = at ? ex2(fmaf(__uint_as_float(v[e + u]) * pow2i(x.x - kref), c_row, off)) : 0.0f;
-            l_run += p;
-            w[u] = at ? p * pow2i(x.y - eref) : 0.0f;
-          }
-          p16[e >> 1] = pack_f16(w[0], w[1]);
-        }
-        tmem_st16(ts + 16 * ch, p16);
-      }
-      announce(0);
-      announce(1);
-    };
-
-    for (int i = 0; i < my_tiles; i++) {
-      if (!wait_warp(kSFull + mt, done + i)) break;
-      fence_after_sync();
-      const int c0 = base_pos + i * BN;
-      const bool full = c0 >= all_lo && c0 + BN <= all_hi;
-      // bit 0 of a warp's word: marked rows, bit 1: non-finite V groups
-      const int4 sum = *reinterpret_cast<const int4 *>(smem + C::INFO + ((all_done + i) % kInfo) * 16);
-      const int any = sum.x | sum.y | sum.z | sum.w;
-      if (any & 2) {
-        const uint2 *bad = reinterpret_cast<const uint2 *>(smem + C::NANS) + ((all_done + i) % kInfo) * 4;
-        for (int w = 0; w < 4; w++) {
-          const uint32_t on = mask32(mask, c0 + 32 * w, end_pos);
-          poison0 = poison0 || (on & bad[w].x);
-          poison1 = poison1 || (on & bad[w].y);
-        }
-      }
-      if ((any & 1) || !steady) {
-        tile_slow(i, (sum.x & 1) | (sum.y & 1) << 1 | (sum.z & 1) << 2 | (sum.w & 1) << 3);
-        steady = __all_sync(0xffffffffu, eref == kUnset || (eref >= vref && eref <= vref + 30));
-      } else if (full) {
-        tile_fast(std::false_type{}, i);
-      } else {
-        tile_fast(std::true_type{}, i);
-      }
-    }
-
-    // ---- results ----------------------------------------------------------------
-    if (ok && my_tiles > 0) wait_warp(kODone + mt, parts);
-    // both row tiles are through with K' and V': their space takes the rows on
-    // their way out
-    named_sync(1, kSoftWarps * 32);
-    if (ok) {
-      fence_after_sync();
-      const float down = 0.0078125f;   // 2^-kPShift
-      const float L = l_run * down;
-      // O carries 2^(kPShift - eref); in two factors. Finished rows are divided here.
-      const int e = eref == kUnset ? 0 : eref;
-      const float inv = it.n_parts > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
-      const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1)) * inv;
-      if (r_loc < it.rows) {
-        if (it.n_parts > 1) {
-          const size_t pr = part_row(a, it.slot, r_loc);
-          a.part_m[pr] = m_run;
-          a.part_l[pr] = L;
-        } else if (a.lse) {
-          extend_lse(a, it, r_loc, m_run, L);
-        }
-      }
-      // A thread's row leaves by way of shared memory, so that whole lines are
-      // stored: up to 256 bytes of a row at a time, 32 rows per warp.
-      uint8_t *stage = smem + C::K + warp * (32 * 256);
-      static_assert(8 * 32 * 256 <= 2 * kStages * C::TILE, "room for the rows of eight warps");
-      const int per_pass = it.n_parts > 1 ? 64 : HD;
-      const bool spoiled = __any_sync(0xffffffffu, poison0 || poison1);
-#pragma unroll 1
-      for (int d0 = 0; d0 < HD; d0 += per_pass) {
-        // 16 columns: dims 4j..4j+7 and 32 on of a 64-dim group
-#pragma unroll 2
-        for (int j = d0 / 8; j < (d0 + per_pass) / 8; j += 2) {
-          uint32_t v[16];
-          if (my_tiles > 0) {
-            tmem_ld16(to + 8 * j, v);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int k = 0; k < 16; k++) v[k] = 0u;
-          }
-          float o[16];
-#pragma unroll
-          for (int k = 0; k < 16; k++) o[k] = __uint_as_float(v[k]) * f0 * f1;
-          if (spoiled && (j < 8 ? poison0 : poison1)) {
-#pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = __uint_as_float(0x7fc00000u);
-          }
-          const float lo[8] = {o[0], o[2], o[1], o[3], o[8], o[10], o[9], o[11]};
-          const float hi[8] = {o[4], o[6], o[5], o[7], o[12], o[14], o[13], o[15]};
-          const int d = 64 * (j >> 3) + 4 * (j & 7) - d0;   // within the pass
-          // 16-byte chunks of the row, rotated by the lane
-          auto put = [&](int byte, uint4 x) {
-            *reinterpret_cast<uint4 *>(stage + lane * 256 + ((byte + 16 * lane) & 255)) = x;
-          };
-          if (it.n_parts > 1) {
-#pragma unroll
-            for (int k = 0; k < 8; k += 4) {
-              put(4 * (d + k), make_uint4(__float_as_uint(lo[k]), __float_as_uint(lo[k + 1]),
-                                          __float_as_uint(lo[k + 2]), __float_as_uint(lo[k + 3])));
-              put(4 * (d + 32 + k), make_uint4(__float_as_uint(hi[k]), __float_as_uint(hi[k + 1]),
-                                               __float_as_uint(hi[k + 2]), __float_as_uint(hi[k + 3])));
+            for (int u = 0; u < 2; u++) {
+              const short2 x = mk ? ex[32 * ch + e + u] : make_short2(kref, vref);
+              const bool at = (on >> (e + u)) & 1;
+              const float p = at ? ex2(fmaf(__uint_as_float(v[e + u]) * pow2i(x.x - kref), c_row, off)) : 0.0f;
+              l_run += p;
+              w[u] = at ? p * pow2i(x.y - eref) : 0.0f;
             }
-          } else {
-            put(2 * d, make_uint4(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(lo[4], lo[5]),
-                                  pack2<T>(lo[6], lo[7])));
-            put(2 * d + 64, make_uint4(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]), pack2<T>(hi[4], hi[5]),
-                                       pack2<T>(hi[6], hi[7])));
+            p16[e >> 1] = pack_f16(w[0], w[1]);
+          }
+          tmem_st16(ts + 16 * ch, p16);
+        }
+        announce(0);
+        announce(1);
+      };
+
+      for (int i = 0; i < my_tiles; i++) {
+        if (!wait_warp(kSFull + mt, done + i)) break;
+        fence_after_sync();
+        const int c0 = base_pos + i * BN;
+        const bool full = c0 >= all_lo && c0 + BN <= all_hi;
+        // bit 0 of a warp's word: marked rows, bit 1: non-finite V groups
+        const int4 sum = *reinterpret_cast<const int4 *>(smem + C::INFO + ((all_done + i) % kInfo) * 16);
+        const int any = sum.x | sum.y | sum.z | sum.w;
+        if (any & 2) {
+          const uint2 *bad = reinterpret_cast<const uint2 *>(smem + C::NANS) + ((all_done + i) % kInfo) * 4;
+          for (int w = 0; w < 4; w++) {
+            const uint32_t on = mask32(mask, c0 + 32 * w, end_pos);
+            poison0 = poison0 || (on & bad[w].x);
+            poison1 = poison1 || (on & bad[w].y);
           }
         }
-        __syncwarp();
-        // whole rows again: a lane's chunk of rows rr0, rr0 + rows per step, ...
-        const bool record = it.n_parts > 1;
-        const int cpr = record ? 16 : HD / 8;   // chunks of a row
-        const int ch = lane & (cpr - 1), step = 32 / cpr, rr0 = lane / cpr;
-        const int n_rows = it.rows - 32 * warp;   // of this warp (row tiles are 4 warps of 32 rows)
-        float *po = a.part_o + part_row(a, it.slot, 32 * warp) * HD + d0 + 4 * ch;
-        RowWalk row(a, it, a.out, 32 * warp + rr0, step);
-        auto chunk = [&](int rr) {
-          return *reinterpret_cast<const uint4 *>(stage + rr * 256 + ((16 * ch + 16 * rr) & 255));
-        };
-        if (record) {
-#pragma unroll 4
-          for (int rr = rr0; rr < min(32, n_rows); rr += step) *reinterpret_cast<uint4 *>(po + rr * HD) = chunk(rr);
+        if ((any & 1) || !steady) {
+          tile_slow(i, (sum.x & 1) | (sum.y & 1) << 1 | (sum.z & 1) << 2 | (sum.w & 1) << 3);
+          steady = __all_sync(0xffffffffu, eref == kUnset || (eref >= vref && eref <= vref + 30));
+        } else if (full) {
+          tile_fast(std::false_type{}, i);
         } else {
-#pragma unroll 4
-          for (int rr = rr0; rr < min(32, n_rows); rr += step) {
-            T *p = reinterpret_cast<T *>(a.out.data) + row.at + 8 * ch;
-            const uint4 y = chunk(rr);
-            if (vec) {
-              // 8-byte pieces: rows start on 4-element boundaries
-              reinterpret_cast<uint2 *>(p)[0] = make_uint2(y.x, y.y);
-              reinterpret_cast<uint2 *>(p)[1] = make_uint2(y.z, y.w);
-            } else {
-              const T *e8 = reinterpret_cast<const T *>(&y);
-#pragma unroll
-              for (int k = 0; k < 8; k++) p[k] = e8[k];
-            }
-            row.step();
+          tile_fast(std::true_type{}, i);
+        }
+      }
+
+      // ---- results ----------------------------------------------------------------
+      if (ok && my_tiles > 0) wait_warp(kODone + mt, parts);
+      // both row tiles are through with K' and V': their space takes the rows on
+      // their way out
+      named_sync(1, kSoftWarps * 32);
+      if (ok) {
+        fence_after_sync();
+        const float down = 0.0078125f;   // 2^-kPShift
+        const float L = l_run * down;
+        // O carries 2^(kPShift - eref); in two factors. Finished rows are divided here.
+        const int e = eref == kUnset ? 0 : eref;
+        const float inv = it.n_parts > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
+        const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1)) * inv;
+        if (r_loc < it.rows) {
+          if (it.n_parts > 1) {
+            const size_t pr = part_row(a, it.slot, r_loc);
+            a.part_m[pr] = m_run;
+            a.part_l[pr] = L;
+          } else if (a.lse) {
+            extend_lse(a, it, r_loc, m_run, L);
           }
         }
-        __syncwarp();
+        // A thread's row leaves by way of shared memory, so that whole lines are
+        // stored: up to 256 bytes of a row at a time, 32 rows per warp.
+        uint8_t *stage = smem + C::K + warp * (32 * 256);
+        static_assert(8 * 32 * 256 <= 2 * kStages * C::TILE, "room for the rows of eight warps");
+        const int per_pass = it.n_parts > 1 ? 64 : HD;
+        const bool spoiled = __any_sync(0xffffffffu, poison0 || poison1);
+#pragma unroll 1
+        for (int d0 = 0; d0 < HD; d0 += per_pass) {
+          // 16 columns: dims 4j..4j+7 and 32 on of a 64-dim group
+#pragma unroll 2
+          for (int j = d0 / 8; j < (d0 + per_pass) / 8; j += 2) {
+            uint32_t v[16];
+            if (my_tiles > 0) {
+              tmem_ld16(to + 8 * j, v);
+              tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; k++) v[k] = 0u;
+            }
+            float o[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = __uint_as_float(v[k]) * f0 * f1;
+            if (spoiled && (j < 8 ? poison0 : poison1)) {
+#pragma unroll
+              for (int k = 0; k < 16; k++) o[k] = __uint_as_float(0x7fc00000u);
+            }
+            const float lo[8] = {o[0], o[2], o[1], o[3], o[8], o[10], o[9], o[11]};
+            const float hi[8] = {o[4], o[6], o[5], o[7], o[12], o[14], o[13], o[15]};
+            const int d = 64 * (j >> 3) + 4 * (j & 7) - d0;   // within the pass
+            // 16-byte chunks of the row, rotated by the lane
+            auto put = [&](int byte, uint4 x) {
+              *reinterpret_cast<uint4 *>(stage + lane * 256 + ((byte + 16 * lane) & 255)) = x;
+            };
+            if (it.n_parts > 1) {
+#pragma unroll
+              for (int k = 0; k < 8; k += 4) {
+                put(4 * (d + k), make_uint4(__float_as_uint(lo[k]), __float_as_uint(lo[k + 1]),
+                                            __float_as_uint(lo[k + 2]), __float_as_uint(lo[k + 3])));
+                put(4 * (d + 32 + k), make_uint4(__float_as_uint(hi[k]), __float_as_uint(hi[k + 1]),
+                                                 __float_as_uint(hi[k + 2]), __float_as_uint(hi[k + 3])));
+              }
+            } else {
+              put(2 * d, make_uint4(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(lo[4], lo[5]),
+                                    pack2<T>(lo[6], lo[7])));
+              put(2 * d + 64, make_uint4(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]), pack2<T>(hi[4], hi[5]),
+                                         pack2<T>(hi[6], hi[7])));
+            }
+          }
+          __syncwarp();
+          // whole rows again: a lane's chunk of rows rr0, rr0 + rows per step, ...
+          const bool record = it.n_parts > 1;
+          const int cpr = record ? 16 : HD / 8;   // chunks of a row
+          const int ch = lane & (cpr - 1), step = 32 / cpr, rr0 = lane / cpr;
+          const int n_rows = it.rows - 32 * warp;   // of this warp (row tiles are 4 warps of 32 rows)
+          float *po = a.part_o + part_row(a, it.slot, 32 * warp) * HD + d0 + 4 * ch;
+          RowWalk row(a, it, a.out, 32 * warp + rr0, step);
+          auto chunk = [&](int rr) {
+            return *reinterpret_cast<const uint4 *>(stage + rr * 256 + ((16 * ch + 16 * rr) & 255));
+          };
+          if (record) {
+#pragma unroll 4
+            for (int rr = rr0; rr < min(32, n_rows); rr += step)
+              *reinterpret_cast<uint4 *>(po + rr * HD) = chunk(rr);
+          } else {
+#pragma unroll 4
+            for (int rr = rr0; rr < min(32, n_rows); rr += step) {
+              T *p = reinterpret_cast<T *>(a.out.data) + row.at + 8 * ch;
+              const uint4 y = chunk(rr);
+              if (vec) {
+                // 8-byte pieces: rows start on 4-element boundaries
+                reinterpret_cast<uint2 *>(p)[0] = make_uint2(y.x, y.y);
+                reinterpret_cast<uint2 *>(p)[1] = make_uint2(y.z, y.w);
+              } else {
+                const T *e8 = reinterpret_cast<const T *>(&y);
+#pragma unroll
+                for (int k = 0; k < 8; k++) p[k] = e8[k];
+              }
+              row.step();
+            }
+          }
+          __syncwarp();
+        }
       }
-    }
-    if (it.n_parts > 1) {
-      // warps that gave up leave their mark ahead of this barrier
-      volatile int *said = reinterpret_cast<volatile int *>(smem + C::SLOT + 12);
-      named_sync(1, kSoftWarps * 32);
-      if (threadIdx.x == 0) *said = !*failed;
-      named_sync(1, kSoftWarps * 32);
-      if (*said && extend_arrive_last<kSoftWarps * 32>(a, it, reinterpret_cast<int *>(smem + C::SLOT + 8), 1))
-        extend_merge<HD, T, kSoftWarps * 32>(a, it, vec, reinterpret_cast<float *>(smem + C::K),
-                                             2 * kStages * C::TILE / 4, 1);
-    }
-    done += my_tiles;
-    all_done += n_tiles;
-    parts += my_tiles > 0;
-    fence_before_sync();
-    meet();
-    fence_after_sync();
-    if (*failed) break;
+      if (it.n_parts > 1) {
+        // warps that gave up leave their mark ahead of this barrier
+        volatile int *said = reinterpret_cast<volatile int *>(smem + C::SLOT + 12);
+        named_sync(1, kSoftWarps * 32);
+        if (threadIdx.x == 0) *said = !*failed;
+        named_sync(1, kSoftWarps * 32);
+        if (*said && extend_arrive_last<kSoftWarps * 32>(a, it, reinterpret_cast<int *>(smem + C::SLOT + 8), 1))
+          extend_merge<HD, T, kSoftWarps * 32>(a, it, vec, reinterpret_cast<float *>(smem + C::K),
+                                               2 * kStages * C::TILE / 4, 1);
+      }
+      done += my_tiles;
+      all_done += n_tiles;
+      parts += my_tiles > 0;
+      fence_before_sync();
+      meet();
+      fence_after_sync();
+      if (*failed) break;
     }
     regs_down<kRegs>();
   }

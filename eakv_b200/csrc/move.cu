@@ -202,7 +202,16 @@ struct ReadArgs {
   long long layer_stride;    // elements
 };
 
-constexpr int kReadTok = 4;   // positions per warp, their loads first
+constexpr int kReadTok = 8;   // positions per warp, their loads first
+
+// Four nibbles of a word (from bit sh, every eighth) as f32: each byte placed in
+// the mantissa of 2^23, and 2^23 taken off.
+__device__ __forceinline__ void nibbles4(uint32_t word, int sh, float (&n)[4]) {
+  const uint32_t w = (word >> sh) & 0x0F0F0F0Fu;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    n[e] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + e)) - 8388608.0f;
+}
 
 // Warp: kReadTok neighbouring tokens of one (layer, K/V, head) (two heads at
 // head_dim 64): 128 elements per token, four per lane. Bound: HBM, mostly the
@@ -217,38 +226,45 @@ read_kernel(const __grid_constant__ ReadArgs a, const __grid_constant__ TokenBat
   const Rows out = a.out[lkv & 1];
   if (!out.data) return;
   const int layer = a.layer0 + (lkv >> 1);
-  const long long w = (long long)blockIdx.x * (kThreads / 32) + warp;
-  const int t0 = (int)(w / hsets) * kReadTok;   // heads vary fastest: a block's stores are near
-  const int h = (int)(w % hsets) * HPW + lane / LPR;
+  const unsigned w = blockIdx.x * (kThreads / 32) + warp;
+  const int run = w / hsets;   // heads vary fastest: a block's stores are near
+  const int t0 = run * kReadTok, h = (int)(w - run * hsets) * HPW + lane / LPR;
   if (t0 >= a.total || h >= a.geom.n_heads) return;
   const int d0 = 4 * (lane % LPR), grp = d0 >> 6, k = d0 & 63;
   uint32_t word[kReadTok];
   float2 sb[kReadTok];
   int cache = token_cache(batch, a.n_caches, t0);
+  // the head's pages of the cache that the tokens are in, and where it ends
+  const uint8_t *unit = batch.base[cache] + page_index(a.geom, layer, lkv & 1, h, 0) * a.geom.page_bytes;
+  int end = batch.first[cache + 1], shift = batch.pos[cache] - batch.first[cache];
 #pragma unroll
   for (int r = 0; r < kReadTok; r++) {
     const int t = t0 + r;
     if (t < a.total) {
-      while (t >= batch.first[cache + 1]) cache++;   // first[n_caches] = total > t
-      const int at = batch.pos[cache] + (t - batch.first[cache]);
-      const int page = at / kPagePositions, slot = (at % kPagePositions) * GPD + grp;
-      const uint8_t *pp = batch.base[cache] +
-                          page_index(a.geom, layer, lkv & 1, h, page) * a.geom.page_bytes;
-      word[r] = *reinterpret_cast<const uint32_t *>(pp + (size_t)slot * 32 + (k & 31));
-      sb[r] = *reinterpret_cast<const float2 *>(pp + a.geom.nib_bytes + (size_t)slot * 8);
+      while (t >= end) {   // first[n_caches] = total > t
+        cache++;
+        unit = batch.base[cache] + page_index(a.geom, layer, lkv & 1, h, 0) * a.geom.page_bytes;
+        end = batch.first[cache + 1];
+        shift = batch.pos[cache] - batch.first[cache];
+      }
+      const int at = t + shift, slot = (at % kPagePositions) * GPD + grp;
+      const uint8_t *pp = unit + (size_t)(at / kPagePositions) * a.geom.page_bytes;
+      word[r] = *reinterpret_cast<const uint32_t *>(pp + slot * 32 + (k & 31));
+      sb[r] = *reinterpret_cast<const float2 *>(pp + a.geom.nib_bytes + slot * 8);
     }
   }
   const int sh = k < 32 ? 0 : 4;
   T *base = reinterpret_cast<T *>(out.data) + (long long)(lkv >> 1) * a.layer_stride +
-            (long long)h * out.head_stride + d0;
+            (long long)h * out.head_stride + d0 + (long long)t0 * out.token_stride;
 #pragma unroll
   for (int r = 0; r < kReadTok; r++) {
     if (t0 + r >= a.total) break;
     float v[4];
+    nibbles4(word[r], sh, v);
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      v[e] = fmaf((float)((word[r] >> (8 * e + sh)) & 15), sb[r].x, sb[r].y);
-    store4<T, kVec>(base + (long long)(t0 + r) * out.token_stride, v);
+    for (int e = 0; e < 4; e++) v[e] = fmaf(v[e], sb[r].x, sb[r].y);
+    store4<T, kVec>(base, v);
+    base += out.token_stride;
   }
 }
 
@@ -258,6 +274,7 @@ cudaError_t read_launch(const ReadArgs &a, const TokenBatch &b, int n_layers, bo
   constexpr int HPW = 128 / HD;
   const long long warps = (long long)((a.total + kReadTok - 1) / kReadTok) *
                           ((a.geom.n_heads + HPW - 1) / HPW);
+  if (warps > (1ll << 31)) return cudaErrorInvalidValue;   // a warp's number is 32 bits
   const dim3 grid((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)), 2 * n_layers);
   if (vec) read_kernel<HD, T, true><<<grid, kThreads, 0, s>>>(a, b);
   else read_kernel<HD, T, false><<<grid, kThreads, 0, s>>>(a, b);
