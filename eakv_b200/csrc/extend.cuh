@@ -327,60 +327,64 @@ __device__ __forceinline__ void extend_store(const ExtendArgs &a, const ExtItem 
 }
 
 // The last part of an item: rows merged over the parts, in their order, four
-// dims per thread at a time, by NT threads that meet on named barrier `id`. `ws`
-// is free shared memory of ws_floats: the parts' weights of a row are worked out
-// once into it, and the records' loads then depend on nothing.
+// dims of kRows rows per thread at a time (their loads are what this waits for: with
+// one row at a time the merge of 3 parts of 256 rows took 27 us), by NT threads
+// that meet on named barrier `id`. `ws` is free shared memory of ws_floats, more
+// than an item has parts: the weights of a row's parts are worked out once into it.
 template <int HD, typename T, int NT>
 __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem &it, bool vec, float *ws,
                                              int ws_floats, int id) {
-  const int ns = it.n_parts;
-  float *m_s = ws, *l_s = ws + it.rows, *f_s = ws + 2 * it.rows;   // [rows], [rows], [rows][ns]
-  const bool staged = (ns + 2) * it.rows <= ws_floats;
-  if (staged) {
-    for (int x = threadIdx.x; x < it.rows * ns; x += NT)
-      f_s[x] = __ldcg(a.part_m + part_row(a, part_slot(it, x % ns), x / ns));
+  constexpr int kRows = 4;
+  const int ns = it.n_parts, most = min(it.rows, ws_floats / (ns + 2));
+  for (int r0 = 0; r0 < it.rows; r0 += most) {
+    const int rows = min(most, it.rows - r0);
+    float *m_s = ws, *l_s = ws + rows, *f_s = ws + 2 * rows;   // [rows], [rows], [rows][ns]
+    for (int x = threadIdx.x; x < rows * ns; x += NT) {
+      const int r = x / ns;
+      f_s[x] = __ldcg(a.part_m + part_row(a, part_slot(it, x - r * ns), r0 + r));
+    }
     named_sync(id, NT);
-    for (int r = threadIdx.x; r < it.rows; r += NT) {
+    for (int r = threadIdx.x; r < rows; r += NT) {
       float M = -INFINITY, L = 0.0f;
       for (int s = 0; s < ns; s++) M = fmaxf(M, f_s[r * ns + s]);
 #pragma unroll 4
       for (int s = 0; s < ns; s++) {
         const float f = part_weight(f_s[r * ns + s], M);
         f_s[r * ns + s] = f;
-        L = fmaf(f, __ldcg(a.part_l + part_row(a, part_slot(it, s), r)), L);
+        L = fmaf(f, __ldcg(a.part_l + part_row(a, part_slot(it, s), r0 + r)), L);
       }
       m_s[r] = M;
       l_s[r] = L;
     }
     named_sync(id, NT);
-  }
-  for (int x = threadIdx.x; x < it.rows * (HD / 4); x += NT) {
-    const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-    float M = -INFINITY, L = 0.0f;
-    if (staged) {
-      M = m_s[r];
-      L = l_s[r];
-    } else {
-      for (int s = 0; s < ns; s++) M = fmaxf(M, __ldcg(a.part_m + part_row(a, part_slot(it, s), r)));
-    }
-    float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < ns; s++) {
-      const size_t pr = part_row(a, part_slot(it, s), r);
-      const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + pr * HD + d));
-      float f;
-      if (staged) {
-        f = f_s[r * ns + s];
-      } else {
-        f = part_weight(__ldcg(a.part_m + pr), M);
-        L = fmaf(f, __ldcg(a.part_l + pr), L);
+    const int n = rows * (HD / 4);
+    for (int x0 = threadIdx.x; x0 < n; x0 += kRows * NT) {
+      float O[kRows][4];
+#pragma unroll
+      for (int k = 0; k < kRows; k++) O[k][0] = O[k][1] = O[k][2] = O[k][3] = 0.0f;
+#pragma unroll 2
+      for (int s = 0; s < ns; s++) {
+        const float *po = a.part_o + part_row(a, part_slot(it, s), r0) * HD;
+        float4 o[kRows];
+#pragma unroll
+        for (int k = 0; k < kRows; k++)   // the last again behind the end
+          o[k] = __ldcg(reinterpret_cast<const float4 *>(po + 4 * min(x0 + k * NT, n - 1)));
+#pragma unroll
+        for (int k = 0; k < kRows; k++) {
+          const float f = f_s[min(x0 + k * NT, n - 1) / (HD / 4) * ns + s];
+          O[k][0] = fmaf(f, o[k].x, O[k][0]);
+          O[k][1] = fmaf(f, o[k].y, O[k][1]);
+          O[k][2] = fmaf(f, o[k].z, O[k][2]);
+          O[k][3] = fmaf(f, o[k].w, O[k][3]);
+        }
       }
-      O[0] = fmaf(f, o.x, O[0]);
-      O[1] = fmaf(f, o.y, O[1]);
-      O[2] = fmaf(f, o.z, O[2]);
-      O[3] = fmaf(f, o.w, O[3]);
+#pragma unroll
+      for (int k = 0; k < kRows; k++) {
+        const int x = x0 + k * NT, r = x / (HD / 4), d = 4 * (x % (HD / 4));
+        if (x < n) extend_store<T>(a, it, r0 + r, d, O[k], m_s[r], l_s[r], vec);
+      }
     }
-    extend_store<T>(a, it, r, d, O, M, L, vec);
+    named_sync(id, NT);   // ws is used again
   }
 }
 
