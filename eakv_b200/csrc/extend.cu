@@ -32,6 +32,9 @@ constexpr int kMmaRows = 32;
 constexpr int kLeastPages = 6, kLeastTiles = 4;
 constexpr int kOverheadPages = 6, kOverheadTiles = 5;
 
+// Parts of an item, at most: a merge keeps two words of each in shared memory.
+constexpr int kMaxParts = 4096;
+
 // One launch's caches and plan: a call's caches with few rows and those with
 // many go to different kernels.
 struct Part {
@@ -71,32 +74,28 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
     if (!mine(i)) continue;
     const int n = t.first[i + 1] - t.first[i];
     const int k = p.n_caches++;
-    p.b.base[k] = t.base[i];
-    p.b.old[k] = t.pos[i];
-    p.b.first[k] = t.first[i];
-    p.b.n_new[k] = n;
-    p.b.tile0[k] = (int)tiles;
+    p.b.c[k] = {t.base[i], t.pos[i], t.first[i], n, (int)tiles};
     tiles += ((long long)n * a.G + p.tile_rows - 1) / p.tile_rows;
     if (tiles * heads > (1ll << 30)) {
       set_error(EAKV_ERR_INVALID, "extend_attention: more than 2^30 tiles of rows");
       return EAKV_ERR_INVALID;
     }
   }
-  for (int i = p.n_caches; i <= kMaxBatch; i++) p.b.tile0[i] = (int)tiles;
+  for (int i = p.n_caches; i <= kMaxBatch; i++) p.b.c[i] = {nullptr, 0, 0, 0, (int)tiles};
   p.tiles = p.launch_tiles = (int)tiles;
   if (p.tiles == 0) return EAKV_OK;
   // units of a tile's items, and of all
   auto units_of = [&](int k, int tile) {
-    const int row0 = (tile - p.b.tile0[k]) * p.tile_rows, all = p.b.n_new[k] * a.G;
+    const int row0 = (tile - p.b.c[k].tile0) * p.tile_rows, all = p.b.c[k].n_new * a.G;
     const int rows = all - row0 < p.tile_rows ? all - row0 : p.tile_rows;
-    const ExtRange r = extend_range(row0, rows, a.G, p.b.old[k], p.b.n_new[k], a.window, tree);
+    const ExtRange r = extend_range(row0, rows, a.G, p.b.c[k].old, p.b.c[k].n_new, a.window, tree);
     return (r.pages + p.unit_pages - 1) / p.unit_pages;
   };
   const int overhead = umma ? kOverheadTiles : kOverheadPages;
   long long units = 0;   // with the items' overheads
   int max_units = 1;
   for (int k = 0; k < p.n_caches; k++)
-    for (int i = p.b.tile0[k]; i < p.b.tile0[k + 1]; i++) {
+    for (int i = p.b.c[k].tile0; i < p.b.c[k + 1].tile0; i++) {
       const int u = units_of(k, i);
       units += (long long)(u + overhead) * heads;
       if (u > max_units) max_units = u;
@@ -126,7 +125,7 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
     long long at = 0;   // units before the tile
     int r = 0;
     for (int k = 0; k < p.n_caches; k++)
-      for (int i = p.b.tile0[k]; i < p.b.tile0[k + 1]; i++) {
+      for (int i = p.b.c[k].tile0; i < p.b.c[k + 1].tile0; i++) {
         const long long u = (long long)(units_of(k, i) + overhead) * heads;
         for (; r < p.n_runs && (long long)r * p.run < at + u; r++)
           p.runs.start[r] = make_int2(i, (int)((long long)r * p.run - at));
@@ -137,6 +136,7 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
   }
   int ns = t_force_splits > 0 ? t_force_splits : even ? (int)fit : (max_units + cap - 1) / cap;
   if (ns > max_units) ns = max_units;
+  if (ns > kMaxParts) ns = kMaxParts;
   p.split_units = (max_units + ns - 1) / ns;
   p.n_splits = (max_units + p.split_units - 1) / p.split_units;
   if (p.n_splits > 1) {

@@ -50,13 +50,18 @@ struct ExtendArgs {
   float *part_o, *part_m, *part_l;   // records [slot][row of the tile]...
 };
 
-// The caches of one launch, all with new tokens.
+// The caches of one launch, all with new tokens. (What one cache needs lies
+// together: a kernel's first look at each line of its arguments takes about as
+// long as a load from memory.)
+struct ExtendCache {
+  const uint8_t *base;
+  int old;      // position of the first new token
+  int first;    // its index in the packed rows
+  int n_new;
+  int tile0;    // first row tile, over one KV head
+};
 struct ExtendBatch {
-  const uint8_t *base[kMaxBatch];
-  int old[kMaxBatch];        // position of the first new token
-  int first[kMaxBatch];      // its index in the packed rows
-  int n_new[kMaxBatch];
-  int tile0[kMaxBatch + 1];  // first row tile of each cache, over one KV head
+  ExtendCache c[kMaxBatch + 1];   // tile0 of the caches behind the last: all tiles
 };
 
 // Where the runs of a balanced launch start: row tile, and units behind the
@@ -84,6 +89,7 @@ __host__ __device__ inline ExtRange extend_range(int row0, int rows, int G, int 
 
 // A CTA's part of an item.
 struct ExtItem {
+  const uint8_t *base;   // the cache's slab
   int b, h;
   int row0, rows;  // rows of the tile, within the (cache, KV head)
   int old, tok0;   // position of the cache's first new token, its packed index
@@ -138,14 +144,16 @@ struct ExtWalk {
       int lo = 0, hi = a.n_caches - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (batch.tile0[mid] <= tile) lo = mid;
+        if (batch.c[mid].tile0 <= tile) lo = mid;
         else hi = mid - 1;
       }
       it.b = lo;
-      it.old = batch.old[lo];
-      it.tok0 = batch.first[lo];
-      it.n_new = batch.n_new[lo];
-      it.row0 = (tile - batch.tile0[lo]) * a.tile_rows;
+      const ExtendCache &c = batch.c[lo];
+      it.base = c.base;
+      it.old = c.old;
+      it.tok0 = c.first;
+      it.n_new = c.n_new;
+      it.row0 = (tile - c.tile0) * a.tile_rows;
       it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
       const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window, a.tree != nullptr);
       const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
@@ -326,64 +334,82 @@ __device__ __forceinline__ void extend_store(const ExtendArgs &a, const ExtItem 
   if (a.lse && d == 0) extend_lse(a, it, r, M, L);
 }
 
-// The last part of an item: rows merged over the parts, in their order, four
-// dims of kRows rows per thread at a time (their loads are what this waits for: with
-// one row at a time the merge of 3 parts of 256 rows took 27 us), by NT threads
-// that meet on named barrier `id`. `ws` is free shared memory of ws_floats, more
-// than an item has parts: the weights of a row's parts are worked out once into it.
+// ROWS times NT elements of four dims from x0 on (row of the chunk x / (HD/4)),
+// merged over the parts, PARTS parts' loads at a time.
+template <int HD, typename T, int NT, int ROWS, int PARTS>
+__device__ __forceinline__ void merge_rows(const ExtendArgs &a, const ExtItem &it, bool vec, int r0, int n,
+                                           const float *m_s, const float *l_s, const float *f_s) {
+  const int ns = it.n_parts;
+  for (int x0 = threadIdx.x; x0 < n; x0 += ROWS * NT) {
+    float O[ROWS][4];
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) O[k][0] = O[k][1] = O[k][2] = O[k][3] = 0.0f;
+#pragma unroll 1
+    for (int s0 = 0; s0 < ns; s0 += PARTS) {
+      float4 o[PARTS][ROWS];
+#pragma unroll
+      for (int s = 0; s < PARTS; s++) {   // the last part, the last element again behind the end
+        const float *po = a.part_o + part_row(a, part_slot(it, min(s0 + s, ns - 1)), r0) * HD;
+#pragma unroll
+        for (int k = 0; k < ROWS; k++)
+          o[s][k] = __ldcg(reinterpret_cast<const float4 *>(po + 4 * min(x0 + k * NT, n - 1)));
+      }
+#pragma unroll
+      for (int s = 0; s < PARTS; s++) {
+        if (s0 + s >= ns) break;
+#pragma unroll
+        for (int k = 0; k < ROWS; k++) {
+          const float f = f_s[min(x0 + k * NT, n - 1) / (HD / 4) * ns + s0 + s];
+          O[k][0] = fmaf(f, o[s][k].x, O[k][0]);
+          O[k][1] = fmaf(f, o[s][k].y, O[k][1]);
+          O[k][2] = fmaf(f, o[s][k].z, O[k][2]);
+          O[k][3] = fmaf(f, o[s][k].w, O[k][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) {
+      const int x = x0 + k * NT, r = x / (HD / 4), d = 4 * (x % (HD / 4));
+      if (x < n) extend_store<T>(a, it, r0 + r, d, O[k], m_s[r], l_s[r], vec);
+    }
+  }
+}
+
+// The last part of an item: rows merged over the parts, in their order, by NT
+// threads that meet on named barrier `id`. `ws` is free shared memory of ws_floats,
+// more than twice the parts of any item: the weights of a row's parts are worked out
+// once into it. What this takes is the loads' time, so that eight are on their way
+// per thread: of four rows, or of eight parts where the rows are few (with one row
+// and part at a time 3 parts of 256 rows took 27 us, 19 parts of 16 rows 9 us).
 template <int HD, typename T, int NT>
 __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem &it, bool vec, float *ws,
                                              int ws_floats, int id) {
-  constexpr int kRows = 4;
-  const int ns = it.n_parts, most = min(it.rows, ws_floats / (ns + 2));
+  const int ns = it.n_parts, most = min(it.rows, ws_floats / (2 * ns + 2));
   for (int r0 = 0; r0 < it.rows; r0 += most) {
     const int rows = min(most, it.rows - r0);
-    float *m_s = ws, *l_s = ws + rows, *f_s = ws + 2 * rows;   // [rows], [rows], [rows][ns]
+    float *m_s = ws, *l_s = ws + rows, *f_s = ws + 2 * rows, *p_s = f_s + rows * ns;   // [rows] twice, [rows][ns]
     for (int x = threadIdx.x; x < rows * ns; x += NT) {
       const int r = x / ns;
-      f_s[x] = __ldcg(a.part_m + part_row(a, part_slot(it, x - r * ns), r0 + r));
+      const size_t pr = part_row(a, part_slot(it, x - r * ns), r0 + r);
+      f_s[x] = __ldcg(a.part_m + pr);
+      p_s[x] = __ldcg(a.part_l + pr);
     }
     named_sync(id, NT);
     for (int r = threadIdx.x; r < rows; r += NT) {
       float M = -INFINITY, L = 0.0f;
       for (int s = 0; s < ns; s++) M = fmaxf(M, f_s[r * ns + s]);
-#pragma unroll 4
       for (int s = 0; s < ns; s++) {
         const float f = part_weight(f_s[r * ns + s], M);
         f_s[r * ns + s] = f;
-        L = fmaf(f, __ldcg(a.part_l + part_row(a, part_slot(it, s), r0 + r)), L);
+        L = fmaf(f, p_s[r * ns + s], L);
       }
       m_s[r] = M;
       l_s[r] = L;
     }
     named_sync(id, NT);
     const int n = rows * (HD / 4);
-    for (int x0 = threadIdx.x; x0 < n; x0 += kRows * NT) {
-      float O[kRows][4];
-#pragma unroll
-      for (int k = 0; k < kRows; k++) O[k][0] = O[k][1] = O[k][2] = O[k][3] = 0.0f;
-#pragma unroll 2
-      for (int s = 0; s < ns; s++) {
-        const float *po = a.part_o + part_row(a, part_slot(it, s), r0) * HD;
-        float4 o[kRows];
-#pragma unroll
-        for (int k = 0; k < kRows; k++)   // the last again behind the end
-          o[k] = __ldcg(reinterpret_cast<const float4 *>(po + 4 * min(x0 + k * NT, n - 1)));
-#pragma unroll
-        for (int k = 0; k < kRows; k++) {
-          const float f = f_s[min(x0 + k * NT, n - 1) / (HD / 4) * ns + s];
-          O[k][0] = fmaf(f, o[k].x, O[k][0]);
-          O[k][1] = fmaf(f, o[k].y, O[k][1]);
-          O[k][2] = fmaf(f, o[k].z, O[k][2]);
-          O[k][3] = fmaf(f, o[k].w, O[k][3]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kRows; k++) {
-        const int x = x0 + k * NT, r = x / (HD / 4), d = 4 * (x % (HD / 4));
-        if (x < n) extend_store<T>(a, it, r0 + r, d, O[k], m_s[r], l_s[r], vec);
-      }
-    }
+    if (n <= NT) merge_rows<HD, T, NT, 1, 8>(a, it, vec, r0, n, m_s, l_s, f_s);
+    else merge_rows<HD, T, NT, 4, 2>(a, it, vec, r0, n, m_s, l_s, f_s);
     named_sync(id, NT);   // ws is used again
   }
 }

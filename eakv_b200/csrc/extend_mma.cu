@@ -59,7 +59,9 @@ struct XCfg {
   // operations per two pairs less than centring, and the sums run within
   // 64 sum |q| of zero, 2^-18 of it lost (one-limb types)
   static constexpr bool KRAW = LIMBS == 1;
-  static constexpr int FRAGOFF = STATOFF + R * (1 + NG) * 4;    // [step][limb][lane]
+  static constexpr int STARTOFF = STATOFF + R * (1 + NG) * 4;   // [R][NG][warp] starts
+  static constexpr int FRAGOFF = STARTOFF + R * NG * NW * 4;    // [step][limb][lane]
+  static_assert(NW == 4, "a warp per step of a group");
   static constexpr int FRAGS = LIMBS * 4 * NG * 32 * 16;
   static constexpr int SMEM = FRAGOFF + FRAGS;
   static_assert(MAIN % 16 == 0 && FRAGOFF % 16 == 0, "alignment");
@@ -132,6 +134,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::MAIN);
   float *q_s = reinterpret_cast<float *>(smem + C::QOFF);
   float *stat_s = reinterpret_cast<float *>(smem + C::STATOFF);
+  float *start_s = reinterpret_cast<float *>(smem + C::STARTOFF);
   uint4 *frag_s = reinterpret_cast<uint4 *>(smem + C::FRAGOFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -153,7 +156,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       if (threadIdx.x == 0 && it.state < 0) abandon_walk(walk, a, batch, part);
       return;
     }
-    const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
+    const uint8_t *kpages = it.base + page_index(a.geom, a.layer, 0, it.h, 0) * C::PB;
     const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
     auto issue = [&](int i) {
       if (i == a.test_stall - 1) return;   // test hook: this stage's wait runs out
@@ -183,23 +186,42 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       *reinterpret_cast<float4 *>(q_s + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
     }
     __syncthreads();
-    for (int r = warp; r < R; r += C::NW) {
-      float mx = 0.0f;
-      bool bad = false;
+    // a warp's rows together, step by step
+    {
+      constexpr int RW = R / C::NW;
+      float mx[RW], sm[RW][NG];
+      bool bad[RW];
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++) {
-        const float v0 = q_s[r * HD + 64 * gg + lane], v1 = q_s[r * HD + 64 * gg + 32 + lane];
-        mx = fmaxf(mx, fmaxf(fabsf(v0), fabsf(v1)));
-        bad = bad || v0 != v0 || v1 != v1;
-        float sm = v0 + v1;
+      for (int i = 0; i < RW; i++) {
+        const float *p = q_s + (warp + C::NW * i) * HD + lane;
+        mx[i] = 0.0f;
+        bad[i] = false;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sm += __shfl_xor_sync(0xffffffffu, sm, o);
-        if (lane == 0) stat_s[R + r * NG + gg] = sm;
+        for (int gg = 0; gg < NG; gg++) {
+          const float v0 = p[64 * gg], v1 = p[64 * gg + 32];
+          mx[i] = fmaxf(mx[i], fmaxf(fabsf(v0), fabsf(v1)));
+          bad[i] = bad[i] || v0 != v0 || v1 != v1;
+          sm[i][gg] = v0 + v1;
+        }
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      bad = __any_sync(0xffffffffu, bad);
-      if (lane == 0) stat_s[r] = bad ? INFINITY : mx;
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < RW; i++) {
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+#pragma unroll
+          for (int gg = 0; gg < NG; gg++) sm[i][gg] += __shfl_xor_sync(0xffffffffu, sm[i][gg], o);
+        }
+#pragma unroll
+      for (int i = 0; i < RW; i++) {
+        const bool any = __any_sync(0xffffffffu, bad[i]);
+        const int r = warp + C::NW * i;
+        if (lane == 0) {
+          stat_s[r] = any ? INFINITY : mx[i];
+#pragma unroll
+          for (int gg = 0; gg < NG; gg++) stat_s[R + r * NG + gg] = sm[i][gg];
+        }
+      }
     }
     __syncthreads();
     // rows g + 8 r of this lane
@@ -230,9 +252,11 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) kstart[r][gg] = 0.0f;
+      // each warp one step of every group
 #pragma unroll
-      for (int s = 0; s < NG * 4; s++) {
-        const int d = 64 * (s >> 2) + 8 * c + 4 * ((s >> 1) & 1) + (s & 1);
+      for (int gg = 0; gg < NG; gg++) {
+        const int s = 4 * gg + warp;
+        const int d = 64 * gg + 8 * c + 4 * ((s >> 1) & 1) + (s & 1);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // k & 1: row, k >> 1: high nibbles
@@ -244,15 +268,13 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           hi[k] = pack_f16(x0, x1);
           if (C::KRAW) {
             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
-            kstart[r][s >> 2] -= 1024.0f * (h.x + h.y);
+            kstart[r][gg] -= 1024.0f * (h.x + h.y);
           }
           lo[k] = LIMBS == 2 ? pack_rest(x0, x1, hi[k]) : 0u;
         }
-        if (s % C::NW == warp) {
-          uint4 *f = frag_s + s * LIMBS * 32 + lane;
-          f[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (LIMBS == 2) f[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
+        uint4 *f = frag_s + s * LIMBS * 32 + lane;
+        f[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (LIMBS == 2) f[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     if (C::KRAW) {
@@ -262,9 +284,19 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         for (int gg = 0; gg < NG; gg++) {
           kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 1);
           kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 2);
+          if (c == 0) start_s[((g + 8 * r) * NG + gg) * C::NW + warp] = kstart[r][gg];
         }
     }
     __syncthreads();
+    if (C::KRAW) {
+#pragma unroll
+      for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++) {
+          const float4 k4 = *reinterpret_cast<const float4 *>(start_s + ((g + 8 * r) * NG + gg) * C::NW);
+          kstart[r][gg] = (k4.x + k4.y) + (k4.z + k4.w);
+        }
+    }
 
     float o[NG][8][4];
 #pragma unroll

@@ -381,7 +381,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
     for (int part = 0;; part++) {
       const ExtItem &it = walk.item[part & 1];
       if (!begin_part(it)) break;
-      const uint8_t *kpages = batch.base[it.b] + page_index(a.geom, a.layer, 0, it.h, it.pg0) * C::PB +
+      const uint8_t *kpages = it.base + page_index(a.geom, a.layer, 0, it.h, it.pg0) * C::PB +
                               (size_t)(crow / kPagePositions) * C::PB;
       const uint8_t *vpages = kpages + (size_t)a.geom.n_heads * a.geom.n_pages * C::PB;
       RawRow<HD> kr, vr;
