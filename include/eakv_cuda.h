@@ -305,8 +305,9 @@ int eakv_cache_read(const eakv_cache_t *const *caches, int n_caches, int layer0,
 /* ---- testing aid ------------------------------------------------------ */
 
 /* Forces every later fused / decode call on this host thread to cut each
- * row into n sequence splits (0 restores the automatic choice), so tests
- * can exercise the split + combine path on small caches. */
+ * row (eakv_extend_attention: each tile of rows) into n sequence splits (0
+ * restores the automatic choice), so tests can exercise the split + combine
+ * path on small caches. */
 int eakv_test_force_splits(int n);
 
 /* The decode planner's split count, for tests of the planner without a GPU
@@ -321,7 +322,9 @@ int eakv_test_choose_splits(long long items, int max_pages, int lo, int hi, int 
  * and side-by-side measurements: 1 the CUDA-core kernel even for shapes the
  * tensor-core kernels serve, 2 the mma.sync tensor-core kernel (the automatic
  * choice), 3 the tcgen05 tensor-core kernel (head_dim 128; other shapes keep
- * the automatic choice); 0 restores the automatic choice. */
+ * the automatic choice); 0 restores the automatic choice. For
+ * eakv_extend_attention on 16-bit types 2 takes the mma.sync kernel and 3 the
+ * tcgen05 kernel whatever the number of rows is. */
 int eakv_test_force_path(int path);
 
 /* on != 0 makes later decode calls on this host thread merge their sequence
@@ -332,8 +335,10 @@ int eakv_test_separate_merge(int on);
 
 /* Failure-detection test: later fused / decode calls on this host thread
  * never request page `page` of each (row, split) work item into the
- * pipeline (page < 0 restores normal operation), and every wait of those
- * kernels gives up after `wait_budget` polls (0: the default budget). The
+ * pipeline (page < 0 restores normal operation; eakv_extend_attention's
+ * tcgen05 kernel never announces the scores of tile `page` instead), and
+ * every wait of those kernels gives up after `wait_budget` polls (0: the
+ * default budget). The
  * wait for the missing page then runs out: the kernel sets bit 1 of the
  * device status word (eakv_device_status), waits for the copies it did
  * request, and returns without writing its outputs. Nothing faults; the
