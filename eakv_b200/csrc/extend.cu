@@ -15,18 +15,25 @@ namespace {
 constexpr int kSplitItems = 16384;
 constexpr size_t kCounterBytes = kSplitItems * sizeof(unsigned);
 
-// Longest split in pages. The tensor core adds into its f32 sums by
+// Longest part of an item in pages. The tensor core adds into its f32 sums by
 // truncation, a drift of up to 2^-24 of the sum per step of 16 positions. In
 // the warp-level kernel four warps take pages in turn: 64 pages are 64 steps of a
-// warp (2^-18 at worst, 2^-19 on average, below what f32 results ask for), and 256
-// pages 2^-16, below 16-bit results' own rounding; in the tcgen05 kernel one
-// sum takes every step, and 1024 pages are 2^-12, 2^-13 on average, against the
-// 2^-9 of its outputs.
-constexpr int kSplitPagesF32 = 64, kSplitPages16 = 256, kSplitPagesUmma = 1024;
+// warp (2^-18 at worst, 2^-19 on average, below what f32 results ask for), and
+// 1024 pages 2^-14; in the tcgen05 kernel one sum takes every step, and 1024 pages
+// are 2^-12, 2^-13 on average: both below the 2^-9 or 2^-12 of 16-bit outputs. (With 256
+// pages for the warp-level kernel 16 caches of up to 32768 positions were kept from
+// equal runs by tiles of 8 rows: 303 us, in runs 231.)
+constexpr int kPartPagesF32 = 64, kPartPages16 = 1024;
 
 // Rows (new tokens x query heads per KV head) up to which 16-bit calls take the
 // warp-level kernel.
 constexpr int kMmaRows = 32;
+// A page's time for tiles of 8, 16 and 24 rows of the warp-level kernel, 16-bit
+// types: 16 caches of 8192 positions (8 KV heads of 128) took 55, 78 and 98 us with
+// one tile each, 15 us of it set-up. A second tile of 8 rows costs as much again (84
+// us), so 16 rows go to one tile, 17 to 24 to one of 24. In f32 the two limbs double
+// the operands and larger tiles lose: 104 rows per head (13, 7, 5 tiles) 73, 78, 86 us.
+constexpr int kTileCost[3] = {10, 16, 21};
 // Shortest parts worth a CTA, and what an item costs beyond its positions (set-up,
 // results), in pages of the warp-level kernel and tiles of the tcgen05 kernel.
 constexpr int kLeastPages = 6, kLeastTiles = 4;
@@ -57,7 +64,7 @@ int sm_count(int dev) {
 // bytes. Call with the caches' device current.
 int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool umma, Part &p) {
   p.umma = umma;
-  p.tile_rows = umma ? kExtendUmmaRows : kExtendMmaRows;
+  p.tile_rows = kExtendUmmaRows;
   auto mine = [&](int i) {
     const long long rows = (long long)(t.first[i + 1] - t.first[i]) * a.G;
     const bool many = a.dtype != EAKV_F32 && t_force_path != 2 && (rows > kMmaRows || t_force_path == 3);
@@ -69,6 +76,24 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
   p.n_splits = p.split_units = 1;
   p.unit_pages = umma ? 2 : 1;   // the tcgen05 kernel's tiles are two pages
   const int heads = a.geom.n_heads;
+  // the tile size that takes least; 8 rows in f32, and where the parts are as
+  // short as they get even so (2 tokens of 32 + 4 heads of 64 behind 2046
+  // positions: 14.8 us, with tiles of 16 rows 18)
+  long long best = 0;
+  for (int size = 8; size <= (a.dtype == EAKV_F32 ? 8 : 24) && !umma; size += 8) {
+    long long cost = 0;
+    for (int i = 0; i < a.n_caches; i++) {
+      if (!mine(i)) continue;
+      const int n = t.first[i + 1] - t.first[i];
+      const ExtRange r = extend_range(0, n * a.G, a.G, t.pos[i], n, a.window, tree);
+      cost += ((long long)n * a.G + size - 1) / size * (r.pages + kOverheadPages) * kTileCost[size / 8 - 1];
+    }
+    if (size == 8 || cost < best) {
+      best = cost;
+      p.tile_rows = size;
+    }
+    if (size == 8 && cost * heads <= 3ll * sm_count(device) * (kLeastPages + kOverheadPages) * kTileCost[0]) break;
+  }
   long long tiles = 0;
   for (int i = 0; i < a.n_caches; i++) {
     if (!mine(i)) continue;
@@ -100,9 +125,9 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
       units += (long long)(u + overhead) * heads;
       if (u > max_units) max_units = u;
     }
-  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype);
+  const int per_sm = umma ? 1 : extend_mma_resident(a.geom.gpd * 64, a.dtype, p.tile_rows);
   if (per_sm <= 0) return EAKV_ERR_INVALID;   // recorded by the lookup
-  const int cap = umma ? kSplitPagesUmma / 2 : a.dtype == EAKV_F32 ? kSplitPagesF32 : kSplitPages16;
+  const int cap = (a.dtype == EAKV_F32 ? kPartPagesF32 : kPartPages16) / p.unit_pages;
   const int least = umma ? kLeastTiles : kLeastPages;
   const long long resident = (long long)per_sm * sm_count(device), items = tiles * heads;
   long long run = (units + resident - 1) / resident;

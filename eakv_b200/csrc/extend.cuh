@@ -387,7 +387,8 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
   const int ns = it.n_parts, most = min(it.rows, ws_floats / (2 * ns + 2));
   for (int r0 = 0; r0 < it.rows; r0 += most) {
     const int rows = min(most, it.rows - r0);
-    float *m_s = ws, *l_s = ws + rows, *f_s = ws + 2 * rows, *p_s = f_s + rows * ns;   // [rows] twice, [rows][ns]
+    float *m_s = ws, *l_s = ws + rows;                          // [rows]
+    float *f_s = ws + 2 * rows, *p_s = f_s + rows * ns;         // [rows][ns]
     for (int x = threadIdx.x; x < rows * ns; x += NT) {
       const int r = x / ns;
       const size_t pr = part_row(a, part_slot(it, x - r * ns), r0 + r);
@@ -414,9 +415,8 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
   }
 }
 
-// extend_mma.cu
-constexpr int kExtendMmaRows = 16;
-int extend_mma_resident(int head_dim, int dtype);
+// extend_mma.cu: tiles of 8, 16 or 24 rows
+int extend_mma_resident(int head_dim, int dtype, int tile_rows);
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                       bool vec, cudaStream_t s);
 // extend_umma.cu: 16-bit types

@@ -1,6 +1,6 @@
 // extend_mma.cu - attention of a few new tokens per cache over the Q4 pages,
 // on the warp-level tensor-core instructions (mma.sync, f16 operands, f32
-// sums): tiles of 16 (token, query head) rows of one KV head.
+// sums): tiles of 8, 16 or 24 (token, query head) rows of one KV head.
 //
 // Mathematics. With a group's centred nibbles n' = n - 8 and b' = b + 8 s,
 //   q.k = sum_g s_g (q_g . n'_g) + b'_g sum(q_g)
@@ -16,19 +16,21 @@
 // for f32. Sums of scores, softmax and outputs are f32; the maximum moves
 // lazily, when a score passes it by more than 8 (base 2), so p <= 256.
 //
-// Tiles. Rows are the m16 of both products, so a page is converted once for
-// 16 rows: scores S[16 rows][8 positions] take K as B operand straight from
-// its bytes (a 32-bit word holds dims d..d+3 and d+32..d+35; the pairs that
-// one mask selects are (d, d+2) and (d+32, d+34), and the dims of a k-step are
-// taken in that order on both sides), the score fragments are, pair by pair,
-// the A fragments of the output product, and V comes as B operand from one
-// transposed ldmatrix per group and 16 positions. Each warp takes whole pages
-// in turn; the page ring, its waits and the split merge are those of the
-// decode kernels.
+// Tiles. Both products are transposed, rows the n8 of the instructions: scores
+// S^T[16 positions][8 rows] take K as A operand straight from its bytes (a 32-bit
+// word holds dims d..d+3 and d+32..d+35; the pairs that one mask selects are (d,
+// d+2) and (d+32, d+34), and the dims of a k-step are taken in that order on both
+// sides), O^T[16 dims][8 rows] takes V as A operand from one transposed ldmatrix
+// per group and 16 positions, and the weights as B operand by one transposition of
+// 8 x 8 pairs (movmatrix). So a page is converted once for a tile, and a tile of few
+// rows costs few products: with rows as the m16 one token of four heads behind each
+// of 16 x 8192 positions took 71 us, transposed 55. Each warp takes whole pages in
+// turn; the page ring, its waits and the split merge are those of the decode kernels.
 //
-// Bound: HBM for up to 16 rows (about 21 instructions per KV position of a
-// KV head), instruction issue from there on: every further tile of 16 rows
-// repeats the conversion.
+// Bound: the chain of a step's dependent instructions (two to four warps per
+// scheduler, as the registers allow), and the set-up and merge of an item, about 15
+// us. 16 caches of 8192 positions (168 MB, 26 us at HBM's rate): 55 us for 8 rows,
+// 78 for 16, 98 for 24.
 #include <math.h>
 
 #include <atomic>
@@ -39,32 +41,39 @@
 namespace eakv {
 namespace {
 
-template <int HD, int LIMBS>
+// NT: tiles of eight rows per CTA.
+template <int HD, int LIMBS, int NT>
 struct XCfg {
-  static constexpr int R = kExtendMmaRows;
+  static constexpr int R = 8 * NT, PAIRS = (NT + 1) / 2, QR = 16 * PAIRS;   // rows, and as q's operands lie
   static constexpr int NG = HD / 64;
   static constexpr int NW = 4;
   static constexpr int THREADS = NW * 32;
-  static constexpr int MINB = 3;                                // CTAs per SM
+  static constexpr int MINB = NT == 3 ? 2 : NT == 1 && HD == 64 ? 4 : 3;   // CTAs per SM
+  // Positions of a lane per step (g + 8 j). A step's time is its chain of dependent
+  // instructions: two of 16 positions side by side where the registers are there.
+  static constexpr int J = NT == 1 ? 4 : 2;
   static constexpr int NIB = kPagePositions * NG * 32;
   static constexpr int PB = kPagePositions * NG * 40;
   static constexpr int NSTAGE = HD == 128 ? 5 : 8;              // pages in flight
   static constexpr int STAGE_BYTES = 2 * PB;
   static constexpr int RING = NSTAGE * STAGE_BYTES;
-  static constexpr int MERGE = NW * R * (HD + 2) * 4;
+  static constexpr int OS = HD + 8;                             // floats from row to row of the warps' sums
+  static constexpr int MERGE = NW * R * (OS + 2) * 4;
   static constexpr int MAIN = RING > MERGE ? RING : MERGE;
-  static constexpr int QOFF = MAIN + 2 * NSTAGE * 8;            // q rows [R][HD] f32
-  static constexpr int STATOFF = QOFF + R * HD * 4;             // [R] max|q|, [R][NG] sums
+  static constexpr int QOFF = MAIN + 2 * NSTAGE * 8;            // q rows [QR][HD] f32
+  // [QR] powers of two, [QR] score factors, [NG][QR] sums
+  static constexpr int STATOFF = QOFF + QR * HD * 4;
   // K enters as 16 (64 + n), the offset taken off by the sums' start: four
   // operations per two pairs less than centring, and the sums run within
   // 64 sum |q| of zero, 2^-18 of it lost (one-limb types)
   static constexpr bool KRAW = LIMBS == 1;
-  static constexpr int STARTOFF = STATOFF + R * (1 + NG) * 4;   // [R][NG][warp] starts
-  static constexpr int FRAGOFF = STARTOFF + R * NG * NW * 4;    // [step][limb][lane]
+  static constexpr int STARTOFF = STATOFF + QR * (2 + NG) * 4;  // [NG][QR][warp] starts
+  static constexpr int MASKOFF = STARTOFF + QR * NG * NW * 4;   // RowMask [R]
+  static constexpr int FRAGOFF = MASKOFF + QR * 32;             // [pair][step][limb][lane]
   static_assert(NW == 4, "a warp per step of a group");
-  static constexpr int FRAGS = LIMBS * 4 * NG * 32 * 16;
+  static constexpr int FRAGS = PAIRS * LIMBS * 4 * NG * 32 * 16;
   static constexpr int SMEM = FRAGOFF + FRAGS;
-  static_assert(MAIN % 16 == 0 && FRAGOFF % 16 == 0, "alignment");
+  static_assert(MAIN % 16 == 0 && FRAGOFF % 16 == 0 && sizeof(RowMask) <= 32, "alignment");
 };
 
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
@@ -100,7 +109,7 @@ __device__ __forceinline__ uint32_t pack_rest(float x0, float x1, uint32_t hi) {
   return pack_f16(x0 - b.x, x1 - b.y);
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float *d, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
@@ -114,6 +123,13 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr));
 }
 
+// The 8 x 8 matrix of f16 pairs that the warp's words hold, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
 // Out of line: between two parts, with few registers to keep over the call.
 __device__ __noinline__ void step_walk(ExtWalk &walk, const ExtendArgs &a, const ExtendBatch &batch, int p) {
   walk.next(a, batch, p);
@@ -122,18 +138,19 @@ __device__ __noinline__ void abandon_walk(ExtWalk &walk, const ExtendArgs &a, co
   walk.abandon(a, batch, p);
 }
 
-template <int HD, int LIMBS, typename T>
-__global__ void __launch_bounds__(XCfg<HD, LIMBS>::THREADS, XCfg<HD, LIMBS>::MINB)
+template <int HD, int LIMBS, int NT, typename T>
+__global__ void __launch_bounds__(XCfg<HD, LIMBS, NT>::THREADS, XCfg<HD, LIMBS, NT>::MINB)
 extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ ExtendBatch batch,
                   const __grid_constant__ ExtendRuns runs, const int vec) {
-  using C = XCfg<HD, LIMBS>;
-  constexpr int NG = C::NG, R = C::R, NR = 2;   // NR: rows of a lane, g + 8 r
+  using C = XCfg<HD, LIMBS, NT>;
+  constexpr int NG = C::NG, R = C::R, QR = C::QR, J = C::J;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last_part;
   __shared__ ExtWalk walk;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::MAIN);
   float *q_s = reinterpret_cast<float *>(smem + C::QOFF);
-  float *stat_s = reinterpret_cast<float *>(smem + C::STATOFF);
+  float *up_s = reinterpret_cast<float *>(smem + C::STATOFF), *fac_s = up_s + QR, *sum_s = fac_s + QR;
+  RowMask *mask_s = reinterpret_cast<RowMask *>(smem + C::MASKOFF);
   float *start_s = reinterpret_cast<float *>(smem + C::STARTOFF);
   uint4 *frag_s = reinterpret_cast<uint4 *>(smem + C::FRAGOFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -168,27 +185,37 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       bulk_g2s(dst + C::PB, vpages + (size_t)(it.pg0 + i) * C::PB, C::PB, full);
       publish_requested(&last_req[st], done + i);
     };
-    if (threadIdx.x == 0)
-      for (int i = 0; i < it.npages && i < C::NSTAGE; i++) issue(i);
-
     // ---- the tile's q rows: f32 in shared memory, row maxima and group sums ------
-    for (int x = threadIdx.x; x < R * (HD / 4); x += C::THREADS) {
-      const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (r < it.rows) {
-        const int row = it.row0 + r;
-        const T *p = reinterpret_cast<const T *>(a.q.data) +
-                     (long long)(it.tok0 + row / a.G) * a.q.token_stride +
-                     (long long)(it.h * a.G + row % a.G) * a.q.head_stride + d;
-        if (vec) load4<T, true>(p, v);
-        else load4<T, false>(p, v);
-      }
-      *reinterpret_cast<float4 *>(q_s + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+    // (all loads, then the first pages' requests, then the stores)
+    if (threadIdx.x < R) mask_s[threadIdx.x] = row_mask(a, it, it.row0 + threadIdx.x);
+    {
+      constexpr int LOADS = QR * (HD / 4) / C::THREADS, STEP = C::THREADS / (HD / 4);
+      const int r0 = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+      float v[LOADS][4];
+      auto load = [&](auto vec_tag) {
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) {
+          const int row = it.row0 + r0 + STEP * k, tok = row / a.G;
+          v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+          if (r0 + STEP * k < it.rows)
+            load4<T, decltype(vec_tag)::value>(
+                reinterpret_cast<const T *>(a.q.data) + (long long)(it.tok0 + tok) * a.q.token_stride +
+                    (long long)(it.h * a.G + row - tok * a.G) * a.q.head_stride + d, v[k]);
+        }
+      };
+      if (vec) load(std::true_type{});
+      else load(std::false_type{});
+      if (threadIdx.x == 0)
+        for (int i = 0; i < it.npages && i < C::NSTAGE; i++) issue(i);
+#pragma unroll
+      for (int k = 0; k < LOADS; k++)
+        *reinterpret_cast<float4 *>(q_s + (r0 + STEP * k) * HD + d) =
+            make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
     }
     __syncthreads();
     // a warp's rows together, step by step
     {
-      constexpr int RW = R / C::NW;
+      constexpr int RW = QR / C::NW;
       float mx[RW], sm[RW][NG];
       bool bad[RW];
 #pragma unroll
@@ -214,301 +241,318 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         }
 #pragma unroll
       for (int i = 0; i < RW; i++) {
-        const bool any = __any_sync(0xffffffffu, bad[i]);
+        const bool fine = !__any_sync(0xffffffffu, bad[i]) && mx[i] <= 3.0e38f;
         const int r = warp + C::NW * i;
+        int e = 0;
+        frexpf(mx[i] > 0.0f && fine ? mx[i] : 1.0f, &e);          // in [2^(e-1), 2^e)
+        const int qe = max(min(5 - e, 126), -126);
         if (lane == 0) {
-          stat_s[r] = any ? INFINITY : mx[i];
+          const float up = fine ? __uint_as_float((uint32_t)(127 + qe) << 23) : 0.0f;
+          up_s[r] = up;
+          // a row with an infinity or NaN in q has NaN scores
+          fac_s[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - qe) << 23)
+                          : __uint_as_float(0x7fc00000u);
 #pragma unroll
-          for (int gg = 0; gg < NG; gg++) stat_s[R + r * NG + gg] = sm[i][gg];
+          for (int gg = 0; gg < NG; gg++) sum_s[gg * QR + r] = fine ? sm[i][gg] * up : 0.0f;
         }
       }
     }
     __syncthreads();
-    // rows g + 8 r of this lane
-    float rowfac[NR], qsum[NR][NG], kstart[NR][NG];
-    RowMask mask[NR];
-    {
-      float up[NR];
+    // q's operands: for k-step s = (word j, byte parity par) of group gg the dims
+    // d = 64 gg + 8c + 4j + par and d + 2 (low nibbles), d + 32 and d + 34 (high
+    // nibbles, held times 16) of rows g, g + 8 of a pair of tiles; each warp one step
+    // of every group
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
-        const float hmax = stat_s[g + 8 * r];
-        const bool fine = hmax <= 3.0e38f;
-        int e = 0;
-        frexpf(hmax > 0.0f && fine ? hmax : 1.0f, &e);          // hmax in [2^(e-1), 2^e)
-        const int qe = max(min(5 - e, 126), -126);
-        up[r] = fine ? __uint_as_float((uint32_t)(127 + qe) << 23) : 0.0f;
-        // a row with an infinity or NaN in q has NaN scores
-        rowfac[r] = fine ? a.scale_log2 * __uint_as_float((uint32_t)(127 - qe) << 23)
-                         : __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int gg = 0; gg < NG; gg++)
-          qsum[r][gg] = fine ? stat_s[R + (g + 8 * r) * NG + gg] * up[r] : 0.0f;
-        mask[r] = row_mask(a, it, it.row0 + g + 8 * r);
-      }
-      // A fragments of k-step s = (word j, byte parity par) of group gg: dims
-      // d = 64 gg + 8c + 4j + par and d + 2 (low nibbles), d + 32 and d + 34 (high
-      // nibbles, held times 16)
-#pragma unroll
-      for (int r = 0; r < NR; r++)
-#pragma unroll
-        for (int gg = 0; gg < NG; gg++) kstart[r][gg] = 0.0f;
-      // each warp one step of every group
+    for (int pr = 0; pr < C::PAIRS; pr++) {
+      const float up[2] = {up_s[16 * pr + g], up_s[16 * pr + g + 8]};
 #pragma unroll
       for (int gg = 0; gg < NG; gg++) {
         const int s = 4 * gg + warp;
         const int d = 64 * gg + 8 * c + 4 * ((s >> 1) & 1) + (s & 1);
         uint32_t hi[4], lo[4];
+        float start[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // k & 1: row, k >> 1: high nibbles
           const int r = k & 1;
-          const float *p = q_s + (g + 8 * r) * HD + d + 32 * (k >> 1);
+          const float *p = q_s + (16 * pr + g + 8 * r) * HD + d + 32 * (k >> 1);
           const float f = up[r] * (C::KRAW || (k >> 1) ? 0.0625f : 1.0f);
           const float x0 = up[r] == 0.0f ? 0.0f : p[0] * f;   // inf * 0
           const float x1 = up[r] == 0.0f ? 0.0f : p[2] * f;
           hi[k] = pack_f16(x0, x1);
           if (C::KRAW) {
             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
-            kstart[r][gg] -= 1024.0f * (h.x + h.y);
+            start[r] -= 1024.0f * (h.x + h.y);
           }
           lo[k] = LIMBS == 2 ? pack_rest(x0, x1, hi[k]) : 0u;
         }
-        uint4 *f = frag_s + s * LIMBS * 32 + lane;
-        f[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (LIMBS == 2) f[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        uint4 *f = frag_s + (pr * 4 * NG + s) * LIMBS * 32 + lane;
+        f[0] = make_uint4(hi[0], hi[2], hi[1], hi[3]);
+        if (LIMBS == 2) f[32] = make_uint4(lo[0], lo[2], lo[1], lo[3]);
+        if (C::KRAW) {
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            start[r] += __shfl_xor_sync(0xffffffffu, start[r], 1);
+            start[r] += __shfl_xor_sync(0xffffffffu, start[r], 2);
+            if (c == 0) start_s[(gg * QR + 16 * pr + g + 8 * r) * C::NW + warp] = start[r];
+          }
+        }
       }
     }
-    if (C::KRAW) {
-#pragma unroll
-      for (int r = 0; r < NR; r++)
-#pragma unroll
-        for (int gg = 0; gg < NG; gg++) {
-          kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 1);
-          kstart[r][gg] += __shfl_xor_sync(0xffffffffu, kstart[r][gg], 2);
-          if (c == 0) start_s[((g + 8 * r) * NG + gg) * C::NW + warp] = kstart[r][gg];
-        }
-    }
     __syncthreads();
-    if (C::KRAW) {
+    // rows 8 n + 2 c + e of this lane
+    float rowfac[NT][2], qsum[NT][2][NG], kstart[NT][2][NG];
 #pragma unroll
-      for (int r = 0; r < NR; r++)
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int r = 8 * n + 2 * c + e;
+        rowfac[n][e] = fac_s[r];
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(start_s + ((g + 8 * r) * NG + gg) * C::NW);
-          kstart[r][gg] = (k4.x + k4.y) + (k4.z + k4.w);
+          qsum[n][e][gg] = sum_s[gg * QR + r];
+          const float4 k4 = *reinterpret_cast<const float4 *>(start_s + (gg * QR + r) * C::NW);
+          kstart[n][e][gg] = (k4.x + k4.y) + (k4.z + k4.w);
         }
-    }
+      }
 
-    float o[NG][8][4];
+    // O transposed: [group][dims 16w + 2g + parity, low and high nibbles][row tile]
+    float o[NG][4][NT][4];
 #pragma unroll
     for (int gg = 0; gg < NG; gg++)
 #pragma unroll
-      for (int n = 0; n < 8; n++)
+      for (int m = 0; m < 4; m++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[gg][n][k] = 0.0f;
-    float m_run[NR], m_eff[NR], l_run[NR], pb[NR][NG];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[gg][m][n][k] = 0.0f;
+    float m_run[NT][2], m_eff[NT][2], l_run[NT][2], pb[NT][2][NG];
     // Everything a row sums is divided by a power of two near the largest V scale
     // the row has attended (eref: its biased exponent, -6 before the first), by
     // way of the exponential's argument (m_eff); it moves like the maximum, when a
     // scale passes it by 2^6, so that p s stays below 2^8 2^7.
-    int eref[NR];
+    int eref[NT][2];
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-      m_run[r] = -INFINITY;
-      m_eff[r] = l_run[r] = 0.0f;
-      eref[r] = -6;
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++) pb[r][gg] = 0.0f;
-    }
+      for (int e = 0; e < 2; e++) {
+        m_run[n][e] = -INFINITY;
+        m_eff[n][e] = l_run[n][e] = 0.0f;
+        eref[n][e] = -6;
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++) pb[n][e][gg] = 0.0f;
+      }
+
+    // (scale, b + 8 scale when centred) of the lane's positions p0 + g + 8 j
+    auto scales = [&](const uint8_t *sb, int p0, bool centred, float (&s)[J][NG], float (&b)[J][NG]) {
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const int tp = p0 + g + 8 * j;
+        if constexpr (NG == 2) {
+          const float4 v4 = *reinterpret_cast<const float4 *>(sb + tp * 16);
+          s[j][0] = v4.x; b[j][0] = v4.y; s[j][NG - 1] = v4.z; b[j][NG - 1] = v4.w;
+        } else {
+          const float2 v2 = *reinterpret_cast<const float2 *>(sb + tp * 8);
+          s[j][0] = v2.x; b[j][0] = v2.y;
+        }
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++)
+          if (centred) b[j][gg] = fmaf(8.0f, s[j][gg], b[j][gg]);
+      }
+    };
 
     // page_ex: largest exponent of a V scale of the page (full pages)
     auto step = [&](auto full_tag, const uint8_t *ks, int page_pos0, int p0, int page_ex) {
       constexpr bool FULL = decltype(full_tag)::value;
       const uint8_t *vsm = ks + C::PB;
-      bool on[NR][4];
-      float sk[4][NG], bk[4][NG];
+      bool on[NT][2][J];   // [row tile][row][position]
+      if (!FULL) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
-        if (!FULL) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int r = 0; r < NR; r++) on[r][j] = mask[r].attends(page_pos0 + tp);
-        }
-        if constexpr (NG == 2) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(ks + C::NIB + tp * 16);
-          sk[j][0] = k4.x; bk[j][0] = k4.y; sk[j][1] = k4.z; bk[j][1] = k4.w;
-        } else {
-          const float2 k2 = *reinterpret_cast<const float2 *>(ks + C::NIB + tp * 8);
-          sk[j][0] = k2.x; bk[j][0] = k2.y;
-        }
+          for (int e = 0; e < 2; e++) {
+            const RowMask m = mask_s[8 * n + 2 * c + e];
 #pragma unroll
-        for (int gg = 0; gg < NG && !C::KRAW; gg++) bk[j][gg] = fmaf(8.0f, sk[j][gg], bk[j][gg]);
+            for (int j = 0; j < J; j++) on[n][e][j] = m.attends(page_pos0 + p0 + g + 8 * j);
+          }
       }
-      // ---- scores --------------------------------------------------------------
-      float sc[NR][4];
+      // ---- scores, transposed: [position g + 8 j][row 2 c + e] ------------------
+      float sc[NT][2][J];
       {
-        float dk[2][NG][4];
+        float sk[J][NG], bk[J][NG], dk[NT][NG][2 * J];   // dk: of 16 positions after the other
+        scales(ks + C::NIB, p0, !C::KRAW, sk, bk);
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) {
-          uint2 wv[2];
+          uint2 wv[J];
 #pragma unroll
-          for (int tile = 0; tile < 2; tile++) {
-            wv[tile] = *reinterpret_cast<const uint2 *>(ks + (p0 + 8 * tile + g) * (HD / 2) + 8 * c + 32 * gg);
+          for (int j = 0; j < J; j++)
+            wv[j] = *reinterpret_cast<const uint2 *>(ks + (p0 + 8 * j + g) * (HD / 2) + 8 * c + 32 * gg);
 #pragma unroll
-            for (int k = 0; k < 4; k++) dk[tile][gg][k] = C::KRAW ? kstart[k >> 1][gg] : 0.0f;
-          }
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int k = 0; k < 2 * J; k++) dk[n][gg][k] = C::KRAW ? kstart[n][k & 1][gg] : 0.0f;
 #pragma unroll
           for (int s = 0; s < 4; s++) {
-            uint32_t b0[2], b1[2];
+            uint32_t af[J / 2][4];
 #pragma unroll
-            for (int tile = 0; tile < 2; tile++) {
-              const uint32_t w = (s >> 1) ? wv[tile].y : wv[tile].x;
+            for (int j = 0; j < J; j++) {
+              const uint32_t w = (s >> 1) ? wv[j].y : wv[j].x;
               const uint32_t y = (s & 1) ? w >> 8 : w;
-              b0[tile] = C::KRAW ? raw_hi((s & 1) ? w >> 4 : w << 4) : nib_lo(y);
-              b1[tile] = C::KRAW ? raw_hi(y) : nib_hi(y);
+              af[j >> 1][j & 1] = C::KRAW ? raw_hi((s & 1) ? w >> 4 : w << 4) : nib_lo(y);
+              af[j >> 1][2 + (j & 1)] = C::KRAW ? raw_hi(y) : nib_hi(y);
             }
 #pragma unroll
-            for (int l = 0; l < LIMBS; l++) {
-              const uint4 f = frag_s[((4 * gg + s) * LIMBS + l) * 32 + lane];
-              const uint32_t af[4] = {f.x, f.y, f.z, f.w};
+            for (int pr = 0; pr < C::PAIRS; pr++)
 #pragma unroll
-              for (int tile = 0; tile < 2; tile++) mma(dk[tile][gg], af, b0[tile], b1[tile]);
-            }
+              for (int l = 0; l < LIMBS; l++) {
+                const uint4 f = frag_s[((pr * 4 * NG + 4 * gg + s) * LIMBS + l) * 32 + lane];
+#pragma unroll
+                for (int u = 0; u < J / 2; u++) {
+                  mma(dk[2 * pr][gg] + 4 * u, af[u], f.x, f.y);
+                  if (2 * pr + 1 < NT) mma(dk[2 * pr + 1 < NT ? 2 * pr + 1 : 0][gg] + 4 * u, af[u], f.z, f.w);
+                }
+              }
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int r = 0; r < NR; r++) {
-            float u = 0.0f;
+          for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int gg = 0; gg < NG; gg++) {
-              u = fmaf(dk[j >> 1][gg][2 * r + (j & 1)], sk[j][gg], u);
-              u = fmaf(qsum[r][gg], bk[j][gg], u);
+            for (int j = 0; j < J; j++) {
+              float u = 0.0f;
+#pragma unroll
+              for (int gg = 0; gg < NG; gg++) {
+                u = fmaf(dk[n][gg][2 * j + e], sk[j][gg], u);
+                u = fmaf(qsum[n][e][gg], bk[j][gg], u);
+              }
+              u *= rowfac[n][e];
+              sc[n][e][j] = (FULL || on[n][e][j]) ? u : -INFINITY;
             }
-            u *= rowfac[r];
-            sc[r][j] = (FULL || on[r][j]) ? u : -INFINITY;
-          }
       }
-      float sv[4][NG], bv[4][NG];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int tp = p0 + 2 * c + (j & 1) + (j >> 1) * 8;
-        if constexpr (NG == 2) {
-          const float4 v4 = *reinterpret_cast<const float4 *>(vsm + C::NIB + tp * 16);
-          sv[j][0] = v4.x; bv[j][0] = v4.y; sv[j][1] = v4.z; bv[j][1] = v4.w;
-        } else {
-          const float2 v2 = *reinterpret_cast<const float2 *>(vsm + C::NIB + tp * 8);
-          sv[j][0] = v2.x; bv[j][0] = v2.y;
-        }
-#pragma unroll
-        for (int gg = 0; gg < NG; gg++) bv[j][gg] = fmaf(8.0f, sv[j][gg], bv[j][gg]);
-      }
+      float sv[J][NG], bv[J][NG];
+      scales(vsm + C::NIB, p0, true, sv, bv);
       // ---- online softmax, base 2, lazy maximum -----------------------------------
       // A row moves when a score passes its maximum by 8, or a V scale that it
       // attends passes its reference by 2^6 (scales are negative only in damaged
       // files; NaN is passed over).
       bool move = false;
-      float lm[NR];
-      int ex[NR];
+      float lm[NT][2];
+      int ex[NT][2];
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
-        lm[r] = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
-        if (FULL) {
-          ex[r] = page_ex;
-        } else {
-          float sx = 0.0f;
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            float s = fabsf(sv[j][0]);
-            if (NG == 2) s = fmaxf(s, fabsf(sv[j][NG - 1]));
-            if (on[r][j]) sx = fmaxf(sx, s);
+        for (int e = 0; e < 2; e++) {
+          lm[n][e] = sc[n][e][0];
+#pragma unroll
+          for (int j = 1; j < J; j++) lm[n][e] = fmaxf(lm[n][e], sc[n][e][j]);
+          if (FULL) {
+            ex[n][e] = page_ex;
+          } else {
+            float sx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+              float s = fabsf(sv[j][0]);
+              if (NG == 2) s = fmaxf(s, fabsf(sv[j][NG - 1]));
+              if (on[n][e][j]) sx = fmaxf(sx, s);
+            }
+            ex[n][e] = (int)(__float_as_uint(sx) >> 23);
           }
-          ex[r] = (int)(__float_as_uint(sx) >> 23);
+          move = move || lm[n][e] > m_run[n][e] + 8.0f || ex[n][e] > eref[n][e] + 6;
         }
-        move = move || lm[r] > m_run[r] + 8.0f || ex[r] > eref[r] + 6;
-      }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-          float t = lm[r];
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-          int x = ex[r];
-          if (!FULL && x >= 253) {   // without the infinite ones
-            x = 0;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+          for (int e = 0; e < 2; e++) {
+            float t = lm[n][e];
+            int x = ex[n][e];
+            if (!FULL && x >= 253) {   // without the infinite ones
+              x = 0;
+#pragma unroll
+              for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int gg = 0; gg < NG; gg++) {
+                  const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
+                  if (on[n][e][j] && e1 < 255) x = max(x, min(e1, 252));
+                }
+            }
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) {
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
+              if (!FULL) x = max(x, __shfl_xor_sync(0xffffffffu, x, b));
+            }
+            const bool mv = t > m_run[n][e] + 8.0f, me = x > eref[n][e] + 6;
+            if (mv || me) {
+              float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
+              if (mv) m_run[n][e] = t;
+              // before the first reference all sums are zero, or NaN
+              if (me && eref[n][e] > 0) alpha *= __uint_as_float((uint32_t)max(127 + eref[n][e] - x, 0) << 23);
+              if (me) eref[n][e] = x;
+              m_eff[n][e] = (m_run[n][e] == -INFINITY ? 0.0f : m_run[n][e]) +
+                            (eref[n][e] > 0 ? (float)(eref[n][e] - 127) : 0.0f);
+              l_run[n][e] *= alpha;
 #pragma unroll
               for (int gg = 0; gg < NG; gg++) {
-                const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
-                if (on[r][j] && e1 < 255) x = max(x, min(e1, 252));
-              }
-          }
-          x = max(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = max(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          const bool mv = t > m_run[r] + 8.0f, me = x > eref[r] + 6;
-          if (mv || me) {
-            float alpha = mv ? ex2(m_run[r] - t) : 1.0f;
-            if (mv) m_run[r] = t;
-            // before the first reference all sums are zero, or NaN
-            if (me && eref[r] > 0) alpha *= __uint_as_float((uint32_t)max(127 + eref[r] - x, 0) << 23);
-            if (me) eref[r] = x;
-            m_eff[r] = (m_run[r] == -INFINITY ? 0.0f : m_run[r]) +
-                       (eref[r] > 0 ? (float)(eref[r] - 127) : 0.0f);
-            l_run[r] *= alpha;
+                pb[n][e][gg] *= alpha;
 #pragma unroll
-            for (int gg = 0; gg < NG; gg++) {
-              pb[r][gg] *= alpha;
-#pragma unroll
-              for (int n = 0; n < 8; n++) {
-                o[gg][n][2 * r] *= alpha;
-                o[gg][n][2 * r + 1] *= alpha;
+                for (int m = 0; m < 4; m++) {
+                  o[gg][m][n][e] *= alpha;
+                  o[gg][m][n][2 + e] *= alpha;
+                }
               }
             }
           }
-        }
       }
 #pragma unroll
-      for (int r = 0; r < NR; r++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          sc[r][j] = ex2(sc[r][j] - m_eff[r]);   // the weights from here on
-          l_run[r] += sc[r][j];
-        }
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int j = 0; j < J; j++) {
+            sc[n][e][j] = ex2(sc[n][e][j] - m_eff[n][e]);   // the weights from here on
+            l_run[n][e] += sc[n][e][j];
+          }
       // ---- outputs -------------------------------------------------------------
 #pragma unroll
       for (int gg = 0; gg < NG; gg++) {
-        uint32_t ah[4], al[4];
+        uint32_t bh[NT][J], bl[NT][J];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {   // k & 1: row, k >> 1: positions 2c+8, 2c+9
-          const int r = k & 1;
-          float x[2];
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int j = 2 * (k >> 1) + e;
-            // what is not attended adds nothing, whatever its scale and bias are
-            x[e] = (FULL || on[r][j]) ? sc[r][j] * sv[j][gg] : 0.0f;
-            if (FULL || on[r][j]) pb[r][gg] = fmaf(sc[r][j], bv[j][gg], pb[r][gg]);
+          for (int j = 0; j < J; j++) {
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              // what is not attended adds nothing, whatever its scale and bias are
+              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * sv[j][gg] : 0.0f;
+              if (FULL || on[n][e][j]) pb[n][e][gg] = fmaf(sc[n][e][j], bv[j][gg], pb[n][e][gg]);
+            }
+            const uint32_t h = pack_f16(x[0], x[1]);
+            bh[n][j] = transpose8(h);
+            bl[n][j] = LIMBS == 2 ? transpose8(pack_rest(x[0], x[1], h)) : 0u;
           }
-          ah[k] = pack_f16(x[0], x[1]);
-          al[k] = LIMBS == 2 ? pack_rest(x[0], x[1], ah[k]) : 0u;
-        }
         // V bytes: lane (g, c) receives bytes 16w + 2g, + 1 of positions 2c, 2c+1
         // (x[2w]) and 2c+8, 2c+9 (x[2w+1])
-        uint32_t x[4];
-        {
-          const int t = lane >> 3, r = lane & 7;
-          ldsm_x4_trans(x, smem_u32(vsm + (p0 + 8 * (t & 1) + r) * (HD / 2) + 32 * gg + 16 * (t >> 1)));
-        }
 #pragma unroll
-        for (int n = 0; n < 8; n++) {   // n = 4w + 2 parity + (high nibbles)
-          const int w = n >> 2, par = (n >> 1) & 1;
-          const uint32_t y0 = par ? x[2 * w] >> 8 : x[2 * w];
-          const uint32_t y1 = par ? x[2 * w + 1] >> 8 : x[2 * w + 1];
-          const uint32_t b0 = (n & 1) ? nib_hi(y0) : nib_lo(y0);
-          const uint32_t b1 = (n & 1) ? nib_hi(y1) : nib_lo(y1);
-          mma(o[gg][n], ah, b0, b1);
-          if constexpr (LIMBS == 2) mma(o[gg][n], al, b0, b1);
+        for (int u = 0; u < J / 2; u++) {
+          uint32_t x[4];
+          {
+            const int t = lane >> 3, r = lane & 7;
+            const int at = p0 + 16 * u + 8 * (t & 1) + r;
+            ldsm_x4_trans(x, smem_u32(vsm + at * (HD / 2) + 32 * gg + 16 * (t >> 1)));
+          }
+#pragma unroll
+          for (int m = 0; m < 4; m++) {   // m = 2w + parity
+            const int w = m >> 1;
+            const uint32_t y0 = (m & 1) ? x[2 * w] >> 8 : x[2 * w];
+            const uint32_t y1 = (m & 1) ? x[2 * w + 1] >> 8 : x[2 * w + 1];
+            const uint32_t af[4] = {nib_lo(y0), nib_hi(y0), nib_lo(y1), nib_hi(y1)};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              mma(o[gg][m][n], af, bh[n][2 * u], bh[n][2 * u + 1]);
+              if constexpr (LIMBS == 2) mma(o[gg][m][n], af, bl[n][2 * u], bl[n][2 * u + 1]);
+            }
+          }
         }
       }
     };
@@ -536,10 +580,10 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         }
         ex = __reduce_max_sync(0xffffffffu, ex);
 #pragma unroll 1
-        for (int s = 0; s < kPagePositions / 16; s++) step(std::true_type{}, ks, page_pos0, 16 * s, ex);
+        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::true_type{}, ks, page_pos0, p0, ex);
       } else {
 #pragma unroll 1
-        for (int s = 0; s < kPagePositions / 16; s++) step(std::false_type{}, ks, page_pos0, 16 * s, 0);
+        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::false_type{}, ks, page_pos0, p0, 0);
       }
       __syncwarp();
       if (lane == 0 && stage_release_last(reinterpret_cast<int *>(&bars[C::NSTAGE]) + st, 1) &&
@@ -562,35 +606,35 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
     __syncthreads();
     float *mw = reinterpret_cast<float *>(smem);   // [NW][R]
     float *lw = mw + C::NW * R;
-    float *ow = lw + C::NW * R;                    // [NW][R][HD]
+    float *ow = lw + C::NW * R;                    // [NW][R][OS]
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int gg = 0; gg < NG; gg++) {
-        pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 1);
-        pb[r][gg] += __shfl_xor_sync(0xffffffffu, pb[r][gg], 2);
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) {
+          l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], b);
+#pragma unroll
+          for (int gg = 0; gg < NG; gg++) pb[n][e][gg] += __shfl_xor_sync(0xffffffffu, pb[n][e][gg], b);
+        }
+        const int row = warp * R + 8 * n + 2 * c + e;
+        const float vs = eref[n][e] > 0 ? __uint_as_float((uint32_t)eref[n][e] << 23) : 1.0f;
+        if (g == 0) {
+          mw[row] = m_run[n][e];
+          lw[row] = l_run[n][e] * vs;
+        }
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++)
+#pragma unroll
+          for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int hi = 0; hi < 2; hi++) {
+              const float f = hi ? vs * 0.0625f : vs, b = pb[n][e][gg] * vs;
+              *reinterpret_cast<float2 *>(ow + row * C::OS + 64 * gg + 32 * hi + 16 * w + 2 * g) =
+                  make_float2(fmaf(o[gg][2 * w][n][2 * hi + e], f, b),
+                              fmaf(o[gg][2 * w + 1][n][2 * hi + e], f, b));
+            }
       }
-      const int row = warp * R + g + 8 * r;
-      const float vs = eref[r] > 0 ? __uint_as_float((uint32_t)eref[r] << 23) : 1.0f;
-      if (c == 0) {
-        mw[row] = m_run[r];
-        lw[row] = l_run[r] * vs;
-      }
-#pragma unroll
-      for (int gg = 0; gg < NG; gg++)
-#pragma unroll
-        for (int w = 0; w < 2; w++)
-#pragma unroll
-          for (int hi = 0; hi < 2; hi++) {
-            const float f = hi ? vs * 0.0625f : vs, b = pb[r][gg] * vs;
-            const float (&e0)[4] = o[gg][4 * w + hi], (&e1)[4] = o[gg][4 * w + 2 + hi];
-            const int k = 2 * r;
-            *reinterpret_cast<float4 *>(ow + row * HD + 64 * gg + 32 * hi + 16 * w + 4 * c) =
-                make_float4(fmaf(e0[k], f, b), fmaf(e1[k], f, b), fmaf(e0[k + 1], f, b), fmaf(e1[k + 1], f, b));
-          }
-    }
     __syncthreads();
     for (int x = threadIdx.x; x < it.rows * (HD / 4); x += C::THREADS) {
       const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
@@ -601,7 +645,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
       for (int w = 0; w < C::NW; w++) {
         const float f = part_weight(mw[w * R + r], M);
-        const float4 v = *reinterpret_cast<const float4 *>(ow + (w * R + r) * HD + d);
+        const float4 v = *reinterpret_cast<const float4 *>(ow + (w * R + r) * C::OS + d);
         L = fmaf(f, lw[w * R + r], L);
         O[0] = fmaf(f, v.x, O[0]);
         O[1] = fmaf(f, v.y, O[1]);
@@ -629,15 +673,15 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
   }
 }
 
-template <int HD, int LIMBS, typename T>
+template <int HD, int LIMBS, int NT, typename T>
 int resident_one() {
-  using C = XCfg<HD, LIMBS>;
+  using C = XCfg<HD, LIMBS, NT>;
   static std::atomic<int> cached[64];
   int dev = 0;
   cudaGetDevice(&dev);
   const int hit = cached[dev & 63].load(std::memory_order_relaxed);
   if (hit) return hit;
-  auto fn = extend_mma_kernel<HD, LIMBS, T>;
+  auto fn = extend_mma_kernel<HD, LIMBS, NT, T>;
   if (check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                  "extend: smem attribute"))
     return 0;
@@ -648,25 +692,31 @@ int resident_one() {
   return per_sm;
 }
 
-template <int HD, int LIMBS, typename T>
+template <int HD, int LIMBS, int NT, typename T>
 int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks, bool vec,
                cudaStream_t s) {
-  using C = XCfg<HD, LIMBS>;
-  extend_mma_kernel<HD, LIMBS, T><<<n_blocks, C::THREADS, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
+  using C = XCfg<HD, LIMBS, NT>;
+  extend_mma_kernel<HD, LIMBS, NT, T><<<n_blocks, C::THREADS, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
   return check_cuda(cudaGetLastError(), "extend_mma launch");
 }
 
 // f(launch or resident functions of the instance that serves the arguments)
+template <int HD, typename T, typename F>
+int pick_rows(int rows, F f) {
+  if (rows == 8) return f.template operator()<HD, 1, 1, T>();
+  if (rows == 16) return f.template operator()<HD, 1, 2, T>();
+  return f.template operator()<HD, 1, 3, T>();
+}
 template <int HD, typename F>
-int pick(int dtype, F f) {
-  if (dtype == EAKV_F32) return f.template operator()<HD, 2, float>();
-  if (dtype == EAKV_F16) return f.template operator()<HD, 1, __half>();
-  return f.template operator()<HD, 1, __nv_bfloat16>();
+int pick(int dtype, int rows, F f) {
+  if (dtype == EAKV_F32) return f.template operator()<HD, 2, 1, float>();
+  if (dtype == EAKV_F16) return pick_rows<HD, __half>(rows, f);
+  return pick_rows<HD, __nv_bfloat16>(rows, f);
 }
 
 struct Resident {
-  template <int HD, int LIMBS, typename T> int operator()() const {
-    return resident_one<HD, LIMBS, T>();
+  template <int HD, int LIMBS, int NT, typename T> int operator()() const {
+    return resident_one<HD, LIMBS, NT, T>();
   }
 };
 struct Launch {
@@ -676,8 +726,8 @@ struct Launch {
   int n_blocks;
   bool vec;
   cudaStream_t s;
-  template <int HD, int LIMBS, typename T> int operator()() const {
-    return launch_one<HD, LIMBS, T>(a, b, runs, n_blocks, vec, s);
+  template <int HD, int LIMBS, int NT, typename T> int operator()() const {
+    return launch_one<HD, LIMBS, NT, T>(a, b, runs, n_blocks, vec, s);
   }
 };
 
@@ -685,14 +735,14 @@ struct Launch {
 
 // CTAs per SM of the kernel for this shape on the current device (0: error).
 // Sets the kernel's shared-memory limit, so it comes before the launch.
-int extend_mma_resident(int head_dim, int dtype) {
-  return head_dim == 128 ? pick<128>(dtype, Resident{}) : pick<64>(dtype, Resident{});
+int extend_mma_resident(int head_dim, int dtype, int tile_rows) {
+  return head_dim == 128 ? pick<128>(dtype, tile_rows, Resident{}) : pick<64>(dtype, tile_rows, Resident{});
 }
 
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                       bool vec, cudaStream_t s) {
   const Launch f{a, b, runs, n_blocks, vec, s};
-  return a.geom.gpd == 2 ? pick<128>(a.dtype, f) : pick<64>(a.dtype, f);
+  return a.geom.gpd == 2 ? pick<128>(a.dtype, a.tile_rows, f) : pick<64>(a.dtype, a.tile_rows, f);
 }
 
 }  // namespace eakv
