@@ -14,6 +14,8 @@ entry points.
 """
 import ctypes
 import os
+import struct
+from array import array
 
 import numpy as np
 
@@ -415,6 +417,21 @@ class _Rows(ctypes.Structure):
     _fields_ = [("data", _P), ("token_stride", _c.c_int64), ("head_stride", _c.c_int64), ("dtype", _I)]
 
 
+# The same as bytes, and C arrays as array.array: a call's arguments take half the
+# time of ctypes objects (append_rotary of 16 caches 16 -> 12 us).
+_pack_rows = struct.Struct("@Qqqi4x").pack
+_pack_rotary = struct.Struct("@QQiiiQqiiiii4x").pack
+
+
+def _address(values):
+    """Address of an array.array, which has to outlive the call."""
+    return values.buffer_info()[0]
+
+
+def _handle_array(caches):
+    return array("Q", [c.h or 0 for c in caches])
+
+
 class _Rotary(ctypes.Structure):
     """eakv_rotary_t"""
     _fields_ = [("cos_table", _P), ("sin_table", _P), ("n_rows", _I), ("rot_dim", _I),
@@ -432,10 +449,16 @@ def _name(x):
     return name
 
 
+_codes = {}   # torch dtype -> EAKV_*
+
+
 def _dtype(x):
-    code = _DTYPES.get(_name(x))
+    code = _codes.get(x.dtype)
     if code is None:
-        raise TypeError(f"float32, float16 or bfloat16 expected, got {x.dtype}")
+        code = _DTYPES.get(_name(x))
+        if code is None:
+            raise TypeError(f"float32, float16 or bfloat16 expected, got {x.dtype}")
+        _codes[x.dtype] = code
     return code
 
 
@@ -447,26 +470,24 @@ def _on(x, cache, what):
 
 
 def _rows(x, cache, heads, tokens, what):
-    """eakv_rows_t of a tensor [tokens, heads, head_dim] whose last dim is contiguous."""
+    """eakv_rows_t (its bytes) of a tensor [tokens, heads, head_dim] whose last dim is contiguous."""
     if x is None:
         return None
-    if x.shape != (tokens, heads, cache.shape[2]):
-        raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(tokens, heads, cache.shape[2])}")
+    _, _, head_dim, device = cache.shape
+    if x.shape != (tokens, heads, head_dim):
+        raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(tokens, heads, head_dim)}")
     t, h, d = x.stride()
     if d != 1:
         raise ValueError(f"{what}: the last dim must be contiguous")
-    _on(x, cache, what)
-    return _Rows(x.data_ptr(), t, h, _dtype(x))
-
-
-def _ref(x):
-    return None if x is None else ctypes.byref(x)
+    if x.get_device() != device:
+        _on(x, cache, what)   # refuses
+    return _pack_rows(x.data_ptr(), t, h, _dtype(x))
 
 
 def _ints(values, n, what):
     if len(values) != n:
         raise ValueError(f"{what}: {len(values)} entries for {n} caches")
-    return (_I * n)(*values)
+    return array("i", values)
 
 
 def _contiguous(x, cache, dtype, shape, what):
@@ -509,31 +530,30 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
             positions = positions[None]
         if cos.dim() != 2 or cos.dtype != sin.dtype:
             raise ValueError("cos, sin: f32 tables [rows, rot_dim/2] expected")
-        shape = cos.shape
+        n_rows, pairs = shape = cos.shape
         _contiguous(cos, c, "float32", shape, "cos")
         _contiguous(sin, c, "float32", shape, "sin")
-        axes = positions.shape[0]
-        if (_name(positions) != "int32" or positions.dim() != 2 or axes > 4 or
-                positions.shape[1] != total or (total > 1 and positions.stride(1) != 1)):
+        axes, n = positions.shape if positions.dim() == 2 else (0, 0)
+        if _name(positions) != "int32" or not 1 <= axes <= 4 or n != total or (total > 1 and positions.stride(1) != 1):
             raise ValueError(f"positions: int32 [1..4, {total}] expected")
         _on(positions, c, "positions")
-        sections = list(sections) if sections is not None else [shape[1]]
+        sections = list(sections) if sections is not None else [pairs]
         if len(sections) != axes:
             raise ValueError(f"{len(sections)} sections for {axes} axes")
-        rot = _Rotary(_ptr(cos), _ptr(sin), shape[0], 2 * shape[1], int(interleaved), _ptr(positions),
-                      positions.stride(0) if axes > 1 else 0, axes, (_I * 4)(*sections))
-    return _check(lib().eakv_append_rotary(_handles(caches), len(caches), layer,
-                                           _ints(counts, len(caches), "counts"), _ref(rk), _ref(rv),
-                                           _ref(rq), _ref(ro), nq, _ref(rot), stream),
-                  "eakv_append_rotary")
+        rot = _pack_rotary(cos.data_ptr(), sin.data_ptr(), n_rows, 2 * pairs, 1 if interleaved else 0,
+                           positions.data_ptr(), positions.stride(0) if axes > 1 else 0, axes, *sections,
+                           *(0,) * (4 - axes))
+    hs, n_new = _handle_array(caches), _ints(counts, len(caches), "counts")
+    return _check(lib().eakv_append_rotary(_address(hs), len(caches), layer, _address(n_new), rk, rv, rq, ro,
+                                           nq, rot, stream), "eakv_append_rotary")
 
 
 def extend_workspace(caches, counts, dtype, n_q_heads, window=0, tree=False):
     """Bytes of workspace eakv_extend_attention takes for this call; dtype is
     EAKV_F32, EAKV_F16 or EAKV_BF16."""
     out = ctypes.c_size_t()
-    _check(lib().eakv_extend_workspace(_handles(caches), len(caches),
-                                       _ints(counts, len(caches), "counts"), dtype, n_q_heads, window,
+    hs, n_new = _handle_array(caches), _ints(counts, len(caches), "counts")
+    _check(lib().eakv_extend_workspace(_address(hs), len(caches), _address(n_new), dtype, n_q_heads, window,
                                        int(bool(tree)), ctypes.byref(out)), "eakv_extend_workspace")
     return out.value
 
@@ -556,17 +576,17 @@ def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=Non
     if workspace is not None:
         size = workspace.numel()
         _contiguous(workspace, c, "uint8", (size,), "workspace")
-    return _check(lib().eakv_extend_attention(_handles(caches), len(caches), layer,
-                                              _ints(counts, len(caches), "counts"), _ref(rq), _ref(ro),
-                                              nq, scale, window, _ptr(tree), _ptr(lse),
-                                              _ptr(workspace), size, stream),
-                  "eakv_extend_attention")
+    hs, n_new = _handle_array(caches), _ints(counts, len(caches), "counts")
+    return _check(lib().eakv_extend_attention(_address(hs), len(caches), layer, _address(n_new), rq, ro, nq,
+                                              scale, window, _ptr(tree), _ptr(lse), _ptr(workspace), size,
+                                              stream), "eakv_extend_attention")
 
 
 def copy_positions(dsts, dst_pos, src, src_pos, n, stream=None):
     """eakv_cache_copy: positions [src_pos, src_pos + n) of src to dst_pos.. of
     every cache of dsts, whose seq_len becomes dst_pos + n."""
-    return _check(lib().eakv_cache_copy(_handles(dsts), len(dsts), dst_pos, src.h, src_pos, n, stream),
+    hs = _handle_array(dsts)
+    return _check(lib().eakv_cache_copy(_address(hs), len(dsts), dst_pos, src.h, src_pos, n, stream),
                   "eakv_cache_copy")
 
 
@@ -594,11 +614,12 @@ def read_positions(caches, begins, counts, out, layer=0, stream=None):
     if last != 1:
         raise ValueError("out: the last dim must be contiguous")
     _on(out, c, "out")
-    rk = _Rows(out.data_ptr(), tok, head, _dtype(out))
-    rv = _Rows(rk.data and rk.data + kv * out.element_size(), tok, head, rk.dtype)
-    return _check(lib().eakv_cache_read(_handles(caches), len(caches), layer, out.shape[0],
-                                        _ints(begins, len(caches), "begins"),
-                                        _ints(counts, len(caches), "counts"), _ref(rk), _ref(rv),
+    code, at = _dtype(out), out.data_ptr()
+    hs, begin = _handle_array(caches), _ints(begins, len(caches), "begins")
+    n = _ints(counts, len(caches), "counts")
+    return _check(lib().eakv_cache_read(_address(hs), len(caches), layer, out.shape[0], _address(begin),
+                                        _address(n), _pack_rows(at, tok, head, code),
+                                        _pack_rows(at and at + kv * out.element_size(), tok, head, code),
                                         layers, stream), "eakv_cache_read")
 
 
