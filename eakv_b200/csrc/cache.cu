@@ -39,39 +39,51 @@ int check_cuda(cudaError_t e, const char *what) {
   return code;
 }
 
-int cache_workspace(const eakv_cache *c, size_t n_counters, size_t bytes, unsigned **counters,
-                    void **data) {
-  const size_t have_data = c->d_scratch ? c->scratch_bytes - c->cnt_bytes : 0;
+// One grow-on-demand allocation [cnt bytes of counters at zero | data], `total`
+// bytes in all.
+static int grow_workspace(const eakv_cache *c, void *&buf, size_t &total, size_t &cnt, size_t n_counters,
+                          size_t bytes, unsigned **counters, void **data) {
+  const size_t have_data = buf ? total - cnt : 0;
   size_t cb = (n_counters * sizeof(unsigned) + 255) / 256 * 256;
-  if (!c->d_scratch || cb > c->cnt_bytes || bytes > have_data) {
+  if (!buf || cb > cnt || bytes > have_data) {
     // grow: neither region ever shrinks
-    if (cb < c->cnt_bytes) cb = c->cnt_bytes;
+    if (cb < cnt) cb = cnt;
     if (cb < 4096) cb = 4096;
     size_t db = bytes > have_data ? bytes : have_data;
     if (db < (1u << 20)) db = 1u << 20;
-    if (c->d_scratch) {
+    if (buf) {
       cudaStreamSynchronize(c->stream);
-      cudaFree(c->d_scratch);
-      c->d_scratch = nullptr;
-      c->scratch_bytes = c->cnt_bytes = 0;
+      cudaFree(buf);
+      buf = nullptr;
+      total = cnt = 0;
     }
     void *p = nullptr;
     int rc = check_cuda(cudaMalloc(&p, cb + db), "scratch allocation");
     if (rc) return rc;
-    // the counters start at zero; the decode kernels leave them at zero
+    // the counters start at zero; the kernels leave them at zero
     rc = check_cuda(cudaMemsetAsync(p, 0, cb, c->stream), "scratch counters");
     if (!rc) rc = check_cuda(cudaStreamSynchronize(c->stream), "scratch counters");
     if (rc) {
       cudaFree(p);
       return rc;
     }
-    c->d_scratch = p;
-    c->cnt_bytes = cb;
-    c->scratch_bytes = cb + db;
+    buf = p;
+    cnt = cb;
+    total = cb + db;
   }
-  if (counters) *counters = (unsigned *)c->d_scratch;
-  *data = (uint8_t *)c->d_scratch + c->cnt_bytes;
+  if (counters) *counters = (unsigned *)buf;
+  *data = (uint8_t *)buf + cnt;
   return EAKV_OK;
+}
+
+int cache_workspace(const eakv_cache *c, size_t n_counters, size_t bytes, unsigned **counters,
+                    void **data) {
+  return grow_workspace(c, c->d_scratch, c->scratch_bytes, c->cnt_bytes, n_counters, bytes, counters, data);
+}
+
+int cache_parts_workspace(const eakv_cache *c, size_t n_counters, size_t bytes, unsigned **counters,
+                          void **data) {
+  return grow_workspace(c, c->d_parts, c->parts_bytes, c->parts_cnt_bytes, n_counters, bytes, counters, data);
 }
 
 void *cache_scratch(const eakv_cache *c, size_t bytes) {
@@ -156,6 +168,7 @@ void eakv_cache_free(eakv_cache_t *c) {
   cudaStreamSynchronize(c->stream);
   if (c->d_buf) cudaFree(c->d_buf);
   if (c->d_scratch) cudaFree(c->d_scratch);
+  if (c->d_parts) cudaFree(c->d_parts);
   if (c->own_stream) cudaStreamDestroy(c->stream);
   free(c);
 }
@@ -317,7 +330,7 @@ int eakv_set_device(int device) {
 int eakv_cache_device(const eakv_cache_t *c) { return c ? c->device : -1; }
 // The page slab plus the cache's scratch (host staging, split workspace).
 size_t eakv_cache_device_bytes(const eakv_cache_t *c) {
-  return c ? c->buf_bytes + (c->d_scratch ? c->scratch_bytes : 0) : 0;
+  return c ? c->buf_bytes + (c->d_scratch ? c->scratch_bytes : 0) + (c->d_parts ? c->parts_bytes : 0) : 0;
 }
 void *eakv_cache_stream(const eakv_cache_t *c) { return c ? (void *)c->stream : nullptr; }
 

@@ -197,6 +197,8 @@ int check_call(const eakv_cache_t *const *caches, int n_caches, const int *n_new
   if (dtype < EAKV_F32 || dtype > EAKV_BF16) return refuse("unknown element type");
   if (window < 0) return refuse("negative window");
   if (caches[0]->n_kv_heads > kSplitItems) return refuse("more than 16384 KV heads");
+  if ((long long)total * (n_q / caches[0]->n_kv_heads) > (1ll << 30))
+    return refuse("more than 2^30 (token, query head) rows per KV head");
   for (int i = 0; i < n_caches && tree; i++)
     if (n_new[i] > 64) return refuse("a tree mask holds 64 new tokens per cache at most");
   memset(&a, 0, sizeof a);
@@ -284,7 +286,7 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
     if (rc) return rc;
     if (cap != cudaStreamCaptureStatusNone)
       return refuse("a captured call needs a workspace of its own (eakv_extend_workspace)");
-    rc = cache_workspace(c0, kSplitItems, need - kCounterBytes, &a.cnt, &data);
+    rc = cache_parts_workspace(c0, kSplitItems, need - kCounterBytes, &a.cnt, &data);
     if (rc) return rc;
   }
   const bool vec = rows_vec(q) && rows_vec(out);

@@ -85,6 +85,11 @@ struct eakv_cache {
   mutable void *d_scratch;
   mutable size_t scratch_bytes;
   mutable size_t cnt_bytes;
+  // the same for the records of eakv_extend_attention: of its own, so that its
+  // growth does not move what a captured decode works on
+  mutable void *d_parts;
+  mutable size_t parts_bytes;
+  mutable size_t parts_cnt_bytes;
 };
 
 namespace eakv {
@@ -116,6 +121,8 @@ void *cache_scratch(const eakv_cache *c, size_t bytes);
 // Both pointers come from one allocation, so one call gives both.
 int cache_workspace(const eakv_cache *c, size_t n_counters, size_t bytes, unsigned **counters,
                     void **data);
+int cache_parts_workspace(const eakv_cache *c, size_t n_counters, size_t bytes, unsigned **counters,
+                          void **data);
 
 // ---- quantize.cu ----
 // Quantizes n_units units of n_tok*head_dim floats each: the n_tok*gpd

@@ -50,7 +50,7 @@ int    eakv_set_device(int device);
 
 int    eakv_cache_device(const eakv_cache_t *cache);         /* -1 for NULL */
 /* HBM held by the cache: its page slab plus the scratch that host-buffer
- * calls and split decodes grow on demand. */
+ * calls, split decodes and eakv_extend_attention grow on demand. */
 size_t eakv_cache_device_bytes(const eakv_cache_t *cache);
 /* Stream used by this cache's calls; NULL restores the cache's own. */
 int    eakv_cache_set_stream(eakv_cache_t *cache, void *stream);
@@ -255,10 +255,11 @@ int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, con
  * that keep 22 bits, 16-bit types on 16-bit tensor-core operands with 32-bit
  * sums. workspace (device, 16-byte aligned) holds the records of long rows'
  * sequence splits: at least eakv_extend_workspace bytes, zeroed once before
- * its first use, and not shared by calls that may overlap; NULL takes the
- * first cache's scratch, which then must not be in use on another stream. A
- * captured call takes a workspace of its own, since the scratch moves when a
- * later call needs more of it. */
+ * its first use, and not shared by calls that may overlap; NULL takes one that
+ * the first cache keeps for this call, which then must not be in use on another
+ * stream. A captured call takes a workspace of its own, since the cache's moves
+ * when a later call needs more of it. (What the cache keeps for its decodes
+ * stays where it is.) */
 int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int layer,
                           const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
                           int n_q_heads, float scale, int window, const uint64_t *tree, float *lse,
@@ -271,7 +272,9 @@ int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const
  * [dst_pos, dst_pos + n) of n_dst other caches in one launch, as they are
  * (nibbles, scales and biases), and sets their seq_len to dst_pos + n:
  * dst_pos <= their seq_len, src_pos + n <= src's. The caches agree in layers,
- * heads and head_dim; their max_seq_len may differ. n_dst <= 256. */
+ * heads and head_dim; their max_seq_len may differ. n_dst <= 256. Here and in
+ * eakv_cache_gather a stream of NULL is src's; what runs on the destinations'
+ * own streams has to be ordered behind it by the caller. */
 int eakv_cache_copy(eakv_cache_t *const *dsts, int n_dst, int dst_pos, const eakv_cache_t *src,
                     int src_pos, int n, void *stream);
 /* A new cache of max_seq_len positions on src's device with src's first n. Not

@@ -233,6 +233,45 @@ def test_calls_side_by_side(gpu, dtype, path):
     assert E.device_status(0) == 0
 
 
+def test_captured_decode_outlives_extend_calls(gpu):
+    """A decode with splits, captured on the cache's own scratch; extend calls that grow
+    what the same cache keeps for them; the replay still gives the decode's bits."""
+    import torch
+    rng = np.random.default_rng(79)
+    b = Batch(rng, 1, 2, 128, [3000], [600])
+    c = b.caches[0]
+    s = torch.cuda.Stream()
+    q = torch.from_numpy(rng.standard_normal((1, 1, 8, 128)).astype(np.float32)).to(gpu)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    E.force_splits(5)
+    E.decode_attention([c], q, 8, out, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    want = out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        E.decode_attention([c], q, 8, out, stream=s.cuda_stream)
+    rows = torch.from_numpy(rng.standard_normal((600, 8, 128)).astype(np.float32)).to(gpu)
+    res = torch.empty_like(rows)
+    torch.cuda.synchronize()
+    held = lambda: E.lib().eakv_cache_device_bytes(c.h)  # noqa: E731
+    before = held()
+    for n, splits in ((1, 5), (600, 7), (600, 40)):
+        E.force_splits(splits)
+        E.extend_attention([c], 0, [n], rows[:n], res[:n])
+        c.synchronize()
+    assert held() > before
+    for _ in range(2):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    del g
+    b.free()
+    assert E.device_status(0) == 0
+
+
 def test_the_same_cache_twice_and_padded_rows(gpu):
     """extend_attention only reads the caches: one of them may be there twice, with
     different counts. Rows behind the last token stay as they are, and a call without
