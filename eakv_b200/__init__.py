@@ -534,7 +534,8 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
         _contiguous(cos, c, "float32", shape, "cos")
         _contiguous(sin, c, "float32", shape, "sin")
         axes, n = positions.shape if positions.dim() == 2 else (0, 0)
-        if _name(positions) != "int32" or not 1 <= axes <= 4 or n != total or (total > 1 and positions.stride(1) != 1):
+        if (_name(positions) != "int32" or not 1 <= axes <= 4 or n != total or
+                (total > 1 and positions.stride(1) != 1)):
             raise ValueError(f"positions: int32 [1..4, {total}] expected")
         _on(positions, c, "positions")
         sections = list(sections) if sections is not None else [pairs]

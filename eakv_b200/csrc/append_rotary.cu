@@ -23,9 +23,11 @@
 // per lane, sixteen lanes to a group, the reductions and the packing were ten times
 // the arithmetic: 16384 tokens of 32 + 16 heads 199-258 us.
 //
-// Bound: HBM for long chunks (q, k, v in, q out, 40 bytes per group), and
-// the launch plus one round trip to memory (positions, then tables) for a
-// step of single tokens.
+// Bound: HBM for long chunks (q, k, v in, q out, 40 bytes per group), though the
+// keys' arithmetic in f64 and their partners' loads keep it from it; the launch
+// plus one round trip to memory (positions, then tables) for a step of single
+// tokens. Measured with cold caches, 32 + 16 heads of 128, bf16: 16384 tokens 161 us
+// (357 MB), 2048 tokens 30 us, 16 caches of one token 11 us.
 #include "tokens.cuh"
 #include "pipeline.cuh"
 

