@@ -541,6 +541,8 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
         sections = list(sections) if sections is not None else [pairs]
         if len(sections) != axes:
             raise ValueError(f"{len(sections)} sections for {axes} axes")
+        if not all(isinstance(s, int) and 0 <= s <= pairs for s in sections):
+            raise ValueError(f"sections: integers in 0 .. {pairs} expected")
         rot = _pack_rotary(cos.data_ptr(), sin.data_ptr(), n_rows, 2 * pairs, 1 if interleaved else 0,
                            positions.data_ptr(), positions.stride(0) if axes > 1 else 0, axes, *sections,
                            *(0,) * (4 - axes))

@@ -82,3 +82,16 @@ def test_python_checks_refuse_before_the_library():
         E._index(torch.zeros(3, 4, 5, dtype=torch.int32), c)
     with pytest.raises(ValueError, match="contiguous"):
         E._contiguous(torch.zeros(4, 2).t(), c, "float32", (2, 4), "lse")
+
+
+@pytest.mark.parametrize("sections", [[16, 17], [-1, 33], [2 ** 40, 0], [16.0, 16], [32]])
+def test_bad_sections_are_refused(sections):
+    import torch
+
+    class Host(FakeCache):
+        shape = (2, 4, 64, -1)   # as if tensors on the host were on its device
+
+    x, tab = torch.zeros(3, 4, 64), torch.zeros(8, 32)
+    pos = torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises((ValueError, E.EakvError)):
+        E.append_rotary([Host()], 0, [3], x, x, cos=tab, sin=tab, positions=pos, sections=sections)
