@@ -130,6 +130,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
+// Power of two of a biased exponent below 255; 0 below 1.
+__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((uint32_t)max(e, 0) << 23); }
+
+// V-scale references (biased exponents): the units of p s are 2^(eref - kRefUp), a
+// scale may pass the reference by 2^kRefRoom, and both 2^(kRefUp - eref) and its
+// inverse are normal numbers from kRefLeast to 254.
+constexpr int kRefUp = 127 + 4, kRefRoom = 2, kRefLeast = 5;
+
 // Out of line: between two parts, with few registers to keep over the call.
 __device__ __noinline__ void step_walk(ExtWalk &walk, const ExtendArgs &a, const ExtendBatch &batch, int p) {
   walk.next(a, batch, p);
@@ -325,19 +333,21 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int k = 0; k < 4; k++) o[gg][m][n][k] = 0.0f;
-    float m_run[NT][2], m_eff[NT][2], l_run[NT][2], pb[NT][2][NG];
-    // Everything a row sums is divided by a power of two near the largest V scale
-    // the row has attended (eref: its biased exponent, -6 before the first), by
-    // way of the exponential's argument (m_eff); it moves like the maximum, when a
-    // scale passes it by 2^6, so that p s stays below 2^8 2^7.
+    float m_run[NT][2], l_run[NT][2], pb[NT][2][NG];
+    // The products p s, f16 operands, are held divided by a power of two near the
+    // largest V scale the row has attended (eref: its biased exponent), and o with
+    // them; p itself and the sums l and p b' are not. It moves like the maximum, when a
+    // scale passes it by 2^2, so that p s stays below 2^8 2^7 in its units (2^4 for a
+    // scale of the reference's size). It starts at the smallest that has an inverse:
+    // scales below it, denormal ones and zeros, need no reference of their own.
     int eref[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         m_run[n][e] = -INFINITY;
-        m_eff[n][e] = l_run[n][e] = 0.0f;
-        eref[n][e] = -6;
+        l_run[n][e] = 0.0f;
+        eref[n][e] = kRefLeast;
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) pb[n][e][gg] = 0.0f;
       }
@@ -433,7 +443,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       scales(vsm + C::NIB, p0, true, sv, bv);
       // ---- online softmax, base 2, lazy maximum -----------------------------------
       // A row moves when a score passes its maximum by 8, or a V scale that it
-      // attends passes its reference by 2^6 (scales are negative only in damaged
+      // attends passes its reference by 2^2 (scales are negative only in damaged
       // files; NaN is passed over).
       bool move = false;
       float lm[NT][2];
@@ -457,7 +467,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
             }
             ex[n][e] = (int)(__float_as_uint(sx) >> 23);
           }
-          move = move || lm[n][e] > m_run[n][e] + 8.0f || ex[n][e] > eref[n][e] + 6;
+          move = move || lm[n][e] > m_run[n][e] + 8.0f || ex[n][e] > eref[n][e] + kRefRoom;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -466,14 +476,14 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           for (int e = 0; e < 2; e++) {
             float t = lm[n][e];
             int x = ex[n][e];
-            if (!FULL && x >= 253) {   // without the infinite ones
+            if (!FULL && x >= 255) {   // without the infinite ones
               x = 0;
 #pragma unroll
               for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int gg = 0; gg < NG; gg++) {
                   const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
-                  if (on[n][e][j] && e1 < 255) x = max(x, min(e1, 252));
+                  if (on[n][e][j] && e1 < 255) x = max(x, e1);
                 }
             }
 #pragma unroll
@@ -481,23 +491,20 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
               if (!FULL) x = max(x, __shfl_xor_sync(0xffffffffu, x, b));
             }
-            const bool mv = t > m_run[n][e] + 8.0f, me = x > eref[n][e] + 6;
+            const bool mv = t > m_run[n][e] + 8.0f, me = x > eref[n][e] + kRefRoom;
             if (mv || me) {
-              float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
+              const float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
+              const float down = me ? alpha * pow2_biased(127 + eref[n][e] - x) : alpha;
               if (mv) m_run[n][e] = t;
-              // before the first reference all sums are zero, or NaN
-              if (me && eref[n][e] > 0) alpha *= __uint_as_float((uint32_t)max(127 + eref[n][e] - x, 0) << 23);
               if (me) eref[n][e] = x;
-              m_eff[n][e] = (m_run[n][e] == -INFINITY ? 0.0f : m_run[n][e]) +
-                            (eref[n][e] > 0 ? (float)(eref[n][e] - 127) : 0.0f);
               l_run[n][e] *= alpha;
 #pragma unroll
               for (int gg = 0; gg < NG; gg++) {
                 pb[n][e][gg] *= alpha;
 #pragma unroll
                 for (int m = 0; m < 4; m++) {
-                  o[gg][m][n][e] *= alpha;
-                  o[gg][m][n][2 + e] *= alpha;
+                  o[gg][m][n][e] *= down;
+                  o[gg][m][n][2 + e] *= down;
                 }
               }
             }
@@ -506,12 +513,14 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 2; e++)
+        for (int e = 0; e < 2; e++) {
+          const float m = m_run[n][e] == -INFINITY ? 0.0f : m_run[n][e];
 #pragma unroll
           for (int j = 0; j < J; j++) {
-            sc[n][e][j] = ex2(sc[n][e][j] - m_eff[n][e]);   // the weights from here on
+            sc[n][e][j] = ex2(sc[n][e][j] - m);   // the weights from here on
             l_run[n][e] += sc[n][e][j];
           }
+        }
       // ---- outputs -------------------------------------------------------------
 #pragma unroll
       for (int gg = 0; gg < NG; gg++) {
@@ -524,7 +533,8 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               // what is not attended adds nothing, whatever its scale and bias are
-              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * sv[j][gg] : 0.0f;
+              const float f = pow2_biased(127 + kRefUp - eref[n][e]);
+              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * (sv[j][gg] * f) : 0.0f;
               if (FULL || on[n][e][j]) pb[n][e][gg] = fmaf(sc[n][e][j], bv[j][gg], pb[n][e][gg]);
             }
             const uint32_t h = pack_f16(x[0], x[1]);
@@ -576,7 +586,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         for (int k = 0; k < 2 * NG; k++) {
           const uint32_t b = *reinterpret_cast<const uint32_t *>(ks + C::PB + C::NIB + 8 * (lane + 32 * k));
           const int e = (int)(b >> 23) & 255;
-          ex = max(ex, e < 255 ? min(e, 252) : 0);
+          ex = max(ex, e < 255 ? e : 0);
         }
         ex = __reduce_max_sync(0xffffffffu, ex);
 #pragma unroll 1
@@ -618,10 +628,10 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           for (int gg = 0; gg < NG; gg++) pb[n][e][gg] += __shfl_xor_sync(0xffffffffu, pb[n][e][gg], b);
         }
         const int row = warp * R + 8 * n + 2 * c + e;
-        const float vs = eref[n][e] > 0 ? __uint_as_float((uint32_t)eref[n][e] << 23) : 1.0f;
+        const float vs = pow2_biased(127 - kRefUp + eref[n][e]);
         if (g == 0) {
           mw[row] = m_run[n][e];
-          lw[row] = l_run[n][e] * vs;
+          lw[row] = l_run[n][e];
         }
 #pragma unroll
         for (int gg = 0; gg < NG; gg++)
@@ -629,7 +639,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           for (int w = 0; w < 2; w++)
 #pragma unroll
             for (int hi = 0; hi < 2; hi++) {
-              const float f = hi ? vs * 0.0625f : vs, b = pb[n][e][gg] * vs;
+              const float f = hi ? vs * 0.0625f : vs, b = pb[n][e][gg];
               *reinterpret_cast<float2 *>(ow + row * C::OS + 64 * gg + 32 * hi + 16 * w + 2 * g) =
                   make_float2(fmaf(o[gg][2 * w][n][2 * hi + e], f, b),
                               fmaf(o[gg][2 * w + 1][n][2 * hi + e], f, b));
