@@ -130,13 +130,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
-// Power of two of a biased exponent below 255; 0 below 1.
-__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((uint32_t)max(e, 0) << 23); }
-
-// V-scale references (biased exponents): the units of p s are 2^(eref - kRefUp), a
-// scale may pass the reference by 2^kRefRoom, and both 2^(kRefUp - eref) and its
-// inverse are normal numbers from kRefLeast to 254.
-constexpr int kRefUp = 127 + 4, kRefRoom = 2, kRefLeast = 5;
+// V-scale references: p s is held times a power of two per group that takes a scale
+// of the reference's size to [2^kRefUp, 2^(kRefUp+1)); a scale that it takes to kRefMost
+// moves it. kRefLeast is the smallest reference (biased exponent) whose power of two and
+// its inverse are both normal numbers. A row's two powers share a word, as the upper
+// halves of their f32.
+constexpr int kRefUp = 4, kRefLeast = 5;
+constexpr float kRefMost = 128.0f;
+__device__ __forceinline__ uint32_t ref_bits(int exponent) {
+  return (uint32_t)(254 + kRefUp - max(exponent, kRefLeast)) << 7;
+}
+template <int NG> __device__ __forceinline__ float ref_power(uint32_t word, int group) {
+  return __uint_as_float(group + 1 < NG ? word << 16 : word & 0xFFFF0000u);
+}
 
 // Out of line: between two parts, with few registers to keep over the call.
 __device__ __noinline__ void step_walk(ExtWalk &walk, const ExtendArgs &a, const ExtendBatch &batch, int p) {
@@ -335,19 +341,20 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           for (int k = 0; k < 4; k++) o[gg][m][n][k] = 0.0f;
     float m_run[NT][2], l_run[NT][2], pb[NT][2][NG];
     // The products p s, f16 operands, are held divided by a power of two near the
-    // largest V scale the row has attended (eref: its biased exponent), and o with
+    // largest V scale of the group that the row has attended, and the group's o with
     // them; p itself and the sums l and p b' are not. It moves like the maximum, when a
-    // scale passes it by 2^2, so that p s stays below 2^8 2^7 in its units (2^4 for a
-    // scale of the reference's size). It starts at the smallest that has an inverse:
-    // scales below it, denormal ones and zeros, need no reference of their own.
-    int eref[NT][2];
+    // scale passes it by 2^3, so that p s stays below 2^8 2^7 in its units. It starts
+    // at the smallest that has an inverse: scales below it, denormal ones and zeros,
+    // need no reference of their own. (One for both groups lost bits of the smaller:
+    // with one 2^-16 of the other f32 outputs were off by 2^-9.)
+    uint32_t vref[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         m_run[n][e] = -INFINITY;
         l_run[n][e] = 0.0f;
-        eref[n][e] = kRefLeast;
+        vref[n][e] = ref_bits(kRefLeast) * 0x10001u;
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) pb[n][e][gg] = 0.0f;
       }
@@ -370,8 +377,8 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       }
     };
 
-    // page_ex: largest exponent of a V scale of the page (full pages)
-    auto step = [&](auto full_tag, const uint8_t *ks, int page_pos0, int p0, int page_ex) {
+    float page_s[NG];   // largest finite V scale of each group of the page (full pages)
+    auto step = [&](auto full_tag, const uint8_t *ks, int page_pos0, int p0) {
       constexpr bool FULL = decltype(full_tag)::value;
       const uint8_t *vsm = ks + C::PB;
       bool on[NT][2][J];   // [row tile][row][position]
@@ -443,11 +450,10 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       scales(vsm + C::NIB, p0, true, sv, bv);
       // ---- online softmax, base 2, lazy maximum -----------------------------------
       // A row moves when a score passes its maximum by 8, or a V scale that it
-      // attends passes its reference by 2^2 (scales are negative only in damaged
+      // attends its group's reference by 2^3 (scales are negative only in damaged
       // files; NaN is passed over).
       bool move = false;
-      float lm[NT][2];
-      int ex[NT][2];
+      float lm[NT][2], sx[NT][2][NG];
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -455,19 +461,15 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           lm[n][e] = sc[n][e][0];
 #pragma unroll
           for (int j = 1; j < J; j++) lm[n][e] = fmaxf(lm[n][e], sc[n][e][j]);
-          if (FULL) {
-            ex[n][e] = page_ex;
-          } else {
-            float sx = 0.0f;
+          move = move || lm[n][e] > m_run[n][e] + 8.0f;
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-              float s = fabsf(sv[j][0]);
-              if (NG == 2) s = fmaxf(s, fabsf(sv[j][NG - 1]));
-              if (on[n][e][j]) sx = fmaxf(sx, s);
-            }
-            ex[n][e] = (int)(__float_as_uint(sx) >> 23);
+          for (int gg = 0; gg < NG; gg++) {
+            sx[n][e][gg] = FULL ? page_s[gg] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+              if (!FULL && on[n][e][j]) sx[n][e][gg] = fmaxf(sx[n][e][gg], fabsf(sv[j][gg]));
+            move = move || sx[n][e][gg] * ref_power<NG>(vref[n][e], gg) >= kRefMost;
           }
-          move = move || lm[n][e] > m_run[n][e] + 8.0f || ex[n][e] > eref[n][e] + kRefRoom;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -475,39 +477,47 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             float t = lm[n][e];
-            int x = ex[n][e];
-            if (!FULL && x >= 255) {   // without the infinite ones
-              x = 0;
 #pragma unroll
-              for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int gg = 0; gg < NG; gg++) {
-                  const int e1 = (int)(__float_as_uint(sv[j][gg]) >> 23) & 255;
-                  if (on[n][e][j] && e1 < 255) x = max(x, e1);
-                }
-            }
-#pragma unroll
-            for (int b = 4; b < 32; b <<= 1) {
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
-              if (!FULL) x = max(x, __shfl_xor_sync(0xffffffffu, x, b));
-            }
-            const bool mv = t > m_run[n][e] + 8.0f, me = x > eref[n][e] + kRefRoom;
-            if (mv || me) {
-              const float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
-              const float down = me ? alpha * pow2_biased(127 + eref[n][e] - x) : alpha;
-              if (mv) m_run[n][e] = t;
-              if (me) eref[n][e] = x;
+            for (int b = 4; b < 32; b <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
+            const bool mv = t > m_run[n][e] + 8.0f;
+            const float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
+            if (mv) {
+              m_run[n][e] = t;
               l_run[n][e] *= alpha;
+            }
+            uint32_t word = 0;
 #pragma unroll
-              for (int gg = 0; gg < NG; gg++) {
-                pb[n][e][gg] *= alpha;
+            for (int gg = 0; gg < NG; gg++) {
+              const float was = ref_power<NG>(vref[n][e], gg);
+              float x = sx[n][e][gg], down = alpha;
+              if (!FULL) {
+                if (x == INFINITY) {   // without the infinite ones
+                  x = 0.0f;
+#pragma unroll
+                  for (int j = 0; j < J; j++)
+                    if (on[n][e][j] && fabsf(sv[j][gg]) < INFINITY) x = fmaxf(x, fabsf(sv[j][gg]));
+                }
+#pragma unroll
+                for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+              }
+              uint32_t half = __float_as_uint(was) >> 16;
+              if (x * was >= kRefMost) {
+                half = ref_bits(__float_as_uint(x) >> 23);
+                // times the new power and the inverse of the old
+                down *= __uint_as_float(half << 16) *
+                        __uint_as_float((254u << 23) - __float_as_uint(was));
+              }
+              word |= half << (gg + 1 < NG ? 0 : 16);
+              if (down != 1.0f) {
 #pragma unroll
                 for (int m = 0; m < 4; m++) {
                   o[gg][m][n][e] *= down;
                   o[gg][m][n][2 + e] *= down;
                 }
               }
+              if (mv) pb[n][e][gg] *= alpha;
             }
+            vref[n][e] = word;
           }
       }
 #pragma unroll
@@ -533,8 +543,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               // what is not attended adds nothing, whatever its scale and bias are
-              const float f = pow2_biased(127 + kRefUp - eref[n][e]);
-              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * (sv[j][gg] * f) : 0.0f;
+              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * (sv[j][gg] * ref_power<NG>(vref[n][e], gg)) : 0.0f;
               if (FULL || on[n][e][j]) pb[n][e][gg] = fmaf(sc[n][e][j], bv[j][gg], pb[n][e][gg]);
             }
             const uint32_t h = pack_f16(x[0], x[1]);
@@ -581,19 +590,21 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       const bool full = page_pos0 >= it.all_lo && page_pos0 + kPagePositions <= it.all_hi;
       if (full) {
         // finite scales only: what an infinite one reaches is NaN anyway
-        int ex = 0;
+        uint32_t most = 0;
 #pragma unroll
-        for (int k = 0; k < 2 * NG; k++) {
-          const uint32_t b = *reinterpret_cast<const uint32_t *>(ks + C::PB + C::NIB + 8 * (lane + 32 * k));
-          const int e = (int)(b >> 23) & 255;
-          ex = max(ex, e < 255 ? e : 0);
+        for (int k = 0; k < 2 * NG; k++) {   // with two groups a lane's are of group lane % 2
+          const uint32_t b =
+              *reinterpret_cast<const uint32_t *>(ks + C::PB + C::NIB + 8 * (lane + 32 * k)) & 0x7fffffffu;
+          if (b < 0x7f800000u) most = max(most, b);
         }
-        ex = __reduce_max_sync(0xffffffffu, ex);
+#pragma unroll
+        for (int gg = 0; gg < NG; gg++)
+          page_s[gg] = __uint_as_float(__reduce_max_sync(0xffffffffu, lane % NG == gg ? most : 0u));
 #pragma unroll 1
-        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::true_type{}, ks, page_pos0, p0, ex);
+        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::true_type{}, ks, page_pos0, p0);
       } else {
 #pragma unroll 1
-        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::false_type{}, ks, page_pos0, p0, 0);
+        for (int p0 = 0; p0 < kPagePositions; p0 += 8 * J) step(std::false_type{}, ks, page_pos0, p0);
       }
       __syncwarp();
       if (lane == 0 && stage_release_last(reinterpret_cast<int *>(&bars[C::NSTAGE]) + st, 1) &&
@@ -628,13 +639,13 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           for (int gg = 0; gg < NG; gg++) pb[n][e][gg] += __shfl_xor_sync(0xffffffffu, pb[n][e][gg], b);
         }
         const int row = warp * R + 8 * n + 2 * c + e;
-        const float vs = pow2_biased(127 - kRefUp + eref[n][e]);
         if (g == 0) {
           mw[row] = m_run[n][e];
           lw[row] = l_run[n][e];
         }
 #pragma unroll
-        for (int gg = 0; gg < NG; gg++)
+        for (int gg = 0; gg < NG; gg++) {
+          const float vs = __uint_as_float((254u << 23) - __float_as_uint(ref_power<NG>(vref[n][e], gg)));
 #pragma unroll
           for (int w = 0; w < 2; w++)
 #pragma unroll
@@ -644,6 +655,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
                   make_float2(fmaf(o[gg][2 * w][n][2 * hi + e], f, b),
                               fmaf(o[gg][2 * w + 1][n][2 * hi + e], f, b));
             }
+        }
       }
     __syncthreads();
     for (int x = threadIdx.x; x < it.rows * (HD / 4); x += C::THREADS) {

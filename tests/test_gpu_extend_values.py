@@ -11,6 +11,7 @@ from test_gpu_extend import CODE, HALF_STEP, rounded, run
 pytestmark = pytest.mark.gpu
 
 KINDS = [("f32", "auto"), ("f16", "mma"), ("bf16", "mma"), ("f16", "umma"), ("bf16", "umma")]
+FEW = [k for k in KINDS if k[1] != "umma"]   # the warp-level kernel
 
 
 @pytest.fixture(autouse=True)
@@ -126,6 +127,25 @@ def test_the_smallest_values(gpu, first, rest, dtype, path):
     H, hd = 2, 128
     seq = Sequence(H, hd, [data(rng, H, 64, hd, v=first), data(rng, H, 4000, hd, v=rest)], 4)
     meets(gpu, seq, rng.standard_normal((4, 4, hd)).astype(np.float32), dtype, path)
+    seq.free()
+
+
+@pytest.mark.parametrize("dtype,path", FEW)
+@pytest.mark.parametrize("k", [8, 10, 12, 14, 16])
+@pytest.mark.parametrize("low", [0, 1])
+@pytest.mark.parametrize("window", [1, 0])
+def test_groups_of_different_size(gpu, window, low, k, dtype, path):
+    """One 64-dim group of V is 2^-k of the other: its dims keep their own precision. A window of one
+    makes each output a single position's value."""
+    rng = np.random.default_rng(k)
+    H, hd, new = 1, 128, 40
+    d = data(rng, H, 170, hd)
+    d[1, :, :, 64 * low:64 * low + 64] *= np.float32(2.0 ** -k)
+    if dtype == "f16":   # into its normal range: 2^-14 .. 2^16
+        d[1] *= np.float32(2.0 ** (k - 4))
+    seq = Sequence(H, hd, [d], new)
+    q = (0.05 * rng.standard_normal((new, 4, hd))).astype(np.float32)
+    meets(gpu, seq, q, dtype, path, window)
     seq.free()
 
 
