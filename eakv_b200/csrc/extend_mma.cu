@@ -9,11 +9,12 @@
 // matters on the V side: sum_j p_j s_j n_j of raw nibbles carries an offset of
 // 7.5 quanta that p_j b_j takes out again, and over 10^4 positions the rest is
 // hundreds of times smaller than the offset; of centred ones it is not.
-// Every row of q is scaled by a power of two into [16, 32): 16-bit q (8 or 11
-// bits) is then exact in f16 but for elements 2^-18 below the row's largest;
-// f32 q becomes two f16 limbs (hi, x - hi: 22 bits). p s is one f16 for 16-bit
-// types (2^-12 of each term, below the output's own rounding) and two limbs
-// for f32. Sums of scores, softmax and outputs are f32; the maximum moves
+// Every row of q is scaled by a power of two into [2^12, 2^13), of which the operands
+// that meet nibbles held times 16 take a sixteenth: 16-bit q (8 or 11 bits) is then
+// exact in f16 but for elements 2^-22 below the row's largest; f32 q becomes two
+// f16 limbs (hi, x - hi: 22 bits of elements down to 2^-11 of the row's largest). p s
+// is one f16 for 16-bit types (2^-12 of each term, below the output's own rounding)
+// and two limbs for f32. Sums of scores, softmax and outputs are f32; the maximum moves
 // lazily, when a score passes it by more than 8 (base 2), so p <= 256.
 //
 // Tiles. Both products are transposed, rows the n8 of the instructions: scores
@@ -259,7 +260,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         const int r = warp + C::NW * i;
         int e = 0;
         frexpf(mx[i] > 0.0f && fine ? mx[i] : 1.0f, &e);          // in [2^(e-1), 2^e)
-        const int qe = max(min(5 - e, 126), -126);
+        const int qe = max(min(13 - e, 126), -126);
         if (lane == 0) {
           const float up = fine ? __uint_as_float((uint32_t)(127 + qe) << 23) : 0.0f;
           up_s[r] = up;

@@ -149,6 +149,36 @@ def test_groups_of_different_size(gpu, window, low, k, dtype, path):
     seq.free()
 
 
+@pytest.mark.parametrize("dtype,path", [k for k in FEW if k[0] != "f16"])
+@pytest.mark.parametrize("k", [8, 12, 16])
+def test_key_groups_of_different_size(gpu, k, dtype, path):
+    """One group of K is 2^-k of the other, and q's dims there 2^k of the others: both groups take
+    the same part in the scores."""
+    rng = np.random.default_rng(k)
+    H, hd, new = 1, 128, 40
+    d = data(rng, H, 170, hd)
+    d[0, :, :, 64:] *= np.float32(2.0 ** -k)
+    seq = Sequence(H, hd, [d], new)
+    q = rng.standard_normal((new, 4, hd)).astype(np.float32) * 0.2
+    q[..., 64:] *= np.float32(2.0 ** k)
+    meets(gpu, seq, q, dtype, path)
+    seq.free()
+
+
+@pytest.mark.parametrize("dtype,path", FEW)
+def test_small_elements_of_q(gpu, dtype, path):
+    """Elements of q down to 2^-16 of their row's largest keep their bits: they meet keys as much larger."""
+    rng = np.random.default_rng(16)
+    H, hd, new = 1, 128, 40
+    d = data(rng, H, 170, hd, k=2.0 ** -6)
+    d[0, :, :, 64:] *= np.float32(2.0 ** 16)
+    seq = Sequence(H, hd, [d], new)
+    q = rng.standard_normal((new, 4, hd)).astype(np.float32) * 2.0 ** 5
+    q[..., 64:] *= np.float32(2.0 ** -16)
+    meets(gpu, seq, q, dtype, path)
+    seq.free()
+
+
 @pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("splits", [0, 4])
 def test_the_same_call_gives_the_same_bits(gpu, splits, dtype, path):
