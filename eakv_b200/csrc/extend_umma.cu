@@ -19,13 +19,16 @@
 // memory has no room, and four more FMAs per score). P' = 2^7 p is at most
 // 2^15, one f16.
 //
-// Ranges. K and V are divided by powers of two taken from the first tile
-// (eref): then 128 values of a row lie in f16's range for rows within 2^-10 and
-// 2^12 of it. A run of 32 positions with a row outside of that is marked: its rows
-// are divided by powers of their own, which go to the softmax threads beside
-// it, and these scale the scores and the weights column by column, with
+// Ranges. K and V are multiplied by powers of two that take the largest row of the
+// first tile (eref) to 2^10. Rows up to 2^4 above it stay in f16's range, and a group's
+// scale is a normal f16 number down to groups 2^-21 of the reference (each factor of two
+// below costs a bit). A run of 32 positions with a row above that, or 2^-10 below the
+// reference, is marked: its rows have powers of their own, which go to the softmax
+// threads beside it, and these scale the scores and the weights column by column, with
 // a V reference of their own per row, taken from attended positions only. So a
 // position that a row does not attend has no influence on it, however large.
+// (With the reference at 2^0 and high nibbles held times 16 with a sixteenth of the
+// scale, groups 2^-12 of their neighbour lost all but 3 to 5 bits.)
 // Non-finite V groups are kept out of the products (0 NaN is NaN) and
 // listed by position; a row that attends one gets NaN in the group's dims.
 //
@@ -82,7 +85,9 @@ constexpr int kThreads = (kSoftWarps + kConvWarps + 4) * 32;   // four warpgroup
 constexpr int kRegs = 128, kRegsSoft = 176, kRegsConv = 104, kRegsMma = 56;
 static_assert(2 * kRegsSoft + kRegsConv + kRegsMma == 4 * kRegs, "register split");
 constexpr int kUnset = -100000;
-constexpr int kUp = 12, kDown = 10;           // rows within 2^kUp, 2^-kDown of eref need no mark
+constexpr int kTop = 10;                      // a row's values below 2^(e+1) are held below 2^(kTop+1)
+constexpr int kUp = 4, kDown = 10;            // rows within 2^kUp, 2^-kDown of eref need no mark
+static_assert(kTop + 1 + kUp <= 15, "rows without a mark fit f16");
 constexpr float kPShift = 7.0f;               // P' = 2^7 p
 constexpr uint32_t kLayoutSW128 = 2;
 
@@ -239,20 +244,23 @@ __device__ __forceinline__ int row_exp(const RawRow<HD> &r, uint32_t &bad) {
   return m > 0.0f ? (int)(__float_as_uint(m) >> 23) - 127 : kUnset;
 }
 
-// The row's values divided by 2^e as f16 into row `row` of an operand: 16-byte
+// The row's values times 2^(kTop - e) as f16 into row `row` of an operand: 16-byte
 // chunk j of half g holds word j of group g. A group in `zero` is stored as 0.
 template <int HD>
 __device__ __forceinline__ void store_row(const RawRow<HD> &r, uint8_t *op, int row, int e,
                                           uint32_t zero) {
   using C = WCfg<HD>;
-  // 2^-e in two factors: e spans more than the exponents of one float
-  const float f0 = pow2i(-(e >> 1)), f1 = pow2i(-(e - (e >> 1)));
+  // in two factors: e spans more than the exponents of one float
+  const int up = kTop - e;
+  const float f0 = pow2i(up >> 1), f1 = pow2i(up - (up >> 1));
 #pragma unroll
   for (int g = 0; g < HD / 64; g++) {
     const float s = r.sb[2 * g] * f0 * f1, b = fmaf(8.0f, r.sb[2 * g], r.sb[2 * g + 1]) * f0 * f1;
-    __half2 sl = __float2half2_rn(s), sh = __float2half2_rn(s * 0.0625f), bb = __float2half2_rn(b);
+    __half2 ss = __float2half2_rn(s), bb = __float2half2_rn(b);
     const bool z = (zero >> g) & 1;
-    if (z) sl = sh = bb = __float2half2_rn(0.0f);
+    if (z) ss = bb = __float2half2_rn(0.0f);
+    // 1024 + 16 n of a high nibble becomes 64 + n, then n - 8: both exact
+    const __half2 down = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.0f);
     const uint32_t words[8] = {r.w[2 * g].x, r.w[2 * g].y, r.w[2 * g].z, r.w[2 * g].w,
                                r.w[2 * g + 1].x, r.w[2 * g + 1].y, r.w[2 * g + 1].z, r.w[2 * g + 1].w};
     uint8_t *base = op + g * C::HALF + row * 128;
@@ -261,10 +269,10 @@ __device__ __forceinline__ void store_row(const RawRow<HD> &r, uint8_t *op, int 
       const uint32_t w = words[j], y = w >> 8;
       const __half2 lo0 = __hsub2(as_half2(and_or(w, 0x000F000Fu, 0x64006400u)), as_half2(0x64086408u));
       const __half2 lo1 = __hsub2(as_half2(and_or(y, 0x000F000Fu, 0x64006400u)), as_half2(0x64086408u));
-      const __half2 hi0 = __hsub2(as_half2(and_or(w, 0x00F000F0u, 0x64006400u)), as_half2(0x64806480u));
-      const __half2 hi1 = __hsub2(as_half2(and_or(y, 0x00F000F0u, 0x64006400u)), as_half2(0x64806480u));
-      const uint4 v = make_uint4(as_u32(__hfma2(lo0, sl, bb)), as_u32(__hfma2(lo1, sl, bb)),
-                                 as_u32(__hfma2(hi0, sh, bb)), as_u32(__hfma2(hi1, sh, bb)));
+      const __half2 hi0 = __hfma2(as_half2(and_or(w, 0x00F000F0u, 0x64006400u)), down, off);
+      const __half2 hi1 = __hfma2(as_half2(and_or(y, 0x00F000F0u, 0x64006400u)), down, off);
+      const uint4 v = make_uint4(as_u32(__hfma2(lo0, ss, bb)), as_u32(__hfma2(lo1, ss, bb)),
+                                 as_u32(__hfma2(hi0, ss, bb)), as_u32(__hfma2(hi1, ss, bb)));
       *reinterpret_cast<uint4 *>(base + ((j ^ (row & 7)) << 4)) = v;
     }
   }
@@ -608,10 +616,10 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       references();
       const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
       const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
-      // score factor: |scale| log2 e / 2^(q exponent), with K's 2^kref
+      // score factor: |scale| log2 e / 2^(q exponent), with K's 2^(kref - kTop)
       float c_row = reinterpret_cast<const float *>(smem + C::ROWC)[r_loc];
-      c_row *= pow2i(kref >> 1);
-      c_row *= pow2i(kref - (kref >> 1));
+      c_row *= pow2i((kref - kTop) >> 1);
+      c_row *= pow2i(kref - kTop - ((kref - kTop) >> 1));
       float m_run = -INFINITY, l_run = 0.0f;
       int eref = kUnset;
       bool poison0 = false, poison1 = false;   // a non-finite V group was attended
@@ -811,8 +819,8 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         fence_after_sync();
         const float down = 0.0078125f;   // 2^-kPShift
         const float L = l_run * down;
-        // O carries 2^(kPShift - eref); in two factors. Finished rows are divided here.
-        const int e = eref == kUnset ? 0 : eref;
+        // O carries 2^(kPShift + kTop - eref); in two factors. Finished rows are divided here.
+        const int e = eref == kUnset ? 0 : eref - kTop;
         const float inv = it.n_parts > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);
         const float f0 = pow2i(e >> 1) * down, f1 = pow2i(e - (e >> 1)) * inv;
         if (r_loc < it.rows) {

@@ -11,7 +11,6 @@ from test_gpu_extend import CODE, HALF_STEP, rounded, run
 pytestmark = pytest.mark.gpu
 
 KINDS = [("f32", "auto"), ("f16", "mma"), ("bf16", "mma"), ("f16", "umma"), ("bf16", "umma")]
-FEW = [k for k in KINDS if k[1] != "umma"]   # the warp-level kernel
 
 
 @pytest.fixture(autouse=True)
@@ -130,7 +129,7 @@ def test_the_smallest_values(gpu, first, rest, dtype, path):
     seq.free()
 
 
-@pytest.mark.parametrize("dtype,path", FEW)
+@pytest.mark.parametrize("dtype,path", KINDS)
 @pytest.mark.parametrize("k", [8, 10, 12, 14, 16])
 @pytest.mark.parametrize("low", [0, 1])
 @pytest.mark.parametrize("window", [1, 0])
@@ -149,7 +148,22 @@ def test_groups_of_different_size(gpu, window, low, k, dtype, path):
     seq.free()
 
 
-@pytest.mark.parametrize("dtype,path", [k for k in FEW if k[0] != "f16"])
+@pytest.mark.parametrize("dtype,path", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("k", [5, 9, 11, 14])
+def test_rows_below_the_first(gpu, hd, k, dtype, path):
+    """V rows 2^-k of those of the part's first positions, each seen alone."""
+    rng = np.random.default_rng(k)
+    new = 70
+    seq = Sequence(1, hd, [data(rng, 1, 128, hd, v=2.0 ** (k - 8)), data(rng, 1, 150, hd, v=2.0 ** -8)], new)
+    E.force_splits(1)
+    q = (0.05 * rng.standard_normal((new, 2, hd))).astype(np.float32)
+    meets(gpu, seq, q, dtype, path, window=1)
+    meets(gpu, seq, q, dtype, path, window=60)
+    seq.free()
+
+
+@pytest.mark.parametrize("dtype,path", [k for k in KINDS if k[0] != "f16"])
 @pytest.mark.parametrize("k", [8, 12, 16])
 def test_key_groups_of_different_size(gpu, k, dtype, path):
     """One group of K is 2^-k of the other, and q's dims there 2^k of the others: both groups take
@@ -165,7 +179,7 @@ def test_key_groups_of_different_size(gpu, k, dtype, path):
     seq.free()
 
 
-@pytest.mark.parametrize("dtype,path", FEW)
+@pytest.mark.parametrize("dtype,path", KINDS)
 def test_small_elements_of_q(gpu, dtype, path):
     """Elements of q down to 2^-16 of their row's largest keep their bits: they meet keys as much larger."""
     rng = np.random.default_rng(16)
