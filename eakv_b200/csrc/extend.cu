@@ -20,7 +20,8 @@ constexpr size_t kCounterBytes = kSplitItems * sizeof(unsigned);
 // the warp-level kernel four warps take pages in turn: 64 pages are 64 steps of a
 // warp (2^-18 at worst, 2^-19 on average, below what f32 results ask for), and
 // 1024 pages 2^-14; in the tcgen05 kernel one sum takes every step, and 1024 pages
-// are 2^-12, 2^-13 on average: both below the 2^-9 or 2^-12 of 16-bit outputs. (With 256
+// are 2^-12, 2^-13 on average: both below the 2^-9 or 2^-12 of 16-bit outputs (and the
+// latter below what K's rounding to f16 does there, 2^-10). (With 256
 // pages for the warp-level kernel 16 caches of up to 32768 positions were kept from
 // equal runs by tiles of 8 rows: 303 us, in runs 231.)
 constexpr int kPartPagesF32 = 64, kPartPages16 = 1024;

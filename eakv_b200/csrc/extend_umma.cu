@@ -11,13 +11,17 @@
 // (when a score passes it by more than 8).
 //
 // Operands are f16. Q' is q times a power of two per row (exact for bf16 and
-// f16 but for elements 2^-18 below the row's largest). K' and V' are the
-// dequantized values s (n - 8) + (b + 8 s): n - 8 is exact, s and b + 8 s are rounded
-// to f16 and the result once more (3 roundings of 2^-12 relative to the
-// value's own size, against the 2^-9 of a bf16 output; keeping the nibbles
-// exact instead needs a second accumulator per 64-dim group, for which tensor
-// memory has no room, and four more FMAs per score). P' = 2^7 p is at most
-// 2^15, one f16.
+// f16 but for elements 2^-18 below the row's largest). K' and V' are the dequantized
+// values in f16. K' is rounded once (half a step, 2^-11 of the value): with b + 8 s =
+// j s + r, j whole, and s = s_hi + s_lo it is m s_hi + (m s_lo + r), m = n - 8 + j, whose first
+// product is exact and whose second term is small. With s and b + 8 s rounded to f16
+// first, one FMA less, all dims of a position are off alike, which adds up in its
+// score: outputs were off by 1.7e-3 of their size in all, now by 0.8e-3, where the rounding
+// of a bf16 output alone is 1.7e-3 and that of an f16 one 0.2e-3. In V', whose errors
+// are independent from position to position, s is one f16. Keeping K's nibbles
+// exact instead needs a second accumulator per 64-dim group, for which tensor memory
+// has no room, and four more FMAs per score; f32 rows, which the warp-level kernel
+// serves, have them exact. P' = 2^7 p is at most 2^15, one f16.
 //
 // Ranges. K and V are multiplied by powers of two that take the largest row of the
 // first tile (eref) to 2^10. Rows up to 2^4 above it stay in f16's range, and a group's
@@ -245,8 +249,9 @@ __device__ __forceinline__ int row_exp(const RawRow<HD> &r, uint32_t &bad) {
 }
 
 // The row's values times 2^(kTop - e) as f16 into row `row` of an operand: 16-byte
-// chunk j of half g holds word j of group g. A group in `zero` is stored as 0.
-template <int HD>
+// chunk k of half g holds word k of group g. A group in `zero` is stored as 0.
+// KEY: with s in two limbs; else s is rounded first.
+template <int HD, bool KEY>
 __device__ __forceinline__ void store_row(const RawRow<HD> &r, uint8_t *op, int row, int e,
                                           uint32_t zero) {
   using C = WCfg<HD>;
@@ -256,24 +261,29 @@ __device__ __forceinline__ void store_row(const RawRow<HD> &r, uint8_t *op, int 
 #pragma unroll
   for (int g = 0; g < HD / 64; g++) {
     const float s = r.sb[2 * g] * f0 * f1, b = fmaf(8.0f, r.sb[2 * g], r.sb[2 * g + 1]) * f0 * f1;
-    __half2 ss = __float2half2_rn(s), bb = __float2half2_rn(b);
-    const bool z = (zero >> g) & 1;
-    if (z) ss = bb = __float2half2_rn(0.0f);
-    // 1024 + 16 n of a high nibble becomes 64 + n, then n - 8: both exact
-    const __half2 down = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.0f);
+    // b = j s + r, and s in two limbs: m s_hi is exact for m = n - 8 + j (6 and 5 bits),
+    // m s_lo + r is small. (s = 0 gives j of either end and r = b.)
+    const float j = fminf(fmaxf(rintf(__fdividef(b, s)), -16.0f), 16.0f);
+    const float hi = KEY ? __uint_as_float(__float_as_uint(s) & 0xFFFC0000u) : s;
+    __half2 sh = __float2half2_rn(hi), sl = __float2half2_rn(s - hi), rr = __float2half2_rn(fmaf(-j, s, b));
+    if ((zero >> g) & 1) sh = sl = rr = __float2half2_rn(0.0f);
+    // n of a low nibble lies in 1024 + n, of a high one in 1024 + 16 n, a sixteenth of
+    // which is 64 + n: all exact
+    const __half2 off_lo = __float2half2_rn(1032.0f - j), off_hi = __float2half2_rn(j - 72.0f);
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
     const uint32_t words[8] = {r.w[2 * g].x, r.w[2 * g].y, r.w[2 * g].z, r.w[2 * g].w,
                                r.w[2 * g + 1].x, r.w[2 * g + 1].y, r.w[2 * g + 1].z, r.w[2 * g + 1].w};
     uint8_t *base = op + g * C::HALF + row * 128;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const uint32_t w = words[j], y = w >> 8;
-      const __half2 lo0 = __hsub2(as_half2(and_or(w, 0x000F000Fu, 0x64006400u)), as_half2(0x64086408u));
-      const __half2 lo1 = __hsub2(as_half2(and_or(y, 0x000F000Fu, 0x64006400u)), as_half2(0x64086408u));
-      const __half2 hi0 = __hfma2(as_half2(and_or(w, 0x00F000F0u, 0x64006400u)), down, off);
-      const __half2 hi1 = __hfma2(as_half2(and_or(y, 0x00F000F0u, 0x64006400u)), down, off);
-      const uint4 v = make_uint4(as_u32(__hfma2(lo0, ss, bb)), as_u32(__hfma2(lo1, ss, bb)),
-                                 as_u32(__hfma2(hi0, ss, bb)), as_u32(__hfma2(hi1, ss, bb)));
-      *reinterpret_cast<uint4 *>(base + ((j ^ (row & 7)) << 4)) = v;
+    for (int k = 0; k < 8; k++) {
+      const uint32_t w = words[k], y = w >> 8;
+      const __half2 lo0 = __hsub2(as_half2(and_or(w, 0x000F000Fu, 0x64006400u)), off_lo);
+      const __half2 lo1 = __hsub2(as_half2(and_or(y, 0x000F000Fu, 0x64006400u)), off_lo);
+      const __half2 hi0 = __hfma2(as_half2(and_or(w, 0x00F000F0u, 0x64006400u)), sixteenth, off_hi);
+      const __half2 hi1 = __hfma2(as_half2(and_or(y, 0x00F000F0u, 0x64006400u)), sixteenth, off_hi);
+      auto value = [&](__half2 m) { return as_u32(__hfma2(m, sh, KEY ? __hfma2(m, sl, rr) : rr)); };
+      *reinterpret_cast<uint4 *>(base + ((k ^ (row & 7)) << 4)) =
+          make_uint4(value(lo0), value(lo1), value(hi0), value(hi1));
     }
   }
 }
@@ -429,13 +439,13 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
           reinterpret_cast<int *>(smem + C::INFO)[(n % kInfo) * 4 + cw] = (mark ? 1 : 0) | ((n0 | n1) ? 2 : 0);
           reinterpret_cast<uint2 *>(smem + C::NANS)[(n % kInfo) * 4 + cw] = make_uint2(n0, n1);
         }
-        store_row<HD>(kr, smem + C::K + st * C::TILE, crow, kx, 0u);
+        store_row<HD, true>(kr, smem + C::K + st * C::TILE, crow, kx, 0u);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kKFull + st));
         fetch(kr, kpages, i + 1);
         if (n >= 2 && !wait_warp(kVFree + st, (n >> 1) - 1)) break;
-        store_row<HD>(vr, smem + C::V + st * C::TILE, crow, vx, vbad);
+        store_row<HD, false>(vr, smem + C::V + st * C::TILE, crow, vx, vbad);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kVFull + st));
