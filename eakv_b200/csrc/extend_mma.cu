@@ -145,6 +145,16 @@ template <int NG> __device__ __forceinline__ float ref_power(uint32_t word, int 
   return __uint_as_float(group + 1 < NG ? word << 16 : word & 0xFFFF0000u);
 }
 
+// Whether a group with a scale of 1 has only zero nibbles: the quantizer's form of 64
+// equal values. Its offset b + 8 s would carry the scale of 1 into sums of values of any
+// size (zero vectors among V of 1e-3: outputs off by several times their size), so such
+// groups get a scale of 0 in the copy of their page.
+__device__ __forceinline__ bool constant_group(const uint8_t *page, int slot) {
+  const uint4 x = *reinterpret_cast<const uint4 *>(page + slot * 32);
+  const uint4 y = *reinterpret_cast<const uint4 *>(page + slot * 32 + 16);
+  return ((x.x | x.y | x.z | x.w) | (y.x | y.y | y.z | y.w)) == 0;
+}
+
 // Out of line: between two parts, with few registers to keep over the call.
 __device__ __noinline__ void step_walk(ExtWalk &walk, const ExtendArgs &a, const ExtendBatch &batch, int p) {
   walk.next(a, batch, p);
@@ -586,9 +596,22 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
         ok = false;
         break;
       }
-      const uint8_t *ks = smem + st * C::STAGE_BYTES;
+      uint8_t *ks = smem + st * C::STAGE_BYTES;
       const int page_pos0 = (it.pg0 + i) * kPagePositions;
       const bool full = page_pos0 >= it.all_lo && page_pos0 + kPagePositions <= it.all_hi;
+      bool one = false;
+#pragma unroll
+      for (int k = 0; k < 4 * NG; k++)   // K, then V
+        one = one || *reinterpret_cast<const float *>(ks + (k / (2 * NG)) * C::PB + C::NIB +
+                                                      8 * (lane + 32 * (k % (2 * NG)))) == 1.0f;
+      if (__any_sync(0xffffffffu, one)) {   // groups of equal values: this warp alone has the page
+        for (int x = lane; x < 2 * kPagePositions * NG; x += 32) {
+          uint8_t *page = ks + x / (kPagePositions * NG) * C::PB;
+          float *s = reinterpret_cast<float *>(page + C::NIB + 8 * (x % (kPagePositions * NG)));
+          if (*s == 1.0f && constant_group(page, x % (kPagePositions * NG))) *s = 0.0f;
+        }
+        __syncwarp();
+      }
       if (full) {
         // finite scales only: what an infinite one reaches is NaN anyway
         uint32_t most = 0;

@@ -231,6 +231,18 @@ __device__ __forceinline__ void load_row(RawRow<HD> &r, const uint8_t *page, int
   }
 }
 
+// A group with a scale of 1 and only zero nibbles, the quantizer's form of 64 equal
+// values, gets a scale of 0: b + 8 s and the row's power of two are the values' own.
+template <int HD>
+__device__ __forceinline__ void drop_idle_scales(RawRow<HD> &r) {
+#pragma unroll
+  for (int g = 0; g < HD / 64; g++)
+    if (r.sb[2 * g] == 1.0f) {
+      const uint4 x = r.w[2 * g], y = r.w[2 * g + 1];
+      if (((x.x | x.y | x.z | x.w) | (y.x | y.y | y.z | y.w)) == 0) r.sb[2 * g] = 0.0f;
+    }
+}
+
 // Exponent e with every |value| of the row's finite groups below 2^(e+1);
 // kUnset when they are all zero or none is finite. Bit g of `bad`: group g is
 // not finite.
@@ -417,6 +429,8 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       };
       fetch(kr, kpages, 0);
       fetch(vr, vpages, 0);
+      drop_idle_scales<HD>(kr);
+      drop_idle_scales<HD>(vr);
       uint32_t bad;
       const int ek = __reduce_max_sync(0xffffffffu, row_exp<HD>(kr, bad));
       const int ev = __reduce_max_sync(0xffffffffu, row_exp<HD>(vr, bad));
@@ -425,6 +439,10 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       references();
       for (int i = 0; i < n_tiles; i++) {
         const int n = done + i, st = n & 1;
+        if (i > 0) {
+          drop_idle_scales<HD>(kr);
+          drop_idle_scales<HD>(vr);
+        }
         uint32_t kbad, vbad;
         const int ke = row_exp<HD>(kr, kbad), ve = row_exp<HD>(vr, vbad);
         const bool mark = __any_sync(0xffffffffu, (ke != kUnset && (ke > kref + kUp || ke < kref - kDown)) ||

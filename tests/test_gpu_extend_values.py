@@ -205,3 +205,22 @@ def test_the_same_call_gives_the_same_bits(gpu, splits, dtype, path):
         out, l = run(gpu, seq, 0, q, dtype, 8)
         assert np.array_equal(out, first) and np.array_equal(l, lse)
     seq.free()
+
+
+@pytest.mark.parametrize("dtype,path", KINDS)
+@pytest.mark.parametrize("hd,new", [(128, 3), (64, 50)])
+@pytest.mark.parametrize("level", [0.0, 3e-4])
+def test_groups_of_one_value(gpu, level, hd, new, dtype, path):
+    """A group of 64 equal values has a scale of 1 whatever they are: zero vectors, or 3e-4 in all dims,
+    among values of 1e-3 do not bring errors of that scale."""
+    rng = np.random.default_rng(hd)
+    d = data(rng, 2, 300, hd, k=0.1, v=1e-3)
+    d[1, :, ::2] = level
+    d[1, 1, 1::4, :64] = -level
+    d[0, :, 5::7] = level
+    d[:, :, 128:192] = level     # a whole page
+    seq = Sequence(2, hd, [d], new)
+    q = rng.standard_normal((new, 4, hd)).astype(np.float32)
+    meets(gpu, seq, q, dtype, path)
+    meets(gpu, seq, q, dtype, path, window=3)
+    seq.free()
