@@ -82,6 +82,7 @@ SIGNATURES = {
     "eakv_lse_combine": (_I, [_I, _I, _I, _P, _P, _P, _P, _P]),
     "eakv_test_force_splits": (_I, [_I]),
     "eakv_test_force_path": (_I, [_I]),
+    "eakv_test_extend_registers": (_I, [_I]),
     "eakv_test_choose_splits": (_I, [_c.c_longlong, _I, _I, _I, _I, _I]),
     "eakv_test_stall": (_I, [_I, ctypes.c_uint]),
     "eakv_test_separate_merge": (_I, [_I]),
@@ -736,6 +737,12 @@ def force_path(path):
     mma.sync tensor-core kernel, 3 the tcgen05 tensor-core kernel (head_dim
     128), 0 the automatic choice."""
     lib().eakv_test_force_path(int(path))
+
+
+def extend_registers(n):
+    """Registers per thread that extend_attention's tcgen05 kernel counts as built with
+    (0: what it was built with); with another number than its own it is left out."""
+    lib().eakv_test_extend_registers(int(n))
 
 
 def test_stall(page, wait_budget=0):

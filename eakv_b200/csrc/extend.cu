@@ -66,13 +66,13 @@ int sm_count(int dev) {
 
 // The caches of `t` that belong to the part, their row tiles, splits and record
 // bytes. Call with the caches' device current.
-int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool umma, Part &p) {
+int plan_part(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool many_ok, bool umma,
+              Part &p) {
   p.umma = umma;
   p.tile_rows = kExtendUmmaRows;
   auto mine = [&](int i) {
     const long long rows = (long long)(t.first[i + 1] - t.first[i]) * a.G;
-    const bool many = a.dtype != EAKV_F32 && t_force_path != 2 && (rows > kMmaRows || t_force_path == 3);
-    return rows > 0 && many == umma;
+    return rows > 0 && (many_ok && (rows > kMmaRows || t_force_path == 3)) == umma;
   };
   p.n_caches = 0;
   p.slots = p.run = p.n_runs = p.overhead = 0;
@@ -179,6 +179,15 @@ int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool u
   return EAKV_OK;
 }
 
+// Both parts of a call: the caches with many rows, which the tcgen05 kernel takes where
+// it can, and the others.
+int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, Part (&p)[2]) {
+  const bool many_ok = a.dtype != EAKV_F32 && t_force_path != 2 &&
+                       extend_umma_usable(a.geom.gpd * 64, a.dtype);
+  int rc = plan_part(a, t, device, tree, many_ok, true, p[0]);
+  return rc ? rc : plan_part(a, t, device, tree, many_ok, false, p[1]);
+}
+
 size_t record_bytes(const ExtendArgs &a, const Part &p) {
   return (size_t)p.slots * p.tile_rows * (a.geom.gpd * 64 + 2) * sizeof(float);
 }
@@ -235,7 +244,7 @@ int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const
   if (rc || total == 0) return rc;
   DeviceGuard g(caches[0]->device);
   Part p[2];
-  for (int k = 0; k < 2 && !rc; k++) rc = plan(a, b, caches[0]->device, tree != 0, k == 0, p[k]);
+  rc = plan(a, b, caches[0]->device, tree != 0, p);
   if (!rc) *bytes = workspace_of(a, p);
   return rc;
 }
@@ -272,7 +281,7 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
   a.status = device_status_ptr();
   if (!a.status) return refuse("device status word unavailable");
   Part p[2];
-  for (int k = 0; k < 2 && !rc; k++) rc = plan(a, b, c0->device, tree != nullptr, k == 0, p[k]);
+  rc = plan(a, b, c0->device, tree != nullptr, p);
   if (rc) return rc;
   cudaStream_t s = stream ? (cudaStream_t)stream : c0->stream;
   const size_t need = workspace_of(a, p);

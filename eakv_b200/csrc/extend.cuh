@@ -419,8 +419,9 @@ __device__ __forceinline__ void extend_merge(const ExtendArgs &a, const ExtItem 
 int extend_mma_resident(int head_dim, int dtype, int tile_rows);
 int extend_mma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                       bool vec, cudaStream_t s);
-// extend_umma.cu: 16-bit types
+// extend_umma.cu: 16-bit types, where the kernel can run (current device)
 constexpr int kExtendUmmaRows = 256;
+bool extend_umma_usable(int head_dim, int dtype);
 int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                        bool vec, cudaStream_t s);
 

@@ -968,6 +968,23 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
   if (warp == kMmaWarp) tmem_dealloc(tm, C::COLS);
 }
 
+// Registers per thread that the kernel was built with (0: unknown).
+template <int HD, typename T>
+int built_registers() {
+  static std::atomic<int> known[64];   // per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int regs = known[dev & 63].load(std::memory_order_relaxed);
+  if (regs) return regs;
+  cudaFuncAttributes at;
+  if (cudaFuncGetAttributes(&at, extend_umma_kernel<HD, T>) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  known[dev & 63].store(at.numRegs, std::memory_order_relaxed);
+  return at.numRegs;
+}
+
 template <int HD, typename T>
 int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks, bool vec,
                cudaStream_t s) {
@@ -980,15 +997,6 @@ int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs
     int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
                         "extend_umma: smem attribute");
     if (rc) return rc;
-    // the warpgroups trade the launch's registers: they have to add up
-    cudaFuncAttributes at;
-    rc = check_cuda(cudaFuncGetAttributes(&at, fn), "extend_umma: attributes");
-    if (rc) return rc;
-    if (at.numRegs != kRegs) {
-      set_error(EAKV_ERR_INVALID, "extend_umma: built with %d registers per thread, %d expected",
-                at.numRegs, kRegs);
-      return EAKV_ERR_INVALID;
-    }
     attr_done.fetch_or(1ull << (dev & 63), std::memory_order_acq_rel);
   }
   fn<<<n_blocks, kThreads, C::SMEM, s>>>(a, b, runs, vec ? 1 : 0);
@@ -996,6 +1004,19 @@ int launch_one(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs
 }
 
 }  // namespace
+
+thread_local int t_extend_registers = 0;
+
+// The warpgroups trade the launch's registers, which have to add up: a compiler (or a
+// debug build) that takes another number per thread leaves this kernel out.
+bool extend_umma_usable(int head_dim, int dtype) {
+  const int regs = t_extend_registers ? t_extend_registers
+                   : head_dim == 128  ? (dtype == EAKV_F16 ? built_registers<128, __half>()
+                                                           : built_registers<128, __nv_bfloat16>())
+                                      : (dtype == EAKV_F16 ? built_registers<64, __half>()
+                                                           : built_registers<64, __nv_bfloat16>());
+  return regs == kRegs;
+}
 
 int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRuns &runs, int n_blocks,
                        bool vec, cudaStream_t s) {
@@ -1007,3 +1028,8 @@ int extend_umma_launch(const ExtendArgs &a, const ExtendBatch &b, const ExtendRu
 }
 
 }  // namespace eakv
+
+extern "C" int eakv_test_extend_registers(int n) {
+  eakv::t_extend_registers = n > 0 ? n : 0;
+  return EAKV_OK;
+}

@@ -334,6 +334,12 @@ int eakv_test_choose_splits(long long items, int max_pages, int lo, int hi, int 
  * tcgen05 kernel whatever the number of rows is. */
 int eakv_test_force_path(int path);
 
+/* Later eakv_extend_attention calls on this host thread take the tcgen05
+ * kernel to have been built with n registers per thread (0: what it was built
+ * with). It can only run with the number it was written for; with another, as
+ * another compiler may give it, the mma.sync kernel serves every call. */
+int eakv_test_extend_registers(int n);
+
 /* on != 0 makes later decode calls on this host thread merge their sequence
  * splits in a second kernel launch after the decode, instead of in the
  * decode kernel's last CTA of each row group; 0 restores the default. The

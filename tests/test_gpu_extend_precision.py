@@ -150,3 +150,26 @@ def test_root_mean_square_of_trees(gpu, dtype, path):
     r, _ = ratios(got[10:11], lse[10:11], [a[10:11] for a in expected(b, q, dtype, path, tree=wrong)])
     assert r > 3, r
     b.free()
+
+
+@pytest.mark.parametrize("dtype,path", [("bf16", "auto"), ("f16", "umma")])
+def test_a_build_without_the_tcgen05_kernel(gpu, dtype, path):
+    """A register count that the kernel's warpgroups cannot trade: calls of many rows run on the
+    warp-level kernel, with its bits."""
+    rng = np.random.default_rng(2)
+    b = Batch(rng, 1, 2, 128, [300, 10], [100, 3])
+    q = rounded(rng.standard_normal((103, 8, 128)).astype(np.float32), dtype)
+    here, _ = run(gpu, b, 0, q, dtype, 8)
+    E.force_path(CODE["mma"])
+    want, wl = run(gpu, b, 0, q, dtype, 8)
+    E.force_path(CODE[path])
+    E.extend_registers(120)
+    try:
+        need = E.extend_workspace(b.caches, b.new, getattr(E, "EAKV_" + dtype.upper()), 8)
+        got, lse = run(gpu, b, 0, q, dtype, 8)
+        assert need >= 0 and np.array_equal(got, want) and np.array_equal(lse, wl)
+    finally:
+        E.extend_registers(0)
+    again, _ = run(gpu, b, 0, q, dtype, 8)
+    assert np.array_equal(again, here) and not np.array_equal(again, got)
+    b.free()
