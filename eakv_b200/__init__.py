@@ -91,6 +91,7 @@ SIGNATURES = {
     "eakv_cache_dequantize": (_I, [_P, _I, _I, _I, _I, _P]),
     "eakv_append_rotary": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
     "eakv_extend_attention": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _I, _P, _P, _P, _c.c_size_t, _P]),
+    "eakv_extend_attention_depths": (_I, [_P, _I, _I, _P, _P, _P, _I, _F, _I, _P, _P, _P, _P, _c.c_size_t, _P]),
     "eakv_extend_workspace": (_I, [_P, _I, _P, _I, _I, _I, _I, _c.POINTER(_c.c_size_t)]),
     "eakv_cache_copy": (_I, [_P, _I, _I, _P, _I, _I, _P]),
     "eakv_cache_fork": (_I, [_P, _I, _I, _c.POINTER(_P)]),
@@ -552,28 +553,33 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
                                            nq, rot, stream), "eakv_append_rotary")
 
 
-def extend_workspace(caches, counts, dtype, n_q_heads, window=0, tree=False):
+def extend_workspace(caches, counts, dtype, n_q_heads, window=0, tree=False, depth=False):
     """Bytes of workspace eakv_extend_attention takes for this call; dtype is
-    EAKV_F32, EAKV_F16 or EAKV_BF16."""
+    EAKV_F32, EAKV_F16 or EAKV_BF16; tree, depth: whether they are given."""
     out = ctypes.c_size_t()
     hs, n_new = _handle_array(caches), _ints(counts, len(caches), "counts")
     _check(lib().eakv_extend_workspace(_address(hs), len(caches), _address(n_new), dtype, n_q_heads, window,
-                                       int(bool(tree)), ctypes.byref(out)), "eakv_extend_workspace")
+                                       2 if depth else int(bool(tree)), ctypes.byref(out)),
+           "eakv_extend_workspace")
     return out.value
 
 
 def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=None, scale=0.0,
-                     workspace=None, stream=None):
+                     workspace=None, stream=None, depth=None):
     """eakv_extend_attention. q, out: [total, n_q_heads, head_dim] (any token
     and head stride); tree: int64 or uint64 [total] bit masks over the cache's
     new tokens; lse: f32 [total, n_q_heads]; workspace: a uint8 tensor, zeroed
-    once, or None for the first cache's scratch."""
+    once, or None for the first cache's scratch. depth: int32 [total], each tree
+    token's number of ancestors, by which a window goes in place of slots
+    (eakv_extend_attention_depths)."""
     c, counts = caches[0], list(counts)
     total, nq = sum(counts), q.shape[1]
     rq, ro = _rows(q, c, nq, total, "q"), _rows(out, c, nq, total, "out")
     if tree is not None:
         kind = "uint64" if _name(tree) == "uint64" else "int64"
         _contiguous(tree, c, kind, (total,), "tree")
+    if depth is not None:
+        _contiguous(depth, c, "int32", (total,), "depth")
     if lse is not None:
         _contiguous(lse, c, "float32", (total, nq), "lse")
     size = 0
@@ -581,9 +587,9 @@ def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=Non
         size = workspace.numel()
         _contiguous(workspace, c, "uint8", (size,), "workspace")
     hs, n_new = _handle_array(caches), _ints(counts, len(caches), "counts")
-    return _check(lib().eakv_extend_attention(_address(hs), len(caches), layer, _address(n_new), rq, ro, nq,
-                                              scale, window, _ptr(tree), _ptr(lse), _ptr(workspace), size,
-                                              stream), "eakv_extend_attention")
+    return _check(lib().eakv_extend_attention_depths(
+        _address(hs), len(caches), layer, _address(n_new), rq, ro, nq, scale, window, _ptr(tree),
+        _ptr(depth), _ptr(lse), _ptr(workspace), size, stream), "eakv_extend_attention")
 
 
 def copy_positions(dsts, dst_pos, src, src_pos, n, stream=None):

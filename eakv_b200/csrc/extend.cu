@@ -66,7 +66,7 @@ int sm_count(int dev) {
 
 // The caches of `t` that belong to the part, their row tiles, splits and record
 // bytes. Call with the caches' device current.
-int plan_part(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, bool many_ok, bool umma,
+int plan_part(const ExtendArgs &a, const TokenBatch &t, int device, int tree, bool many_ok, bool umma,
               Part &p) {
   p.umma = umma;
   p.tile_rows = kExtendUmmaRows;
@@ -181,7 +181,7 @@ int plan_part(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, b
 
 // Both parts of a call: the caches with many rows, which the tcgen05 kernel takes where
 // it can, and the others.
-int plan(const ExtendArgs &a, const TokenBatch &t, int device, bool tree, Part (&p)[2]) {
+int plan(const ExtendArgs &a, const TokenBatch &t, int device, int tree, Part (&p)[2]) {
   const bool many_ok = a.dtype != EAKV_F32 && t_force_path != 2 &&
                        extend_umma_usable(a.geom.gpd * 64, a.dtype);
   int rc = plan_part(a, t, device, tree, many_ok, true, p[0]);
@@ -244,7 +244,7 @@ int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const
   if (rc || total == 0) return rc;
   DeviceGuard g(caches[0]->device);
   Part p[2];
-  rc = plan(a, b, caches[0]->device, tree != 0, p);
+  rc = plan(a, b, caches[0]->device, tree == 2 ? kTreeDepths : tree ? kTree : kCausal, p);
   if (!rc) *bytes = workspace_of(a, p);
   return rc;
 }
@@ -253,6 +253,15 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
                           const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
                           int n_q_heads, float scale, int window, const uint64_t *tree, float *lse,
                           void *workspace, size_t workspace_bytes, void *stream) {
+  return eakv_extend_attention_depths(caches, n_caches, layer, n_new, q, out, n_q_heads, scale, window,
+                                      tree, nullptr, lse, workspace, workspace_bytes, stream);
+}
+
+int eakv_extend_attention_depths(const eakv_cache_t *const *caches, int n_caches, int layer,
+                                 const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
+                                 int n_q_heads, float scale, int window, const uint64_t *tree,
+                                 const int32_t *depth, float *lse, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
   clear_error();
   ExtendArgs a;
   TokenBatch b;
@@ -267,13 +276,16 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
   if (q->dtype != out->dtype) return refuse("q and out differ in element type");
   if (layer < 0 || layer >= c0->n_layers) return refuse("layer out of range");
   if (!(fabsf(scale) <= 3.0e38f)) return refuse("scale is not a finite number");
-  if ((uintptr_t)tree % 8 || (uintptr_t)lse % 4) return refuse("misaligned tree or lse");
+  if ((uintptr_t)tree % 8 || (uintptr_t)lse % 4 || (uintptr_t)depth % 4)
+    return refuse("misaligned tree, depth or lse");
+  if (depth && !tree) return refuse("depths without a tree");
   if ((uintptr_t)workspace % 16) return refuse("workspace must be 16-byte aligned");
   a.layer = layer;
   a.q = rows_of(q);
   a.out = rows_of(out);
   a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)c0->head_dim) : scale) * kLog2e;
   a.tree = (const unsigned long long *)tree;
+  a.depth = depth;
   a.lse = lse;
   a.wait_budget = t_wait_budget ? t_wait_budget : kWaitBudget;
   a.test_stall = t_test_stall;
@@ -281,7 +293,7 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
   a.status = device_status_ptr();
   if (!a.status) return refuse("device status word unavailable");
   Part p[2];
-  rc = plan(a, b, c0->device, tree != nullptr, p);
+  rc = plan(a, b, c0->device, tree ? (depth ? kTreeDepths : kTree) : kCausal, p);
   if (rc) return rc;
   cudaStream_t s = stream ? (cudaStream_t)stream : c0->stream;
   const size_t need = workspace_of(a, p);

@@ -48,6 +48,7 @@ struct ExtendArgs {
   int n_splits, split_units;
   unsigned *cnt;             // counters of cut items, zero between calls
   float *part_o, *part_m, *part_l;   // records [slot][row of the tile]...
+  const int32_t *depth;      // of a tree's tokens, or NULL: their slots
 };
 
 // The caches of one launch, all with new tokens. (What one cache needs lies
@@ -71,15 +72,18 @@ struct ExtendRuns {
   int2 start[kMaxRuns];
 };
 
+// Masks of the new tokens: none, a tree's, a tree's with depths that windows go by.
+enum { kCausal = 0, kTree = 1, kTreeDepths = 2 };
+
 // Positions [lo, hi) that some row of rows [row0, row0 + rows) of a cache may
-// attend, and the pages that hold them.
+// attend, and the pages that hold them. (A depth may be anything up to the slot.)
 struct ExtRange {
   int lo, hi, pg0, pages;
 };
 __host__ __device__ inline ExtRange extend_range(int row0, int rows, int G, int old, int n_new,
-                                                 int window, bool tree) {
+                                                 int window, int tree) {
   ExtRange r;
-  const int t_first = row0 / G, t_last = (row0 + rows - 1) / G;
+  const int t_first = tree == kTreeDepths ? 0 : row0 / G, t_last = (row0 + rows - 1) / G;
   r.lo = window > 0 && old + t_first + 1 > window ? old + t_first + 1 - window : 0;
   r.hi = tree ? old + n_new : old + t_last + 1;
   r.pg0 = r.lo / kPagePositions;
@@ -155,7 +159,8 @@ struct ExtWalk {
       it.n_new = c.n_new;
       it.row0 = (tile - c.tile0) * a.tile_rows;
       it.rows = min(a.tile_rows, it.n_new * a.G - it.row0);
-      const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window, a.tree != nullptr);
+      const ExtRange r = extend_range(it.row0, it.rows, a.G, it.old, it.n_new, a.window,
+                                      a.tree ? (a.depth ? kTreeDepths : kTree) : kCausal);
       const int t_first = it.row0 / a.G, t_last = (it.row0 + it.rows - 1) / a.G;
       it.lo = r.lo;
       it.hi = r.hi;
@@ -233,7 +238,7 @@ struct RowMask {
   }
 };
 
-// Mask of row r of the (cache, KV head); rows behind the last repeat it.
+// Mask of row r of the (cache, KV head), but for depths; rows behind the last repeat it.
 __device__ __forceinline__ RowMask row_mask(const ExtendArgs &a, const ExtItem &it, int r) {
   RowMask m;
   const int t = min(r, it.n_new * a.G - 1) / a.G;
@@ -247,6 +252,25 @@ __device__ __forceinline__ RowMask row_mask(const ExtendArgs &a, const ExtItem &
     m.bits = 0;
   }
   return m;
+}
+
+// Depth of the cache's new token t: one outside [0, t] is reported and counts as t.
+__device__ __forceinline__ int token_depth(const ExtendArgs &a, const ExtItem &it, int t) {
+  const int d = __ldg(a.depth + it.tok0 + t);
+  if (d >= 0 && d <= t) return d;
+  atomicOr(a.status, kStatusBadIndex);
+  return t;
+}
+
+// The mask m of row r with its window by depths.
+__device__ __forceinline__ void depth_window(const ExtendArgs &a, const ExtItem &it, int r, RowMask &m) {
+  const int t = min(r, it.n_new * a.G - 1) / a.G;
+  // what lies in the window by its depth lies in it by its slot, depths being no larger
+  const int d = token_depth(a, it, t);
+  m.lo = max(0, it.old + d + 1 - a.window);
+  if (d >= a.window)   // new tokens may lie before the window
+    for (int j = 0; j < it.n_new; j++)
+      if (((m.bits >> j) & 1) && token_depth(a, it, j) <= d - a.window) m.bits &= ~(1ull << j);
 }
 
 // Record of row r in a slot, and the slot of part p of the item.

@@ -212,7 +212,12 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
     };
     // ---- the tile's q rows: f32 in shared memory, row maxima and group sums ------
     // (all loads, then the first pages' requests, then the stores)
-    if (threadIdx.x < R) mask_s[threadIdx.x] = row_mask(a, it, it.row0 + threadIdx.x);
+    if (threadIdx.x < R) {
+      const int r = it.row0 + threadIdx.x;
+      RowMask m = row_mask(a, it, r);
+      if (a.depth && a.window > 0) depth_window(a, it, r, m);
+      mask_s[threadIdx.x] = m;
+    }
     {
       constexpr int LOADS = QR * (HD / 4) / C::THREADS, STEP = C::THREADS / (HD / 4);
       const int r0 = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));

@@ -314,6 +314,13 @@ __device__ __forceinline__ uint32_t mask32(const RowMask &m, int c0, int end) {
   return b;
 }
 
+// Out of line: hardly any call has depths.
+__device__ __noinline__ RowMask depth_mask(const ExtendArgs &a, const ExtItem &it, int r) {
+  RowMask m = row_mask(a, it, r);
+  depth_window(a, it, r, m);
+  return m;
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ ExtendBatch batch,
@@ -643,7 +650,8 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
       meet();
       references();
       const int r_loc = 128 * mt + (threadIdx.x & 127);    // row within the item
-      const RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
+      RowMask mask = row_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
+      if (a.depth && a.window > 0) mask = depth_mask(a, it, it.row0 + min(r_loc, it.rows - 1));
       // score factor: |scale| log2 e / 2^(q exponent), with K's 2^(kref - kTop)
       float c_row = reinterpret_cast<const float *>(smem + C::ROWC)[r_loc];
       c_row *= pow2i((kref - kTop) >> 1);

@@ -246,7 +246,8 @@ int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, con
  * its own and the earlier new tokens' among them (they are appended, and not
  * yet advanced over); with window > 0 only the last `window` of those; with
  * tree (device uint64[total tokens], n_new <= 64) of the new tokens exactly
- * those j whose bit j is set in its word, within the window. Query head h reads KV
+ * those j whose bit j is set in its word, within the window (of slots: the call
+ * with depths below goes by positions). Query head h reads KV
  * head h / (n_q_heads / n_kv_heads). out gets softmax(scale q.k) v, scale
  * 1/sqrt(head_dim) when given as 0; lse (device f32[total tokens][n_q_heads],
  * or NULL) the natural-log log-sum-exp of the scaled scores. A token that
@@ -268,7 +269,20 @@ int eakv_extend_attention(const eakv_cache_t *const *caches, int n_caches, int l
                           const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
                           int n_q_heads, float scale, int window, const uint64_t *tree, float *lse,
                           void *workspace, size_t workspace_bytes, void *stream);
-/* Bytes of workspace that call needs (0: none). */
+/* The same for a tree under a sliding window, which goes by positions: token t of a
+ * cache stands at seq_len + depth[t], not at its slot seq_len + t (depth: device
+ * int32[total tokens], the number of its ancestors, 0 <= depth[t] <= t), and
+ * attends what its mask names and the cached positions, of these the last
+ * `window` up to its own: what it attends once the accepted branch is kept by
+ * eakv_cache_compact. Another depth sets status bit 2 and counts as t. depth NULL
+ * is eakv_extend_attention; depth needs a tree. */
+int eakv_extend_attention_depths(const eakv_cache_t *const *caches, int n_caches, int layer,
+                                 const int *n_new, const eakv_rows_t *q, const eakv_rows_t *out,
+                                 int n_q_heads, float scale, int window, const uint64_t *tree,
+                                 const int32_t *depth, float *lse, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+/* Bytes of workspace such a call needs (0: none); tree is 0 without masks, 1 with
+ * them, 2 with depths too. */
 int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const int *n_new,
                           int dtype, int n_q_heads, int window, int tree, size_t *bytes);
 
