@@ -392,7 +392,7 @@ int eakv_cache_gather(eakv_cache_t *dst, int dst_pos, const eakv_cache_t *src, c
                       int64_t layer_stride, int64_t head_stride, int n, void *stream) {
   clear_error();
   const char *who = "cache_gather";
-  if (!src || !index || n < 0 || layer_stride < 0 || head_stride < 0)
+  if (!src || (!index && n > 0) || n < 0 || layer_stride < 0 || head_stride < 0)
     return refuse(who, "invalid argument");
   int rc = check_units(src, who);
   if (!rc) rc = check_pair(dst, src, dst_pos, n, who);
@@ -425,7 +425,7 @@ int eakv_cache_compact(eakv_cache_t *c, int begin, const int32_t *index, int64_t
                        int64_t head_stride, int n, void *stream) {
   clear_error();
   const char *who = "cache_compact";
-  if (!c || !index || n < 0 || layer_stride < 0 || head_stride < 0 || begin < 0 ||
+  if (!c || (!index && n > 0) || n < 0 || layer_stride < 0 || head_stride < 0 || begin < 0 ||
       begin > c->seq_len || (long long)begin + n > c->max_seq_len)
     return refuse(who, "invalid argument");
   if (c->geom.gpd > 2) return refuse(who, "head_dim above 128");

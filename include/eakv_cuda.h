@@ -301,7 +301,7 @@ int eakv_cache_fork(const eakv_cache_t *src, int n, int max_seq_len, eakv_cache_
 /* Position dst_pos + j of (layer l, KV head h) of dst becomes position
  * index[l*layer_stride + h*head_stride + j] of src, j < n, for K and V; sets
  * dst's seq_len to dst_pos + n. index is device int32; a stride of 0 shares
- * one list between layers or heads. An index outside [0, src's seq_len) sets
+ * one list between layers or heads; with n == 0 it may be NULL. An index outside [0, src's seq_len) sets
  * status bit 2 and leaves its position as it was. */
 int eakv_cache_gather(eakv_cache_t *dst, int dst_pos, const eakv_cache_t *src, const int32_t *index,
                       int64_t layer_stride, int64_t head_stride, int n, void *stream);
