@@ -493,8 +493,9 @@ extern "C" int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int
   a.qo = rows_of(q_out);
   if (rotary) {
     if (!rotary->cos_table || !rotary->sin_table || !rotary->positions ||
-        ((uintptr_t)rotary->cos_table | (uintptr_t)rotary->sin_table) % 16)
-      return refuse("a rotary table or positions NULL, or a table not 16-byte aligned");
+        ((uintptr_t)rotary->cos_table | (uintptr_t)rotary->sin_table) % 16 ||
+        (uintptr_t)rotary->positions % 4)
+      return refuse("a rotary table or positions NULL, a table not 16-byte aligned or positions not 4-byte");
     if (rotary->rot_dim <= 0 || rotary->rot_dim % 8 != 0 || rotary->rot_dim > c0->head_dim)
       return refuse("rot_dim must be a multiple of 8 within head_dim");
     if (rotary->n_rows <= 0 || rotary->n_axes < 1 || rotary->n_axes > EAKV_MAX_AXES ||

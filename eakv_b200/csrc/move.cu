@@ -394,6 +394,7 @@ int eakv_cache_gather(eakv_cache_t *dst, int dst_pos, const eakv_cache_t *src, c
   const char *who = "cache_gather";
   if (!src || (!index && n > 0) || n < 0 || layer_stride < 0 || head_stride < 0)
     return refuse(who, "invalid argument");
+  if ((uintptr_t)index % 4) return refuse(who, "misaligned index");
   int rc = check_units(src, who);
   if (!rc) rc = check_pair(dst, src, dst_pos, n, who);
   if (rc) return rc;
@@ -428,6 +429,7 @@ int eakv_cache_compact(eakv_cache_t *c, int begin, const int32_t *index, int64_t
   if (!c || (!index && n > 0) || n < 0 || layer_stride < 0 || head_stride < 0 || begin < 0 ||
       begin > c->seq_len || (long long)begin + n > c->max_seq_len)
     return refuse(who, "invalid argument");
+  if ((uintptr_t)index % 4) return refuse(who, "misaligned index");
   if (c->geom.gpd > 2) return refuse(who, "head_dim above 128");
   if (n > 0 && c->geom.gpd > 0) {
     DeviceGuard g(c->device);

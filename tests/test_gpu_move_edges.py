@@ -36,3 +36,27 @@ def test_empty_lists(gpu, shape):
     assert (dst.seq_len, src.seq_len) == (7, 80)
     src.free()
     dst.free()
+
+
+def test_misaligned_lists_and_positions_are_refused(gpu):
+    """An address that is no multiple of 4 is refused on the host."""
+    import torch
+    L = E.lib()
+    src, dst = make(1, 2, 64, 100, 90), make(1, 2, 64, 100, 20)
+    room = torch.zeros(64, dtype=torch.int32, device=gpu)
+    x = torch.zeros(4, 2, 64, device=gpu)
+    tab = torch.ones(8, 32, device=gpu)
+    rows = E._Rows(x.data_ptr(), 128, 64, E.EAKV_F32)
+    hs, n = (ctypes.c_void_p * 1)(dst.h), (ctypes.c_int * 1)(4)
+    for off in (1, 2, 3):
+        at = room.data_ptr() + off
+        assert L.eakv_cache_gather(dst.h, 0, src.h, at, 0, 0, 4, None) == E.EAKV_ERR_INVALID
+        assert L.eakv_cache_compact(src.h, 0, at, 0, 0, 4, None) == E.EAKV_ERR_INVALID
+        rot = E._Rotary(tab.data_ptr(), tab.data_ptr(), 8, 64, 0, at, 0, 1, (ctypes.c_int * 4)(32, 0, 0, 0))
+        assert L.eakv_append_rotary(hs, 1, 0, n, ctypes.byref(rows), ctypes.byref(rows), None, None, 2,
+                                    ctypes.byref(rot), None) == E.EAKV_ERR_INVALID
+        assert "misaligned" in E.last_error()[1] or "4-byte" in E.last_error()[1]
+    assert (src.seq_len, dst.seq_len) == (90, 20)
+    src.free()
+    dst.free()
+    assert E.device_status(0) == 0
