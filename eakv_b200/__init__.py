@@ -623,6 +623,8 @@ def read_positions(caches, begins, counts, out, layer=0, stream=None):
     layers, kv, tok, head, last = out.stride()
     if last != 1:
         raise ValueError("out: the last dim must be contiguous")
+    if kv < c.shape[2]:
+        raise ValueError("out: K and V overlap")
     _on(out, c, "out")
     code, at = _dtype(out), out.data_ptr()
     hs, begin = _handle_array(caches), _ints(begins, len(caches), "begins")

@@ -423,6 +423,18 @@ int check_rows(const eakv_rows_t *r, const char *name, const char *who) {
   return EAKV_OK;
 }
 
+int check_out_rows(const eakv_rows_t *r, const char *name, const char *who, int tokens, int heads,
+                   int head_dim) {
+  int rc = check_rows(r, name, who);
+  if (rc) return rc;
+  if ((tokens > 1 && r->token_stride < head_dim) || (heads > 1 && r->head_stride < head_dim)) {
+    set_error(EAKV_ERR_INVALID, "%s: %s rows overlap (token stride %lld, head stride %lld)", who, name,
+              (long long)r->token_stride, (long long)r->head_stride);
+    return EAKV_ERR_INVALID;
+  }
+  return EAKV_OK;
+}
+
 int token_batch(const eakv_cache_t *const *caches, int n_caches, int n_q, const int *pos0,
                 const int *n, const char *who, TokenBatch &b, int &total) {
   int rc = check_batch(caches, n_caches, n_q, who);
@@ -473,7 +485,9 @@ extern "C" int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int
   if ((rc = check_rows(k, "k", who)) || (rc = check_rows(v, "v", who))) return rc;
   if (layer < 0 || layer >= caches[0]->n_layers) return refuse("layer out of range");
   if (!q != !q_out) return refuse("q and q_out go together");
-  if (q && ((rc = check_rows(q, "q", who)) || (rc = check_rows(q_out, "q_out", who)))) return rc;
+  if (q && ((rc = check_rows(q, "q", who)) ||
+            (rc = check_out_rows(q_out, "q_out", who, a.total, n_q_heads, caches[0]->head_dim))))
+    return rc;
   if (v->dtype != k->dtype || (q && (q->dtype != k->dtype || q_out->dtype != k->dtype)))
     return refuse("k, v, q and q_out differ in element type");
   // the same cache twice would write the same positions twice

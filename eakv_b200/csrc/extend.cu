@@ -269,10 +269,10 @@ int eakv_extend_attention_depths(const eakv_cache_t *const *caches, int n_caches
   if (!q || !out) return refuse("NULL q or out");
   int rc = check_call(caches, n_caches, n_new, q->dtype, n_q_heads, window, tree != nullptr, a, b, total);
   if (rc || total == 0) return rc;
-  if ((rc = check_rows(q, "q", "extend_attention")) ||
-      (rc = check_rows(out, "out", "extend_attention")))
-    return rc;
   const eakv_cache_t *c0 = caches[0];
+  if ((rc = check_rows(q, "q", "extend_attention")) ||
+      (rc = check_out_rows(out, "out", "extend_attention", total, n_q_heads, c0->head_dim)))
+    return rc;
   if (q->dtype != out->dtype) return refuse("q and out differ in element type");
   if (layer < 0 || layer >= c0->n_layers) return refuse("layer out of range");
   if (!(fabsf(scale) <= 3.0e38f)) return refuse("scale is not a finite number");

@@ -466,11 +466,14 @@ int eakv_cache_read(const eakv_cache_t *const *caches, int n_caches, int layer0,
   int rc = token_batch(caches, n_caches, c0->n_kv_heads, begin, n, who, b, a.total);
   if (rc || a.total == 0) return rc;
   if (!k && !v) return refuse(who, "neither k nor v");
-  if ((k && (rc = check_rows(k, "k", who))) || (v && (rc = check_rows(v, "v", who)))) return rc;
+  if ((k && (rc = check_out_rows(k, "k", who, a.total, c0->n_kv_heads, c0->head_dim))) ||
+      (v && (rc = check_out_rows(v, "v", who, a.total, c0->n_kv_heads, c0->head_dim))))
+    return rc;
   if (k && v && k->dtype != v->dtype) return refuse(who, "k and v differ in element type");
   if (layer0 < 0 || n_layers < 1 || (long long)layer0 + n_layers > c0->n_layers || n_layers > 32767 ||
       layer_stride < 0)
     return refuse(who, "layers out of range");
+  if (n_layers > 1 && layer_stride < c0->head_dim) return refuse(who, "layers' rows overlap");
   DeviceGuard g(c0->device);
   a.geom = c0->geom;
   a.n_caches = n_caches;

@@ -94,5 +94,8 @@ int token_batch(const eakv_cache_t *const *caches, int n_caches, int n_q, const 
                 const int *n, const char *who, TokenBatch &b, int &total);
 // A rows argument: pointer, element type, strides that are not negative.
 int check_rows(const eakv_rows_t *r, const char *name, const char *who);
+// The same of rows that are written: neighbouring ones may not overlap.
+int check_out_rows(const eakv_rows_t *r, const char *name, const char *who, int tokens, int heads,
+                   int head_dim);
 
 }  // namespace eakv

@@ -196,7 +196,9 @@ int eakv_cache_dequantize(const eakv_cache_t *cache, int layer, int kv_idx, int 
 
 /* Rows [token][head][head_dim] of a device buffer: element d of (token t,
  * head h) is at data + t*token_stride + h*head_stride + d (strides in
- * elements), so a slice of a fused q/k/v projection needs no copy. Rows that
+ * elements), so a slice of a fused q/k/v projection needs no copy. Rows that are
+ * read may overlap (a stride of 0 broadcasts one); of rows that are written a stride
+ * below head_dim is refused where there is more than one row along it. Rows that
  * do not start on a 4-element boundary are read and written one element at a
  * time. */
 typedef struct {

@@ -60,3 +60,42 @@ def test_misaligned_lists_and_positions_are_refused(gpu):
     src.free()
     dst.free()
     assert E.device_status(0) == 0
+
+
+def test_outputs_that_overlap_are_refused(gpu):
+    """A broadcast tensor as an output would be written by several rows at once; as an input it is
+    one row for all."""
+    import torch
+    c = make(2, 2, 64, 40, 20)
+    n, H, G, hd = 3, 2, 2, 64
+    k = torch.randn(n, H, hd, device=gpu)
+    q = torch.randn(n, H * G, hd, device=gpu)
+    tab = torch.ones(8, 32, device=gpu)
+    pos = torch.zeros(n, dtype=torch.int32, device=gpu)
+    turn = dict(cos=tab, sin=tab * 0, positions=pos)
+    one_token, one_head = torch.zeros(1, H * G, hd, device=gpu), torch.zeros(n, 1, hd, device=gpu)
+    near = torch.zeros(n * H * G * 8 + hd, device=gpu).as_strided((n, H * G, hd), (H * G * 8, 8, 1))
+    bad = [one_token.expand(n, -1, -1), one_head.expand(-1, H * G, -1), near]
+    for out in bad:
+        with pytest.raises(E.EakvError, match="overlap"):
+            E.append_rotary([c], 0, [n], k, k, q=q, q_out=out, **turn)
+        with pytest.raises(E.EakvError, match="overlap"):
+            E.extend_attention([c], 0, [n], q, out)
+    out = torch.zeros(2, 2, n, H, hd, device=gpu)
+    for dim in range(4):
+        with pytest.raises((E.EakvError, ValueError), match="overlap"):
+            E.read_positions([c], [0], [n], out[(slice(None),) * dim + (slice(0, 1),)].expand(out.shape))
+    # as inputs, and where there is one row along the stride
+    torch.cuda.synchronize()
+    E.append_rotary([c], 0, [n], k[:1].expand(n, -1, -1), k[:, :1].expand(-1, H, -1), q=q, **turn)
+    E.extend_attention([c], 0, [n], one_token.expand(n, -1, -1), q)
+    E.extend_attention([c], 0, [1], q[:1], one_token.as_strided((1, H * G, hd), (0, hd, 1)))
+    E.read_positions([c], [0], [1], torch.zeros(2, H * hd, device=gpu).as_strided((1, 2, 1, H, hd), (0, H * hd, 0, hd, 1)))
+    c.synchronize()
+    got = torch.zeros(1, 2, n, H, hd, device=gpu)
+    torch.cuda.synchronize()
+    E.read_positions([c], [20], [n], got)
+    c.synchronize()
+    assert torch.equal(got[0, 0, 0], got[0, 0, 1]) and torch.equal(got[0, 1, :, 0], got[0, 1, :, 1])
+    c.free()
+    assert E.device_status(0) == 0
