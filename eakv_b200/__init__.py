@@ -255,8 +255,9 @@ class Cache:
     def fork(self, n, max_seq_len=None):
         """eakv_cache_fork: a new cache holding the first n positions."""
         out = ctypes.c_void_p()
-        _check(lib().eakv_cache_fork(self.h, n, max_seq_len or self.max_seq_len, ctypes.byref(out)),
-               "eakv_cache_fork")
+        if max_seq_len is None:
+            max_seq_len = self.max_seq_len
+        _check(lib().eakv_cache_fork(self.h, n, max_seq_len, ctypes.byref(out)), "eakv_cache_fork")
         return Cache(_handle=out.value)
 
     def compact(self, begin, index, stream=None):
