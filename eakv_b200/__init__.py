@@ -528,7 +528,10 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
     rk, rv = _rows(k, c, nkv, total, "k"), _rows(v, c, nkv, total, "v")
     rq, ro = _rows(q, c, nq, total, "q"), _rows(q_out, c, nq, total, "q_out")
     rot = None
-    if cos is not None:
+    if cos is None or sin is None or positions is None:
+        if not cos is sin is positions is None:
+            raise ValueError("cos, sin and positions go together")
+    else:
         if positions.dim() == 1:
             positions = positions[None]
         if cos.dim() != 2 or cos.dtype != sin.dtype:

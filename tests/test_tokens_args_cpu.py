@@ -29,3 +29,17 @@ def test_fork_passes_a_capacity_of_zero_on(monkeypatch):
         with pytest.raises(E.EakvError):
             c.fork(3, size)
     assert asked == [0, 77, 5, -1]
+
+
+class Host:
+    """A cache as the argument checks see one, on the host."""
+    h, shape = 0, (2, 4, 64, -1)
+
+
+def test_rotary_tables_and_positions_go_together():
+    import torch
+    x, tab, pos = torch.zeros(3, 4, 64), torch.zeros(8, 32), torch.zeros(3, dtype=torch.int32)
+    whole = dict(cos=tab, sin=tab, positions=pos)
+    for given in (["cos"], ["sin"], ["positions"], ["cos", "sin"], ["cos", "positions"], ["sin", "positions"]):
+        with pytest.raises(ValueError, match="together"):
+            E.append_rotary([Host()], 0, [3], x, x, **{k: whole[k] for k in given})
