@@ -43,3 +43,14 @@ def test_rotary_tables_and_positions_go_together():
     for given in (["cos"], ["sin"], ["positions"], ["cos", "sin"], ["cos", "positions"], ["sin", "positions"]):
         with pytest.raises(ValueError, match="together"):
             E.append_rotary([Host()], 0, [3], x, x, **{k: whole[k] for k in given})
+
+
+def test_packed_arguments_are_the_structures():
+    """The calls pass eakv_rows_t and eakv_rotary_t as packed bytes: the same bytes as the ctypes structures,
+    whose layout is the header's."""
+    import ctypes
+    rows = (2 ** 63 + 16, 2 ** 40 + 3, 2 ** 33, E.EAKV_BF16)
+    assert E._pack_rows(*rows) == bytes(E._Rows(*rows))
+    rot = (2 ** 63 + 32, 2 ** 62, 7, 128, 1, 2 ** 61 + 4, 2 ** 35, 3, 20, 30, 14, 0)
+    packed = E._pack_rotary(*rot)
+    assert packed == bytes(E._Rotary(*rot[:8], (ctypes.c_int * 4)(*rot[8:])))
