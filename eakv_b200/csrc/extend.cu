@@ -275,7 +275,8 @@ int eakv_extend_attention_depths(const eakv_cache_t *const *caches, int n_caches
     return rc;
   if (q->dtype != out->dtype) return refuse("q and out differ in element type");
   if (layer < 0 || layer >= c0->n_layers) return refuse("layer out of range");
-  if (!(fabsf(scale) <= 3.0e38f)) return refuse("scale is not a finite number");
+  // 2.3e38 log2 e is the last one below f32's largest number
+  if (!(fabsf(scale) <= 2.3e38f)) return refuse("scale is not a number below 2.3e38");
   if ((uintptr_t)tree % 8 || (uintptr_t)lse % 4 || (uintptr_t)depth % 4)
     return refuse("misaligned tree, depth or lse");
   if (depth && !tree) return refuse("depths without a tree");

@@ -123,3 +123,15 @@ def test_the_widest_batch(gpu):
     for c in many + alone:
         c.free()
     assert E.device_status(0) == 0
+
+
+def test_scales_that_leave_f32_are_refused(gpu):
+    """A scale whose base-2 form is infinite, or that is no number."""
+    import torch
+    c = E.Cache(1, 1, 64, 20)
+    assert c.advance(18) == 0
+    q = torch.ones(2, 2, 64, device=gpu)
+    for scale in (3e38, -3e38, 2.4e38, float("inf"), float("nan")):
+        with pytest.raises(E.EakvError, match="scale"):
+            E.extend_attention([c], 0, [2], q, torch.empty_like(q), scale=scale)
+    c.free()
