@@ -43,6 +43,18 @@ constexpr int kTileCost[3] = {10, 16, 21};
 constexpr int kLeastPages = 6, kLeastTiles = 4;
 constexpr int kOverheadPages = 6, kOverheadTiles = 5;
 
+// What the cuts of a balanced run cost a CTA, its records and merges: in pages of the
+// warp-level kernel, in tiles of the tcgen05 kernel per 64 dims of the head.
+// Measured in runs / as whole items, us (8 KV heads, 32 query heads):
+// 512-token prompts of the tcgen05 kernel, head_dim 128, at 1.7, 3.0, 4.3 items per CTA:
+// no earlier positions 62/45, 90/70, 120/102; 2048 of them 141/111, 214/207, 304/277;
+// 8192: 328/324, 590/639, 834/802 (at 2.2 403/475); head_dim 64: 45/35, 64/52, 82/72;
+// 102/96, 158/173, 215/225; 257/277, 437/540, 613/685. Single tokens of the warp-level
+// kernel, head_dim 128, at 1.2, 2.3, 3.5 items per CTA: 512 positions 33/31, 49/47, 72/63;
+// 2048: 59/60, 103/95, 147/135; head_dim 64, at 1.3, 2.2, 3.5: 27/26, 41/38, 58/52; 54/49,
+// 75/72, 115/102.
+constexpr int kCutPages = 28, kCutTiles = 14;
+
 // Parts of an item, at most: a merge keeps two words of each in shared memory.
 constexpr int kMaxParts = 4096;
 
@@ -137,15 +149,19 @@ int plan_part(const ExtendArgs &a, const TokenBatch &t, int device, int tree, bo
   const long long resident = (long long)per_sm * sm_count(device), items = tiles * heads;
   long long run = (units + resident - 1) / resident;
   if (run < least + overhead) run = least + overhead;
-  // splits that fit on the GPU at once, against a run
+  // splits that fit on the GPU at once, no longer than a run
   long long fit = resident / items;
   if (fit > max_units / least) fit = max_units / least;
   if (fit < 1) fit = 1;
-  // or whole items, where there are enough of them for the last to end together
-  // (at 4.5 items per CTA 136 us against 187 in runs, at 1.7 1.14 ms against 1.05)
-  const bool even = (items * fit <= resident && (max_units + fit - 1) / fit + overhead <= run + run / 8 &&
-                     (max_units + fit - 1) / fit <= cap) ||
-                    (items >= 4 * resident && max_units <= cap);
+  const bool splits = items * fit <= resident && (max_units + fit - 1) / fit + overhead <= run + run / 8 &&
+                      (max_units + fit - 1) / fit <= cap;
+  // or whole items, where the last round's idle CTAs cost less than the cuts of runs:
+  // rounds of the mean item, and what the longest has beyond it, against a run
+  const double mean = (double)units / items, rounds = (double)((items + resident - 1) / resident);
+  const bool whole = max_units <= cap && rounds * mean + (max_units + overhead - mean) <=
+                                             run + (umma ? kCutTiles * a.geom.gpd : kCutPages);
+  const bool even = splits || whole;
+  if (!splits) fit = 1;
   if (t_force_splits == 0 && !even && run <= cap && (units + run - 1) / run <= kMaxRuns) {
     p.overhead = overhead;
     p.units = units;
@@ -275,7 +291,7 @@ int eakv_extend_attention_depths(const eakv_cache_t *const *caches, int n_caches
     return rc;
   if (q->dtype != out->dtype) return refuse("q and out differ in element type");
   if (layer < 0 || layer >= c0->n_layers) return refuse("layer out of range");
-  // 2.3e38 log2 e is the last one below f32's largest number
+  // 2.3e38 log2 e is below f32's largest number
   if (!(fabsf(scale) <= 2.3e38f)) return refuse("scale is not a number below 2.3e38");
   if ((uintptr_t)tree % 8 || (uintptr_t)lse % 4 || (uintptr_t)depth % 4)
     return refuse("misaligned tree, depth or lse");

@@ -135,3 +135,36 @@ def test_scales_that_leave_f32_are_refused(gpu):
         with pytest.raises(E.EakvError, match="scale"):
             E.extend_attention([c], 0, [2], q, torch.empty_like(q), scale=scale)
     c.free()
+
+
+@pytest.mark.parametrize("hd,caches,new,old", [(128, 4, 130, 0), (128, 5, 130, 700), (64, 9, 129, 300),
+                                               (64, 12, 129, 3000), (128, 96, 1, 600), (64, 200, 1, 100)])
+def test_plans_agree(gpu, hd, caches, new, old):
+    """Batches that are cut into runs, into whole items or into one part each give the same results to
+    twice the output's half step."""
+    import torch
+    H, nq = 8, 32
+    group = []
+    for i in range(caches):
+        c = E.Cache(1, H, hd, old + new)
+        g = torch.Generator(device=gpu).manual_seed(i)
+        raw = torch.randn(1, 2, H, old + new, hd, generator=g, device=gpu)
+        torch.cuda.synchronize()
+        assert c.load_raw_device(raw, old + new) == 0
+        c.synchronize()
+        assert c.restore(old) == 0
+        group.append(c)
+    q = torch.randn(caches * new, nq, hd, device=gpu).bfloat16()
+    outs = []
+    for splits in (0, 1, 3):
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        E.force_splits(splits)
+        E.extend_attention(group, 0, [new] * caches, q, out)
+        group[0].synchronize()
+        outs.append(out.float())
+    for o in outs[1:]:
+        assert ((o - outs[0]).abs() <= 2.0 ** -7 * outs[0].abs() + 2.0 ** -9).all()
+    for c in group:
+        c.free()
+    assert E.device_status(0) == 0
