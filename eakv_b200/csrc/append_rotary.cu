@@ -40,7 +40,6 @@ constexpr int kPasses = 2;    // sets of 512 elements per warp, at most
 struct RotaryArgs {
   PageGeom geom;
   int n_caches, layer, n_q, n_kv, total, tokens_y;
-  int head_dim;
   Rows q, k, v, qo;
   const float *cos_t, *sin_t;
   int n_rows, pairs, interleaved, n_axes;
@@ -498,7 +497,6 @@ extern "C" int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int
   a.geom = c0->geom;
   a.n_caches = n_caches;
   a.layer = layer;
-  a.head_dim = c0->head_dim;
   a.n_kv = n_kv;
   a.n_q = q ? n_q_heads : 0;
   a.k = rows_of(k);

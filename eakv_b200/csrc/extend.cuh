@@ -273,6 +273,18 @@ __device__ __forceinline__ void depth_window(const ExtendArgs &a, const ExtItem 
       if (((m.bits >> j) & 1) && token_depth(a, it, j) <= d - a.window) m.bits &= ~(1ull << j);
 }
 
+// (w & mask) | magic
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
+}
+// Two values as f16 in one word.
+__device__ __forceinline__ uint32_t pack_f16(float x0, float x1) {
+  const __half2 h = __floats2half2_rn(x0, x1);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // Record of row r in a slot, and the slot of part p of the item.
 __device__ __forceinline__ size_t part_row(const ExtendArgs &a, int slot, int r) {
   return (size_t)slot * a.tile_rows + r;

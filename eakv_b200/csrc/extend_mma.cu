@@ -77,11 +77,6 @@ struct XCfg {
   static_assert(MAIN % 16 == 0 && FRAGOFF % 16 == 0 && sizeof(RowMask) <= 32, "alignment");
 };
 
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-  return r;
-}
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t x, uint32_t y) {
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
@@ -100,10 +95,6 @@ __device__ __forceinline__ uint32_t nib_hi(uint32_t w) {
 // High nibbles of bytes 0 and 2 with the offset left in: 1024 + 16 n = 16 (64 + n).
 __device__ __forceinline__ uint32_t raw_hi(uint32_t w) { return and_or(w, 0x00F000F0u, 0x64006400u); }
 
-__device__ __forceinline__ uint32_t pack_f16(float x0, float x1) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
 // x - f16(x) of both halves, as f16
 __device__ __forceinline__ uint32_t pack_rest(float x0, float x1, uint32_t hi) {
   const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));

@@ -154,16 +154,8 @@ __host__ __device__ constexpr uint32_t idesc_f16(int N, int b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-  return r;
-}
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
-__device__ __forceinline__ uint32_t pack_f16(float x0, float x1) {
-  return as_u32(__floats2half2_rn(x0, x1));
-}
 __device__ __forceinline__ uint4 ldg_row(const void *p) {
   uint4 r;
   asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
