@@ -253,7 +253,8 @@ class Cache:
 
     # --- copies -----------------------------------------------------------------
     def fork(self, n, max_seq_len=None):
-        """eakv_cache_fork: a new cache holding the first n positions."""
+        """eakv_cache_fork: a new cache holding the first n positions, as the cache's own
+        stream leaves them (work on other streams is ordered before it by the caller)."""
         out = ctypes.c_void_p()
         if max_seq_len is None:
             max_seq_len = self.max_seq_len
@@ -263,7 +264,8 @@ class Cache:
     def compact(self, begin, index, stream=None):
         """eakv_cache_compact: position begin + j becomes position index[..., j].
         index: int32 device tensor [n], [heads, n] or [layers, heads, n] (a
-        size of 1 is shared)."""
+        size of 1 is shared). stream None is the cache's own, which is not ordered
+        with torch's current one."""
         index, ls, hs = _index(index, self)
         return _check(lib().eakv_cache_compact(self.h, begin, _ptr(index), ls, hs, index.shape[-1],
                                                stream), "eakv_cache_compact")
@@ -411,6 +413,13 @@ def decode_attention_partial(caches, d_queries, n_q_heads, pos_begin, pos_end, d
 
 
 # --- several tokens per call ------------------------------------------------------
+# Streams. Each call runs on `stream`, a CUDA stream's address; None (and 0) is the first
+# cache's own stream, in copies and gathers the source's, which waits for no other stream and
+# which torch's allocator does not know. So tensors that torch's current stream writes or
+# frees are in order with a call only if it runs there:
+# stream=torch.cuda.current_stream().cuda_stream or 1 (torch's default stream is 0, whose own
+# address is 1), or cache.set_stream() with the same once. Otherwise the caller synchronizes, or orders
+# the streams by events and keeps the tensors until the call has run.
 EAKV_F32, EAKV_F16, EAKV_BF16 = 0, 1, 2
 _DTYPES = {"float32": EAKV_F32, "float16": EAKV_F16, "bfloat16": EAKV_BF16}
 
@@ -519,7 +528,8 @@ def append_rotary(caches, layer, counts, k, v, q=None, q_out=None, cos=None, sin
     head stride), q and q_out: [total, n_q_heads, head_dim] (q_out defaults to
     q); counts[i] tokens of each cache, packed. cos, sin: f32 tables [rows,
     rot_dim/2]; positions: int32 [axes, total] (or [total]); sections: pairs
-    that follow each axis. Without tables K goes in as it is."""
+    that follow each axis. Without tables K goes in as it is. stream None is the
+    first cache's own, which is not ordered with torch's current one (see above)."""
     c, counts = caches[0], list(counts)
     total, nkv = sum(counts), c.shape[1]
     if q is not None and q_out is None:
@@ -575,7 +585,8 @@ def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=Non
     new tokens; lse: f32 [total, n_q_heads]; workspace: a uint8 tensor, zeroed
     once, or None for the first cache's scratch. depth: int32 [total], each tree
     token's number of ancestors, by which a window goes in place of slots
-    (eakv_extend_attention_depths)."""
+    (eakv_extend_attention_depths). stream None is the first cache's own, which is
+    not ordered with torch's current one (see above)."""
     c, counts = caches[0], list(counts)
     total, nq = sum(counts), q.shape[1]
     rq, ro = _rows(q, c, nq, total, "q"), _rows(out, c, nq, total, "out")
@@ -598,7 +609,8 @@ def extend_attention(caches, layer, counts, q, out, window=0, tree=None, lse=Non
 
 def copy_positions(dsts, dst_pos, src, src_pos, n, stream=None):
     """eakv_cache_copy: positions [src_pos, src_pos + n) of src to dst_pos.. of
-    every cache of dsts, whose seq_len becomes dst_pos + n."""
+    every cache of dsts, whose seq_len becomes dst_pos + n. stream None is src's own;
+    what runs on the destinations' streams is the caller's to order behind it."""
     hs = _handle_array(dsts)
     return _check(lib().eakv_cache_copy(_address(hs), len(dsts), dst_pos, src.h, src_pos, n, stream),
                   "eakv_cache_copy")
@@ -606,7 +618,8 @@ def copy_positions(dsts, dst_pos, src, src_pos, n, stream=None):
 
 def gather_positions(dst, dst_pos, src, index, stream=None):
     """eakv_cache_gather: position dst_pos + j of dst becomes position
-    index[..., j] of src. index: int32 [n], [heads, n] or [layers, heads, n]."""
+    index[..., j] of src. index: int32 [n], [heads, n] or [layers, heads, n]. stream
+    None is src's own, which is not ordered with torch's current one (see above)."""
     index, ls, hs = _index(index, src)
     return _check(lib().eakv_cache_gather(dst.h, dst_pos, src.h, _ptr(index), ls, hs, index.shape[-1],
                                           stream), "eakv_cache_gather")
@@ -615,7 +628,8 @@ def gather_positions(dst, dst_pos, src, index, stream=None):
 def read_positions(caches, begins, counts, out, layer=0, stream=None):
     """eakv_cache_read: the values of positions [begins[i], begins[i] +
     counts[i]) of each cache, into out [layers, 2, total, n_kv_heads, head_dim]
-    (layers from `layer` on; K then V)."""
+    (layers from `layer` on; K then V). stream None is the first cache's own, which
+    is not ordered with torch's current one (see above)."""
     c, counts = caches[0], list(counts)
     total = sum(counts)
     if out.dim() != 5 or out.shape[1] != 2:

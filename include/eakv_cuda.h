@@ -297,8 +297,9 @@ int eakv_extend_workspace(const eakv_cache_t *const *caches, int n_caches, const
  * own streams has to be ordered behind it by the caller. */
 int eakv_cache_copy(eakv_cache_t *const *dsts, int n_dst, int dst_pos, const eakv_cache_t *src,
                     int src_pos, int n, void *stream);
-/* A new cache of max_seq_len positions on src's device with src's first n. Not
- * for stream capture (it allocates). */
+/* A new cache of max_seq_len positions on src's device with src's first n, copied on
+ * src's own stream, behind which the new cache's starts. Not for stream capture
+ * (it allocates). */
 int eakv_cache_fork(const eakv_cache_t *src, int n, int max_seq_len, eakv_cache_t **out);
 /* Position dst_pos + j of (layer l, KV head h) of dst becomes position
  * index[l*layer_stride + h*head_stride + j] of src, j < n, for K and V; sets
