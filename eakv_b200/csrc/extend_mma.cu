@@ -606,6 +606,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           float *s = reinterpret_cast<float *>(page + C::NIB + 8 * (x % (kPagePositions * NG)));
           if (*s == 1.0f && constant_group(page, x % (kPagePositions * NG))) *s = 0.0f;
         }
+        fence_proxy_async_smem();   // ahead of the copy that fills the stage next
         __syncwarp();
       }
       if (full) {
