@@ -254,7 +254,9 @@ int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, con
  * 1/sqrt(head_dim) when given as 0; lse (device f32[total tokens][n_q_heads],
  * or NULL) the natural-log log-sum-exp of the scaled scores. A token that
  * attends nothing gets zeros and -inf. What is not attended has no influence,
- * NaN among it. q and out have one element type, and sums are f32. f32 runs on
+ * NaN among it. q and out have one element type, and out may be q itself (an
+ * item's rows are read by all its parts before one of them is written); sums
+ * are f32. f32 runs on
  * split operands that keep 22 bits, at any number of rows; a 16-bit type on one
  * f16 operand each: with up to 32 rows (new tokens x query heads) per KV head
  * the cache's values enter exactly, with more each is rounded to f16, which puts

@@ -37,6 +37,7 @@ def test_a_captured_step(gpu, new, dtype):
 
     mine, eager = batch(), batch()
     tab = torch.rand(64, hd // 2, device=gpu)
+    sin = 1 - tab   # made here: on torch's stream it would not be ordered with the calls'
     pos = torch.randint(0, 64, (total,), dtype=torch.int32, device=gpu)
 
     def buffers():
@@ -47,7 +48,7 @@ def test_a_captured_step(gpu, new, dtype):
 
     def step(caches, b, stream, ws):
         x = b["x"]
-        E.append_rotary(caches, 0, new, x[:, nq:nq + H], x[:, nq + H:], x[:, :nq], b["q"], tab, 1 - tab, pos,
+        E.append_rotary(caches, 0, new, x[:, nq:nq + H], x[:, nq + H:], x[:, :nq], b["q"], tab, sin, pos,
                         stream=stream)
         E.extend_attention(caches, 0, new, b["q"], b["o"], workspace=ws, stream=stream)
         E.read_positions(caches, old, new, b["kv"], stream=stream)
@@ -165,6 +166,34 @@ def test_plans_agree(gpu, hd, caches, new, old):
         outs.append(out.float())
     for o in outs[1:]:
         assert ((o - outs[0]).abs() <= 2.0 ** -7 * outs[0].abs() + 2.0 ** -9).all()
+    for c in group:
+        c.free()
+    assert E.device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("splits", [0, 1, 4])
+@pytest.mark.parametrize("hd,new", [(64, [3, 1]), (128, [150, 9, 70])])
+def test_out_may_be_q(gpu, hd, new, splits, dtype):
+    """In place, whole or cut: the bits of a call with an output of its own."""
+    import torch
+    t = getattr(torch, DT[dtype])
+    group = []
+    for i in range(len(new)):
+        c = E.Cache(1, 2, hd, 2000)
+        assert c.load_raw(kv_data(np.random.default_rng(i), 1, 2, 1500, hd), 1500) == 0
+        group.append(c)
+    q = torch.randn(sum(new), 8, hd, device=gpu).to(t)
+    out, own = torch.empty_like(q), q.clone()
+    torch.cuda.synchronize()
+    E.force_splits(splits)
+    for _ in range(3):
+        own.copy_(q)
+        torch.cuda.synchronize()
+        E.extend_attention(group, 0, new, q, out)
+        E.extend_attention(group, 0, new, own, own)
+        group[0].synchronize()
+        assert torch.equal(out, own)
     for c in group:
         c.free()
     assert E.device_status(0) == 0
