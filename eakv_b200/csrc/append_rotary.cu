@@ -23,11 +23,13 @@
 // per lane, sixteen lanes to a group, the reductions and the packing were ten times
 // the arithmetic: 16384 tokens of 32 + 16 heads 199-258 us.
 //
-// Bound: HBM for long chunks (q, k, v in, q out, 40 bytes per group), though the
-// keys' arithmetic in f64 and their partners' loads keep it from it; the launch
-// plus one round trip to memory (positions, then tables) for a step of single
-// tokens. Measured with cold caches, 32 + 16 heads of 128, bf16: 16384 tokens 161 us
-// (357 MB), 2048 tokens 30 us, 16 caches of one token 11 us.
+// Bound: for long chunks HBM (q, k, v in, q out, 40 bytes per group: 55 us for 16384
+// tokens of 32 + 16 heads of 128, bf16), from which it is far: 171 us with cold
+// caches, of which K and V as they are take 45, the keys' rotation (f64, their
+// partners loaded again) 32, the queries as they are 63 (0.65 of HBM's rate: positions,
+// tables and rows are a warp's one round trip, two heads' sets at a time) and their
+// rotation 31. 2048 tokens 31 us. For a step of single tokens the launch plus a round
+// trip to memory (positions, then tables): 16 caches of one token 11 us.
 #include "tokens.cuh"
 #include "pipeline.cuh"
 

@@ -16,8 +16,8 @@
 // j s + r, j whole, and s = s_hi + s_lo it is m s_hi + (m s_lo + r), m = n - 8 + j, whose first
 // product is exact and whose second term is small. With s and b + 8 s rounded to f16
 // first, one FMA less, all dims of a position are off alike, which adds up in its
-// score: outputs were off by 1.7e-3 of their size in all, now by 0.8e-3, where the rounding
-// of a bf16 output alone is 1.7e-3 and that of an f16 one 0.2e-3. In V', whose errors
+// score: f16 outputs were off by 1.3e-3 of their size in all, now by 0.7e-3, where the
+// rounding of a bf16 output alone is 1.7e-3 and that of an f16 one 0.2e-3. In V', whose errors
 // are independent from position to position, s is one f16. Keeping K's nibbles
 // exact instead needs a second accumulator per 64-dim group, for which tensor memory
 // has no room, and four more FMAs per score; f32 rows, which the warp-level kernel
@@ -53,8 +53,8 @@
 //
 // Bound: the tensor pipe, whose operands come from shared memory at its full rate
 // (S = Q'K' reads 128 bytes a cycle) next to the dequantizing stores: 2048 tokens
-// of 32 heads (8 KV heads, head_dim 128) behind 32768 positions in 1.03 ms,
-// 1.10 PFLOP/s. Tried and slower: tiles of 64 positions with two S buffers (its
+// of 32 heads (8 KV heads, head_dim 128) behind 32768 positions in 1.15 to 1.24 ms,
+// 0.91 to 0.99 PFLOP/s, box to box. Tried and slower: tiles of 64 positions with two S buffers (its
 // MMAs are 1.4 times slower per value), one pass over the scores in place of the
 // registers, exponentials by polynomial on the FMA pipe for a quarter or half of
 // them (the exponentials are not what it waits for).

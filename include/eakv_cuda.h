@@ -260,8 +260,8 @@ int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, con
  * split operands that keep 22 bits, at any number of rows; a 16-bit type on one
  * f16 operand each: with up to 32 rows (new tokens x query heads) per KV head
  * the cache's values enter exactly, with more each is rounded to f16, which puts
- * outputs 0.8e-3 of their size off in the mean where an f16 output's own
- * rounding is 0.2e-3 and a bf16 one's 1.7e-3. A caller who needs more bits there
+ * f16 outputs 0.7e-3 of their size off in the mean (0.3e-3 with few rows) and
+ * bf16 ones 1.8e-3, of which 1.7e-3 are the output's own rounding. A caller who needs more bits there
  * passes f32 rows. workspace (device, 16-byte aligned) holds the records of long rows'
  * sequence splits: at least eakv_extend_workspace bytes, zeroed once before
  * its first use, and not shared by calls that may overlap; NULL takes one that
