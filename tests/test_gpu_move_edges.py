@@ -99,3 +99,57 @@ def test_outputs_that_overlap_are_refused(gpu):
     assert torch.equal(got[0, 0, 0], got[0, 0, 1]) and torch.equal(got[0, 1, :, 0], got[0, 1, :, 1])
     c.free()
     assert E.device_status(0) == 0
+
+
+def test_captured_moves(gpu):
+    """Copy, gather and compact in one graph, replayed: each replay moves what its sources and
+    lists hold then, for the lengths that it was captured with."""
+    import torch
+    src, keep, a, b = (make(2, 2, 128, 300, 200, seed=i) for i in range(4))
+    index = torch.arange(0, 200, 2, dtype=torch.int32, device=gpu)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        E.copy_positions([a], 5, src, 10, 150, stream=s.cuda_stream)
+        E.gather_positions(b, 0, src, index, stream=s.cuda_stream)
+        keep.compact(0, index, stream=s.cuda_stream)
+    assert (a.seq_len, b.seq_len, keep.seq_len) == (155, 100, 100)
+    for step in (1, 2):
+        data = kv_data(np.random.default_rng(10 + step), 2, 2, 200, 128)
+        for c in (src, keep):
+            c.clear()
+            assert c.load_raw(data, 200) == 0
+        index.copy_(torch.arange(step, 100 + step, dtype=torch.int32, device=gpu))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert keep.seq_len == 200       # a replay is the device's work alone
+        assert keep.restore(100) == 0
+        for l in range(2):
+            for kv in (0, 1):
+                whole = src.dequantize(l, kv, 0, 200)
+                assert np.array_equal(a.dequantize(l, kv, 5, 155), whole[:, 10:160])
+                assert np.array_equal(b.dequantize(l, kv, 0, 100), whole[:, step:100 + step])
+                assert np.array_equal(keep.dequantize(l, kv, 0, 100), whole[:, step:100 + step])
+    del g
+    for c in (src, keep, a, b):
+        c.free()
+    assert E.device_status(0) == 0
+
+
+def test_copies_to_256(gpu):
+    src = make(1, 1, 64, 80, 70)
+    dsts = [make(1, 1, 64, 75 + i % 7, 3) for i in range(257)]
+    with pytest.raises(E.EakvError, match="256"):
+        E.copy_positions(dsts, 3, src, 0, 70)
+    E.copy_positions(dsts[:256], 3, src, 0, 70)
+    src.synchronize()
+    want = [src.dequantize(0, kv, 0, 70) for kv in (0, 1)]
+    for d in dsts[:256]:
+        assert d.seq_len == 73
+        assert all(np.array_equal(d.dequantize(0, kv, 3, 73), want[kv]) for kv in (0, 1))
+    assert dsts[256].seq_len == 3
+    for c in dsts + [src]:
+        c.free()
+    assert E.device_status(0) == 0
