@@ -203,9 +203,10 @@ struct ExtWalk {
         it.counter = item;
         left = 0;
       }
-      it.pg0 = r.pg0 + u0 * a.unit_pages;
-      it.npages = min(u1 * a.unit_pages, r.pages) - u0 * a.unit_pages;
-      if (it.npages < 0) it.npages = 0;
+      // the last unit may be half a one: a part behind it starts at the last page's end
+      const int p0 = min(u0 * a.unit_pages, r.pages);
+      it.pg0 = r.pg0 + p0;
+      it.npages = min(u1 * a.unit_pages, r.pages) - p0;
       const bool ok = it.b >= 0 && it.b < a.n_caches && it.h >= 0 && it.h < a.geom.n_heads && it.rows >= 1 &&
                       it.row0 >= 0 && it.pg0 >= 0 && it.pg0 + it.npages <= a.geom.n_pages;
       if (!ok) atomicOr(a.status, kStatusBadIndex);

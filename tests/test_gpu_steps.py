@@ -197,3 +197,30 @@ def test_out_may_be_q(gpu, hd, new, splits, dtype):
     for c in group:
         c.free()
     assert E.device_status(0) == 0
+
+
+@pytest.mark.parametrize("splits", [2, 3, 10])
+@pytest.mark.parametrize("hd,window,size,new,G", [(64, 18, 2598, 349, 3), (128, 100, 448, 260, 2), (64, 0, 64, 60, 3),
+                                                  (128, 1, 577, 513, 1)])
+def test_parts_behind_the_last_page(gpu, hd, window, size, new, G, splits):
+    """A cache filled to its last page, whose last tile has fewer pairs of pages than the others: its
+    empty parts lie behind the pages, and count as empty."""
+    import torch
+    c = E.Cache(1, 1, hd, size)
+    assert c.load_raw(kv_data(np.random.default_rng(size), 1, 1, size, hd), size) == 0
+    assert c.restore(size - new) == 0
+    q = torch.randn(new, G, hd, device=gpu).bfloat16()
+    outs = []
+    for s in (1, splits):
+        for path in (2, 3):
+            out = torch.full_like(q, float("nan"))
+            torch.cuda.synchronize()
+            E.force_splits(s)
+            E.force_path(path)
+            E.extend_attention([c], 0, [new], q, out, window=window)
+            c.synchronize()
+            outs.append(out.float())
+    assert E.device_status(0, reset=True) == 0
+    for o in outs[1:]:
+        assert ((o - outs[0]).abs() <= 2.0 ** -7 * outs[0].abs() + 2.0 ** -7).all()
+    c.free()
