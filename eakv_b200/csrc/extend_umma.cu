@@ -27,10 +27,10 @@
 // first tile (eref) to 2^10. Rows up to 2^4 above it stay in f16's range, and a group's
 // scale is a normal f16 number down to groups 2^-21 of the reference (each factor of two
 // below costs a bit). A run of 32 positions with a row above that, or 2^-10 below the
-// reference, is marked: its rows have powers of their own, which go to the softmax
-// threads beside it, and these scale the scores and the weights column by column, with
-// a V reference of their own per row, taken from attended positions only. So a
-// position that a row does not attend has no influence on it, however large.
+// reference, or with V of zeros, is marked: its rows have powers of their own, which go to
+// the softmax threads beside it, and these scale the scores and the weights column by column, with
+// a V reference of their own per row, taken from attended positions only (of zeros:
+// none). So a position that a row does not attend has no influence on it, however large.
 // (With the reference at 2^0 and high nibbles held times 16 with a sixteenth of the
 // scale, groups 2^-12 of their neighbour lost all but 3 to 5 bits.)
 // Non-finite V groups are kept out of the products (0 NaN is NaN) and
@@ -89,6 +89,7 @@ constexpr int kThreads = (kSoftWarps + kConvWarps + 4) * 32;   // four warpgroup
 constexpr int kRegs = 128, kRegsSoft = 176, kRegsConv = 104, kRegsMma = 56;
 static_assert(2 * kRegsSoft + kRegsConv + kRegsMma == 4 * kRegs, "register split");
 constexpr int kUnset = -100000;
+constexpr int kZeroRow = -1000;               // exponent of a row of zeros, below every other
 constexpr int kTop = 10;                      // a row's values below 2^(e+1) are held below 2^(kTop+1)
 constexpr int kUp = 4, kDown = 10;            // rows within 2^kUp, 2^-kDown of eref need no mark
 static_assert(kTop + 1 + kUp <= 15, "rows without a mark fit f16");
@@ -444,9 +445,13 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         }
         uint32_t kbad, vbad;
         const int ke = row_exp<HD>(kr, kbad), ve = row_exp<HD>(vr, vbad);
+        const int pos = base_pos + i * BN + crow;
+        const bool in = pos >= it.lo && pos < it.hi && pos < end_pos;   // zeros outside are not attended
         const bool mark = __any_sync(0xffffffffu, (ke != kUnset && (ke > kref + kUp || ke < kref - kDown)) ||
-                                                      (ve != kUnset && (ve > vref + kUp || ve < vref - kDown)));
-        const int kx = mark && ke != kUnset ? ke : kref, vx = mark && ve != kUnset ? ve : vref;
+                                                      (ve != kUnset && (ve > vref + kUp || ve < vref - kDown)) ||
+                                                      (ve == kUnset && !vbad && in));
+        const int kx = mark && ke != kUnset ? ke : kref;
+        const int vx = !mark ? vref : ve != kUnset ? ve : kZeroRow;
         // a non-finite K group keeps its NaN, which reaches its own score only; a V
         // group is listed instead
         const uint32_t n0 = __ballot_sync(0xffffffffu, vbad & 1), n1 = __ballot_sync(0xffffffffu, vbad & 2);
@@ -723,14 +728,16 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         const float mx = fmaxf(max3(t[0], t[1], t[2]), t[3]);
         // the maximum of nothing stays -inf (-inf * 0 is NaN)
         const float xm = mx == -INFINITY ? mx : mx * c_row;
-        if (eref == kUnset) eref = vref;
+        // the first positions that the row attends (of each their V is within vref's range)
+        if (eref == kUnset && mx > -INFINITY) eref = vref;
+        const int e_off = eref == kUnset ? 0 : vref - eref;
         if (__any_sync(0xffffffffu, xm > m_run + 8.0f)) {
           float f;
           new_max(xm, f);
           if (i > 0) scale_out(f);
         }
         // the weights carry 2^(vref - eref) whole; the sum takes it off
-        const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run) + (float)(vref - eref);
+        const float off = kPShift - (m_run == -INFINITY ? 0.0f : m_run) + (float)e_off;
         const float2 c2 = make_float2(c_row, c_row), o2 = make_float2(off, off);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -751,7 +758,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
           tmem_st16(ts + 16 * ch, p16);
           if (ch == 1) announce(0);
         }
-        l_run += (sum[0].x + sum[0].y + sum[1].x + sum[1].y) * pow2i(eref - vref);
+        l_run += (sum[0].x + sum[0].y + sum[1].x + sum[1].y) * pow2i(-e_off);
         announce(1);
       };
 
@@ -760,7 +767,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         const int c0 = base_pos + i * BN;
         const short2 *ex = reinterpret_cast<const short2 *>(smem + C::EXPS) + ((all_done + i) % kInfo) * BN;
         float mx = -INFINITY;
-        int emax = kUnset;
+        int emax = kZeroRow;
 #pragma unroll 1
         for (int ch = 0; ch < 4; ch++) {
           uint32_t v[32];
@@ -779,7 +786,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
         }
         float f;
         bool move = new_max(mx == -INFINITY ? mx : mx * c_row, f);
-        if (emax != kUnset && (eref == kUnset || emax > eref)) {
+        if (emax > kZeroRow && (eref == kUnset || emax > eref)) {
           if (eref != kUnset) f *= pow2i(eref - emax);
           eref = emax;
           move = true;
@@ -802,7 +809,7 @@ extend_umma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__
               const bool at = (on >> (e + u)) & 1;
               const float p = at ? ex2(fmaf(__uint_as_float(v[e + u]) * pow2i(x.x - kref), c_row, off)) : 0.0f;
               l_run += p;
-              w[u] = at ? p * pow2i(x.y - eref) : 0.0f;
+              w[u] = at && x.y > kZeroRow ? p * pow2i(x.y - eref) : 0.0f;
             }
             p16[e >> 1] = pack_f16(w[0], w[1]);
           }

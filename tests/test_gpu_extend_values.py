@@ -224,3 +224,32 @@ def test_groups_of_one_value(gpu, level, hd, new, dtype, path):
     meets(gpu, seq, q, dtype, path)
     meets(gpu, seq, q, dtype, path, window=3)
     seq.free()
+
+
+@pytest.mark.parametrize("dtype,path", [("bf16", "umma")])
+@pytest.mark.parametrize("size", [1e-12, 1e-3, 1e12])
+@pytest.mark.parametrize("kind", ["unwritten", "zeros", "one in three", "scattered", "large ones before"])
+@pytest.mark.parametrize("hd,new", [(128, 3), (64, 50), (128, 150)])
+def test_rows_of_zeros_among_values_of_any_size(gpu, hd, new, kind, size, dtype, path):
+    """V rows of zeros, never written or written, in a part's first tile, in runs of 32 and among others,
+    leave values of any size their weights; so do large values before a row's window."""
+    rng = np.random.default_rng(hd + len(kind))
+    d = data(rng, 2, 300 + new, hd, v=size)
+    window = 0
+    segments = [d]
+    if kind == "unwritten":
+        segments = [256, d]
+    elif kind == "zeros":
+        d[1, :, 32:200] = 0
+    elif kind == "one in three":
+        d[1, :, ::3] = 0
+    elif kind == "scattered":
+        d[1, :, rng.integers(0, 300, 5)] = 0
+    else:
+        window = 40
+        d[1, :, :300 + new // 2] *= np.float32(1e15)
+        d[1, :, 260 + new // 2:300 + new // 2] = 0
+    seq = Sequence(2, hd, segments, new)
+    q = rng.standard_normal((new, 4, hd)).astype(np.float32)
+    meets(gpu, seq, q, dtype, path, window)
+    seq.free()
