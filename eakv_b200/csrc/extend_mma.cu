@@ -15,7 +15,7 @@
 // f16 limbs (hi, x - hi: 22 bits of elements down to 2^-11 of the row's largest). p s
 // is one f16 for 16-bit types (2^-12 of each term, below the output's own rounding)
 // and two limbs for f32. Sums of scores, softmax and outputs are f32; the maximum moves
-// lazily, when a score passes it by more than 8 (base 2), so p <= 256.
+// lazily, from below a score to 8 above it (base 2), a whole number, so that p <= 1.
 //
 // Tiles. Both products are transposed, rows the n8 of the instructions: scores
 // S^T[16 positions][8 rows] take K as A operand straight from its bytes (a 32-bit
@@ -122,16 +122,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
-// V-scale references: p s is held times a power of two per group that takes a scale
-// of the reference's size to [2^kRefUp, 2^(kRefUp+1)); a scale that it takes to kRefMost
-// moves it. kRefLeast is the smallest reference (biased exponent) whose power of two and
-// its inverse are both normal numbers. A row's two powers share a word, as the upper
-// halves of their f32.
-constexpr int kRefUp = 4, kRefLeast = 5;
-constexpr float kRefMost = 128.0f;
-__device__ __forceinline__ uint32_t ref_bits(int exponent) {
-  return (uint32_t)(254 + kRefUp - max(exponent, kRefLeast)) << 7;
+// Units of p s. The products of weight and scale of a row and group are held times a power
+// of two that takes the largest of them to [1, 2) when it is set, and keeps it from
+// kRefLeast (above, two f16 limbs hold 22 bits) to below kRefMost later. A row's two powers share a word, as the upper halves of their f32; kPowerMost, the
+// exponent field of the largest power (its inverse is a normal number too), is the first.
+constexpr int kPowerMost = 253;
+constexpr float kRefMost = 16384.0f, kRefLeast = 0.125f;
+template <int NG> __device__ __forceinline__ void set_power(uint32_t &word, int group, int field) {
+  if (NG == 1) word = (uint32_t)field << 23;
+  else if (group == 0) word = (word & 0xFFFF0000u) | (uint32_t)field << 7;
+  else word = (word & 0xFFFFu) | (uint32_t)field << 23;
 }
+// 2^e, 0 below the normal range
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)max(127 + e, 0) << 23); }
 template <int NG> __device__ __forceinline__ float ref_power(uint32_t word, int group) {
   return __uint_as_float(group + 1 < NG ? word << 16 : word & 0xFFFF0000u);
 }
@@ -347,13 +350,15 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
           for (int k = 0; k < 4; k++) o[gg][m][n][k] = 0.0f;
     float m_run[NT][2], l_run[NT][2], pb[NT][2][NG];
-    // The products p s, f16 operands, are held divided by a power of two near the
-    // largest V scale of the group that the row has attended, and the group's o with
-    // them; p itself and the sums l and p b' are not. It moves like the maximum, when a
-    // scale passes it by 2^3, so that p s stays below 2^8 2^7 in its units. It starts
-    // at the smallest that has an inverse: scales below it, denormal ones and zeros,
-    // need no reference of their own. (One for both groups lost bits of the smaller:
-    // with one 2^-16 of the other f32 outputs were off by 2^-9.)
+    // The products p s, f16 operands, are held times a power of two of the row's and
+    // group's own (vref), and the group's o with them; p itself and the sums l and p b' are
+    // not. What sets it is the largest p s that the row has attended, not the largest s: a
+    // weight near 1 on V of zeros, or on V much smaller than the rest, leaves the others their
+    // bits. (One power for both groups lost bits of the smaller: with one 2^-16 of the
+    // other f32 outputs were off by 2^-9.) When the maximum moves, p shrinks by a power of
+    // two, and o with it, or if what moved it has hardly any V, vref grows by it; when p s comes
+    // to kRefMost in these units, vref and o shrink. It starts at the largest: denormal
+    // scales need nothing of their own.
     uint32_t vref[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -361,7 +366,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       for (int e = 0; e < 2; e++) {
         m_run[n][e] = -INFINITY;
         l_run[n][e] = 0.0f;
-        vref[n][e] = ref_bits(kRefLeast) * 0x10001u;
+        vref[n][e] = (uint32_t)(kPowerMost << 7) * 0x10001u;
 #pragma unroll
         for (int gg = 0; gg < NG; gg++) pb[n][e][gg] = 0.0f;
       }
@@ -456,11 +461,9 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
       float sv[J][NG], bv[J][NG];
       scales(vsm + C::NIB, p0, true, sv, bv);
       // ---- online softmax, base 2, lazy maximum -----------------------------------
-      // A row moves when a score passes its maximum by 8, or a V scale that it
-      // attends its group's reference by 2^3 (scales are negative only in damaged
-      // files; NaN is passed over).
+      // (Scales are negative only in damaged files; NaN is passed over.)
       bool move = false;
-      float lm[NT][2], sx[NT][2][NG];
+      float lm[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -468,17 +471,39 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
           lm[n][e] = sc[n][e][0];
 #pragma unroll
           for (int j = 1; j < J; j++) lm[n][e] = fmaxf(lm[n][e], sc[n][e][j]);
-          move = move || lm[n][e] > m_run[n][e] + 8.0f;
+          move = move || lm[n][e] > m_run[n][e];
 #pragma unroll
-          for (int gg = 0; gg < NG; gg++) {
-            sx[n][e][gg] = FULL ? page_s[gg] : 0.0f;
+          for (int gg = 0; gg < NG; gg++) {   // p is at most 1
+            float s = FULL ? page_s[gg] : 0.0f;
 #pragma unroll
             for (int j = 0; j < J; j++)
-              if (!FULL && on[n][e][j]) sx[n][e][gg] = fmaxf(sx[n][e][gg], fabsf(sv[j][gg]));
-            move = move || sx[n][e][gg] * ref_power<NG>(vref[n][e], gg) >= kRefMost;
+              if (!FULL && on[n][e][j]) s = fmaxf(s, fabsf(sv[j][gg]));
+            move = move || s * ref_power<NG>(vref[n][e], gg) >= kRefMost;
           }
         }
       if (__any_sync(0xffffffffu, move)) {
+        // largest p s of the lane's positions, without infinite scales
+        auto most = [&](int n, int e, int gg) {
+          const float m = m_run[n][e] == -INFINITY ? 0.0f : m_run[n][e];
+          float y = 0.0f;
+#pragma unroll
+          for (int j = 0; j < J; j++) {
+            const float s = fabsf(sv[j][gg]);
+            if ((FULL || on[n][e][j]) && s < INFINITY) y = fmaxf(y, ex2(sc[n][e][j] - m) * s);
+          }
+          return y;
+        };
+        auto scale_out = [&](int gg, int n, int e, float f) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            o[gg][k][n][e] *= f;
+            o[gg][k][n][2 + e] *= f;
+          }
+        };
+        // per row and group: p s too large for its units (lower bits), large enough (upper)
+        static_assert(2 * NT * NG <= 16, "room for the bits");
+        uint32_t bits = 0;
+        int d[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -486,46 +511,62 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
             float t = lm[n][e];
 #pragma unroll
             for (int b = 4; b < 32; b <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
-            const bool mv = t > m_run[n][e] + 8.0f;
-            const float alpha = mv ? ex2(m_run[n][e] - t) : 1.0f;
-            if (mv) {
+            d[n][e] = 0;
+            if (t > m_run[n][e]) {
+              t = ceilf(t) + 8.0f;
+              d[n][e] = (int)fminf(t - m_run[n][e], 1000.0f);   // from -inf: sums of nothing
               m_run[n][e] = t;
-              l_run[n][e] *= alpha;
+              l_run[n][e] *= pow2i(-d[n][e]);
             }
-            uint32_t word = 0;
 #pragma unroll
             for (int gg = 0; gg < NG; gg++) {
-              const float was = ref_power<NG>(vref[n][e], gg);
-              float x = sx[n][e][gg], down = alpha;
-              if (!FULL) {
-                if (x == INFINITY) {   // without the infinite ones
-                  x = 0.0f;
-#pragma unroll
-                  for (int j = 0; j < J; j++)
-                    if (on[n][e][j] && fabsf(sv[j][gg]) < INFINITY) x = fmaxf(x, fabsf(sv[j][gg]));
-                }
-#pragma unroll
-                for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
-              }
-              uint32_t half = __float_as_uint(was) >> 16;
-              if (x * was >= kRefMost) {
-                half = ref_bits(__float_as_uint(x) >> 23);
-                // times the new power and the inverse of the old
-                down *= __uint_as_float(half << 16) *
-                        __uint_as_float((254u << 23) - __float_as_uint(was));
-              }
-              word |= half << (gg + 1 < NG ? 0 : 16);
-              if (down != 1.0f) {
-#pragma unroll
-                for (int m = 0; m < 4; m++) {
-                  o[gg][m][n][e] *= down;
-                  o[gg][m][n][2 + e] *= down;
-                }
-              }
-              if (mv) pb[n][e][gg] *= alpha;
+              const float v = most(n, e, gg) * ref_power<NG>(vref[n][e], gg);
+              const int k = (2 * n + e) * NG + gg;
+              bits |= (v >= kRefMost ? 1u << k : 0u) | (v >= kRefLeast ? 0x10000u << k : 0u);
             }
-            vref[n][e] = word;
           }
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, b);
+        bool again = (bits & 0xFFFFu) != 0;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            if (d[n][e] > 0) {
+#pragma unroll
+              for (int gg = 0; gg < NG; gg++) {
+                const float alpha = pow2i(-d[n][e]);
+                pb[n][e][gg] *= alpha;
+                if (bits & (0x10000u << ((2 * n + e) * NG + gg))) {
+                  scale_out(gg, n, e, alpha);
+                } else {   // the new largest weight stands on hardly any V
+                  const int was = (int)(__float_as_uint(ref_power<NG>(vref[n][e], gg)) >> 23);
+                  const int now = min(was + d[n][e], kPowerMost);
+                  set_power<NG>(vref[n][e], gg, now);
+                  scale_out(gg, n, e, pow2i(now - was - d[n][e]));
+                  again = true;
+                }
+              }
+            }
+        if (__any_sync(0xffffffffu, again)) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+              for (int gg = 0; gg < NG; gg++) {
+                float y = most(n, e, gg);
+#pragma unroll
+                for (int b = 4; b < 32; b <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, b));
+                const float f = ref_power<NG>(vref[n][e], gg);
+                if (y * f >= kRefMost) {
+                  const int was = (int)(__float_as_uint(f) >> 23);
+                  const int now = min(max(254 - (int)(__float_as_uint(y) >> 23), 1), kPowerMost);
+                  set_power<NG>(vref[n][e], gg, now);
+                  scale_out(gg, n, e, pow2i(now - was));
+                }
+              }
+        }
       }
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -550,7 +591,7 @@ extend_mma_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               // what is not attended adds nothing, whatever its scale and bias are
-              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * (sv[j][gg] * ref_power<NG>(vref[n][e], gg)) : 0.0f;
+              x[e] = (FULL || on[n][e][j]) ? sc[n][e][j] * sv[j][gg] * ref_power<NG>(vref[n][e], gg) : 0.0f;
               if (FULL || on[n][e][j]) pb[n][e][gg] = fmaf(sc[n][e][j], bv[j][gg], pb[n][e][gg]);
             }
             const uint32_t h = pack_f16(x[0], x[1]);

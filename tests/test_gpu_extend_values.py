@@ -226,7 +226,7 @@ def test_groups_of_one_value(gpu, level, hd, new, dtype, path):
     seq.free()
 
 
-@pytest.mark.parametrize("dtype,path", [("bf16", "umma")])
+@pytest.mark.parametrize("dtype,path", [k for k in KINDS if k[0] != "f16"])
 @pytest.mark.parametrize("size", [1e-12, 1e-3, 1e12])
 @pytest.mark.parametrize("kind", ["unwritten", "zeros", "one in three", "scattered", "large ones before"])
 @pytest.mark.parametrize("hd,new", [(128, 3), (64, 50), (128, 150)])
