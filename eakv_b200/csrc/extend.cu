@@ -28,12 +28,12 @@ constexpr int kPartPagesF32 = 64, kPartPages16 = 1024;
 
 // Rows (new tokens x query heads per KV head) up to which 16-bit calls take the
 // warp-level kernel. 16 caches of 8192 positions, 8 KV heads of 128: at 24, 32, 40, 64
-// rows 104, 128, 171, 249 us, the tcgen05 kernel 169, 170, 170, 169; head_dim 64 at
-// 32, 40, 64 rows 79, 107, 157 against 118, 119, 118; 64 caches of 512 positions 68,
-// 103, 152 against 95, 95, 95.
+// rows 112, 128, 173, 256 us, the tcgen05 kernel 171 each; head_dim 64 at 32, 40, 64
+// rows 81, 107, 160 against 118, 120, 120; 64 caches of 512 positions 73, 112, 166
+// against 99 each.
 constexpr int kMmaRows = 32;
 // A page's time for tiles of 8, 16 and 24 rows of the warp-level kernel, 16-bit
-// types: 16 caches of 8192 positions (8 KV heads of 128) took 56, 78 and 104 us with
+// types: 16 caches of 8192 positions (8 KV heads of 128) took 58, 81 and 112 us with
 // one tile each, 15 us of it set-up. A second tile of 8 rows costs as much again (84
 // us), so 16 rows go to one tile, 17 to 24 to one of 24. In f32 the two limbs double
 // the operands and larger tiles lose: 104 rows per head (13, 7, 5 tiles) 73, 78, 86 us.

@@ -25,13 +25,13 @@
 // per group and 16 positions, and the weights as B operand by one transposition of
 // 8 x 8 pairs (movmatrix). So a page is converted once for a tile, and a tile of few
 // rows costs few products: with rows as the m16 one token of four heads behind each
-// of 16 x 8192 positions took 71 us, transposed 56. Each warp takes whole pages in
+// of 16 x 8192 positions took 71 us, transposed 55. Each warp takes whole pages in
 // turn; the page ring, its waits and the split merge are those of the decode kernels.
 //
 // Bound: the chain of a step's dependent instructions (two to four warps per
 // scheduler, as the registers allow), and the set-up and merge of an item, about 15
-// us. 16 caches of 8192 positions (168 MB, 26 us at HBM's rate): 56 us for 8 rows,
-// 78 for 16, 104 for 24.
+// us. 16 caches of 8192 positions (168 MB, 26 us at HBM's rate): 58 us for 8 rows,
+// 81 for 16, 112 for 24.
 #include <math.h>
 
 #include <atomic>

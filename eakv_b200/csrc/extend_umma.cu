@@ -53,8 +53,8 @@
 //
 // Bound: the tensor pipe, whose operands come from shared memory at its full rate
 // (S = Q'K' reads 128 bytes a cycle) next to the dequantizing stores: 2048 tokens
-// of 32 heads (8 KV heads, head_dim 128) behind 32768 positions in 1.15 to 1.24 ms,
-// 0.91 to 0.99 PFLOP/s, box to box. Tried and slower: tiles of 64 positions with two S buffers (its
+// of 32 heads (8 KV heads, head_dim 128) behind 32768 positions in 1.19 to 1.24 ms,
+// 0.92 to 0.95 PFLOP/s, box to box. Tried and slower: tiles of 64 positions with two S buffers (its
 // MMAs are 1.4 times slower per value), one pass over the scores in place of the
 // registers, exponentials by polynomial on the FMA pipe for a quarter or half of
 // them (the exponentials are not what it waits for).
