@@ -122,10 +122,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
-// Units of p s. The products of weight and scale of a row and group are held times a power
-// of two that takes the largest of them to [1, 2) when it is set, and keeps it from
-// kRefLeast (above, two f16 limbs hold 22 bits) to below kRefMost later. A row's two powers share a word, as the upper halves of their f32; kPowerMost, the
-// exponent field of the largest power (its inverse is a normal number too), is the first.
+// Units of p s. The products of weight and scale of a row and group are held times a
+// power of two that takes the largest of them to [1, 2) when it is set, and keeps it from
+// kRefLeast (above, two f16 limbs hold 22 bits) to below kRefMost later. A row's two
+// powers share a word, as the upper halves of their f32. kPowerMost, the exponent field
+// of the largest power (its inverse is a normal number too), is the first.
 constexpr int kPowerMost = 253;
 constexpr float kRefMost = 16384.0f, kRefLeast = 0.125f;
 template <int NG> __device__ __forceinline__ void set_power(uint32_t &word, int group, int field) {

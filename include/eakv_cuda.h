@@ -254,16 +254,15 @@ int eakv_append_rotary(eakv_cache_t *const *caches, int n_caches, int layer, con
  * 1/sqrt(head_dim) when given as 0; lse (device f32[total tokens][n_q_heads],
  * or NULL) the natural-log log-sum-exp of the scaled scores. A token that
  * attends nothing gets zeros and -inf. What is not attended has no influence,
- * NaN among it. q and out have one element type, and out may be q itself (an
- * item's rows are read by all its parts before one of them is written); sums
- * are f32. f32 runs on
+ * NaN among it. q and out have one element type, and out may be q itself (a
+ * row is read by all its parts before it is written). Sums are f32. f32 runs on
  * split operands that keep 22 bits, at any number of rows; a 16-bit type on one
  * f16 operand each: with up to 32 rows (new tokens x query heads) per KV head
  * the cache's values enter exactly, with more each is rounded to f16, which puts
  * f16 outputs 0.7e-3 of their size off in the mean (0.3e-3 with few rows) and
- * bf16 ones 1.8e-3, of which 1.7e-3 are the output's own rounding. A caller who needs more bits there
- * passes f32 rows. workspace (device, 16-byte aligned) holds the records of long rows'
- * sequence splits: at least eakv_extend_workspace bytes, zeroed once before
+ * bf16 ones 1.8e-3, of which 1.7e-3 are the output's own rounding. A caller who
+ * needs more bits there passes f32 rows. workspace (device, 16-byte aligned)
+ * holds the records of long rows' sequence splits: at least eakv_extend_workspace bytes, zeroed once before
  * its first use, and not shared by calls that may overlap; NULL takes one that
  * the first cache keeps for this call, which then must not be in use on another
  * stream. A captured call takes a workspace of its own, since the cache's moves
